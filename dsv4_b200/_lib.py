@@ -29,6 +29,7 @@ ERRORS = {
     5: "scheduler row scan overran its cap",
     6: "request exceeds the fixed scratch of the allocation-free scheduler",
     7: "block-table entry outside the table or the pool (rows dropped)",
+    8: "position outside the cos / sin tables (nearest row used)",
 }
 STATUS_BAD_BLOCK_ENTRY = 7
 STATUS_TIMEOUT_BASE = 16
@@ -56,6 +57,15 @@ EXPORTS = {
                                       i32, vp, i64, i32, vp, i32, vp, i32, vp, f32, i32, i32, i32, vp, vp, vp, vp,
                                       vp, vp], ctypes.c_int),
     "sas_bwd_cast": ([vp, vp, i64, i32, vp], ctypes.c_int),
+    "sas_head_norm_rope_fwd": ([vp, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, vp,
+                                vp, vp, i32, i32, vp, vp, f32, i32, vp, vp], ctypes.c_int),
+    "sas_head_norm_rope_bwd_workspace_bytes": ([i32], sz),
+    "sas_head_norm_rope_bwd": ([vp, i64, i64, vp, i64, i64, vp, i32, vp, i64, i64, vp, i64, i64, vp, i32, i32, i32,
+                                i32, vp, vp, vp, i32, i32, vp, vp, vp, vp, f32, i32, vp, vp, sz, vp], ctypes.c_int),
+    "sas_append_sharedkv": ([vp, i64, vp, i64, i32, vp, i32, vp, vp, i32, i32, i32, vp, i64, i64, vp, i64, i64, i32,
+                             i32, i32, i32, vp, vp, vp, i32, i32, vp, vp, f32, i32, vp, vp], ctypes.c_int),
+    "sas_append_sharedkv_bwd": ([vp, i64, i32, vp, i32, vp, vp, i32, i32, i32, vp, i64, vp, i32, i32, i32, vp, vp,
+                                 vp, i32, i32, vp, vp, f32, i32, vp, vp, sz, vp], ctypes.c_int),
     "sas_fwd_workspace_bytes": ([i32, i32, i32], sz),
     "sas_fwd_set_option": ([i32, ctypes.c_double, vp], ctypes.c_int),
     "sas_sparse_attn_sharedkv_fwd": ([vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, i64, i32, vp, i32, vp, i64,

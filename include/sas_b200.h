@@ -34,6 +34,8 @@ extern "C" {
 #define SAS_ERR_BAD_BLOCK_ENTRY 7 /* device status, non-fatal: a block-table column past the table's width
                                      (seqused_kv longer than the table) or an entry >= the pool's block
                                      count was met; those rows were dropped like -1 entries */
+#define SAS_ERR_BAD_POSITION 8    /* device status, non-fatal: a position outside the cos / sin tables (the nearest
+                                     row was used) */
 #define SAS_ERR_TIMEOUT_BASE 16  /* device status: 16 + id of the bounded wait that ran out */
 
 #define SAS_META_SIZE 1024
@@ -235,6 +237,69 @@ int sas_sparse_attn_sharedkv_bwd(
     int32_t ori_win_left, int32_t scenario, void* dq, float* d_ori_kv, float* d_cmp_kv, float* d_sinks,
     int32_t* status, void* stream);
 int sas_bwd_cast(const float* src, void* dst, int64_t n, int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * RMS norm of each head with the position rotation of its last R dims, in one
+ * pass (no counterpart in the reference, whose op takes rotated q and KV):
+ *   y = Rot(pos) (x * w / sqrt(mean(x^2) + eps)),
+ * fp32 inside, rounded once. Rows are q [T, H, D] and optionally k [T, Hk, D]
+ * (Hk = 0: none) in the I/O type, D a multiple of 8 up to 1024, the last dim
+ * contiguous; *_ts / *_hs are the token and head strides in elements,
+ * multiples of 8, and every pointer is 16-byte aligned. y may be x. cos and sin
+ * are fp32 [P, R/2]; R = 0 leaves out the rotation, else R is a multiple of 8
+ * (SAS_ROPE_INTERLEAVED) or 16. positions [T] are int32, or int64 with
+ * SAS_ROPE_POS64. Weights are fp32 [D] or NULL.
+ * The backward takes dy (dq_out, dk_out) and x and writes dense dq [T, H, D],
+ * dk [T, Hk, D] in the I/O type and, where dq_weight / dk_weight are given,
+ * the weights' gradients in fp32 (summed in a fixed order; needs the
+ * workspace, which may be NULL otherwise).
+ * ---------------------------------------------------------------------- */
+#define SAS_ROPE_NORM 1        /* divide by the root mean square (else weights must be NULL) */
+#define SAS_ROPE_INVERSE 2     /* turn by the negative angle */
+#define SAS_ROPE_INTERLEAVED 4 /* pairs are neighbouring dims (else dims i and i + R/2 of the rotated part) */
+#define SAS_ROPE_POS64 8
+int sas_head_norm_rope_fwd(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                           int32_t H, const void* k, int64_t k_ts, int64_t k_hs, void* k_out, int64_t ko_ts,
+                           int64_t ko_hs, int32_t Hk, int32_t T, int32_t D, int32_t dtype, const void* positions,
+                           const float* cos, const float* sin, int32_t P, int32_t R, const float* q_weight,
+                           const float* k_weight, float eps, int32_t flags, int32_t* status, void* stream);
+size_t sas_head_norm_rope_bwd_workspace_bytes(int32_t D);
+int sas_head_norm_rope_bwd(const void* dq_out, int64_t dqo_ts, int64_t dqo_hs, const void* q, int64_t q_ts,
+                           int64_t q_hs, void* dq, int32_t H, const void* dk_out, int64_t dko_ts, int64_t dko_hs,
+                           const void* k, int64_t k_ts, int64_t k_hs, void* dk, int32_t Hk, int32_t T, int32_t D,
+                           int32_t dtype, const void* positions, const float* cos, const float* sin, int32_t P,
+                           int32_t R, const float* q_weight, const float* k_weight, float* dq_weight,
+                           float* dk_weight, float eps, int32_t flags, int32_t* status, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Append of the new tokens' shared K=V rows to a paged cache, with the same
+ * norm and rotation on the way, and optionally their queries (H > 0) in the
+ * same launch. Token i of the n new ones of request b goes to slot
+ * seqused_kv[b] - n + i, as the attention reads it; the slot is the position
+ * too unless `positions` gives one for every token (drafted trees). A token
+ * whose block-table entry is negative, or that lies before slot 0, is not
+ * written; one past the table's width or the pool is not written and recorded
+ * as SAS_ERR_BAD_BLOCK_ENTRY. kv [T, D] has token stride kv_ts. No two tokens
+ * may share a slot. Layouts as in the attention: TND with cu_seqlens_q [B+1],
+ * BSND with S tokens per request (cu_seqlens_q then optional).
+ * The backward gathers dy from the cache's gradient (I/O type, shaped like
+ * the pool) and writes dense dkv [T, D]; tokens that were not written get 0.
+ * ---------------------------------------------------------------------- */
+int sas_append_sharedkv(const void* kv, int64_t kv_ts, void* pool, int64_t num_blocks, int32_t block_size,
+                        const int32_t* block_table, int32_t table_stride, const int32_t* cu_seqlens_q,
+                        const int32_t* seqused_kv, int32_t batch, int32_t max_seqlen_q, int32_t layout_q,
+                        const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                        int32_t H, int32_t T, int32_t D, int32_t dtype, const void* positions, const float* cos,
+                        const float* sin, int32_t P, int32_t R, const float* kv_weight, const float* q_weight,
+                        float eps, int32_t flags, int32_t* status, void* stream);
+int sas_append_sharedkv_bwd(const void* d_pool, int64_t num_blocks, int32_t block_size, const int32_t* block_table,
+                            int32_t table_stride, const int32_t* cu_seqlens_q, const int32_t* seqused_kv,
+                            int32_t batch, int32_t max_seqlen_q, int32_t layout_q, const void* kv, int64_t kv_ts,
+                            void* dkv, int32_t T, int32_t D, int32_t dtype, const void* positions, const float* cos,
+                            const float* sin, int32_t P, int32_t R, const float* kv_weight, float* dkv_weight,
+                            float eps, int32_t flags, int32_t* status, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* ------------------------------------------------------------------------
  * Process-wide options of the forward kernel (no counterpart in the
