@@ -9,7 +9,8 @@ and the backward the reference documents but does not ship
 (``sparse_attn_sharedkv_backward``, ``sparse_attn_sharedkv_train``).
 
 What fills their inputs is in ``rope``: head norm with rotation
-(``head_norm_rope``) and the append to the paged cache (``append_shared_kv``).
+(``head_norm_rope``) and the append to the paged cache (``append_shared_kv``);
+``tree`` has the attention of drafted trees (``tree_attn_sharedkv``).
 
 All run hand-written sm_100a kernels from ``libsas_b200.so`` (C ABI in
 ``include/sas_b200.h``). ``sharding`` holds the request-parallel and
@@ -27,6 +28,7 @@ from .rope import (  # noqa: F401
     head_norm_rope_train,
 )
 from .metadata import SAS_META_SIZE, sparse_attn_sharedkv_metadata  # noqa: F401
+from .tree import tree_attn_sharedkv  # noqa: F401
 from ._lib import check_device_status, device_status, reset_device_status  # noqa: F401
 
 __all__ = [
@@ -41,6 +43,7 @@ __all__ = [
     "HeadNormRope",
     "append_shared_kv",
     "append_shared_kv_backward",
+    "tree_attn_sharedkv",
     "SAS_META_SIZE",
     "check_device_status",
     "device_status",

@@ -30,6 +30,7 @@ ERRORS = {
     6: "request exceeds the fixed scratch of the allocation-free scheduler",
     7: "block-table entry outside the table or the pool (rows dropped)",
     8: "position outside the cos / sin tables (nearest row used)",
+    9: "draft tree with a bad parent, over 1024 tokens or more tokens than seqused_kv (outputs zero)",
 }
 STATUS_BAD_BLOCK_ENTRY = 7
 STATUS_TIMEOUT_BASE = 16
@@ -66,6 +67,9 @@ EXPORTS = {
                              i32, i32, i32, vp, vp, vp, i32, i32, vp, vp, f32, i32, vp, vp], ctypes.c_int),
     "sas_append_sharedkv_bwd": ([vp, i64, i32, vp, i32, vp, vp, i32, i32, i32, vp, i64, vp, i32, i32, i32, vp, vp,
                                  vp, i32, i32, vp, vp, f32, i32, vp, vp, sz, vp], ctypes.c_int),
+    "sas_tree_attn_workspace_bytes": ([i32], sz),
+    "sas_tree_attn_sharedkv": ([vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i64, i32, vp, i32, vp, i64, i32,
+                                vp, i32, vp, i32, vp, f32, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp], ctypes.c_int),
     "sas_fwd_workspace_bytes": ([i32, i32, i32], sz),
     "sas_fwd_set_option": ([i32, ctypes.c_double, vp], ctypes.c_int),
     "sas_sparse_attn_sharedkv_fwd": ([vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp, i64, i32, vp, i32, vp, i64,

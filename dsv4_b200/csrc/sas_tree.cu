@@ -1,0 +1,868 @@
+// Attention of drafted tokens that form a tree over the paged shared-KV caches (sm_100a).
+//
+// A request's n drafted tokens sit in the window cache at slots [ctx, ctx + n)
+// (ctx = seqused_kv - n); parents[i] < i is the token that i follows, -1 the
+// cached context, anything below an unused slot. Token i at depth d has
+// position s = ctx + d and attends to
+//   the cached rows [s - win, ctx), its ancestors no more than win back, itself;
+//   compressed rows below ctx // ratio: all of them, or its top-k list.
+// o = sum_j p_j v_j / (sum_j p_j + e^sink),  p_j = e^(scale q.k_j),  K = V.
+//
+// Work: one unit is 64 (token, head) rows of one request, in order, so a
+// request's units read the same rows; with top-k lists a unit is 64 heads of
+// one token. A unit's rows of KV come in tiles of 128: the window (cached and
+// drafted rows together), then the compressed ones. All tiles of all units
+// form one sequence that is cut into equal ranges, one per CTA; a unit cut by
+// a range's end leaves partial sums that tree_combine_kernel joins in order.
+//
+// Per tile, S[64 x 128] = Q K^T and O[64 x 512] += P V are tcgen05.mma.ws with
+// M = 64: weight-stationary because its M = 64 accumulators use all 128 TMEM
+// lanes (lanes 64-127 hold the upper half of the columns), so O takes 256
+// columns and the next scores fit beside it, and because it runs at 0.66
+// (N = 128) to 0.80 (N = 256) of the full rate where plain M = 64 stops at 0.5
+// (48.2 and 80.2 cycles measured). A tile's 128 KB are resident once and read
+// as K (K-major) and as V (MN-major). The softmax is one pass with a running
+// maximum that moves, and rescales O, only when a row's maximum rises by more
+// than 2^8: P then stays below 2^8, and P, l and O keep one common scale.
+// P is rounded to the I/O type for the product, l sums it unrounded (as the
+// framework's forward does).
+//
+// Roles (14 warps): 0-3 softmax and epilogue (thread = row, half of the tile's
+// columns), 4 MMA issuer, 5 coordinator (walks the range and the trees and
+// publishes tiles in a ring), 6-13 loaders (cp.async, 16 rows of a tile each).
+#include "sas_common.cuh"
+
+namespace {
+
+constexpr int D = 512;
+constexpr int MR = 64;    // rows of a unit
+constexpr int CH = 128;   // KV rows of a tile
+constexpr int kMaxTok = 8;      // tokens of a unit: heads are a multiple of 8
+constexpr int kMaxTree = 1024;  // drafted tokens of a request
+constexpr int kWords = kMaxTree / 32;
+constexpr int kMaxCtx = 1 << 30;  // rows cached before them
+constexpr int SLAB = CH * 128;    // 64 columns of a tile
+constexpr int QSLAB = MR * 128;   // 64 columns of Q, or 64 rows' P
+constexpr int kMmaWarp = 4, kCoordWarp = 5, kLoadWarp0 = 6, kLoadWarps = 8;
+constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
+constexpr int kRing = 4;          // tiles the coordinator may be ahead
+constexpr int kUnitSlots = 6;     // > kRing + 1: no slot is rewritten while a published tile names it
+constexpr uint32_t TM_O = 0, TM_S = 256, TM_COLS = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kMove = 8.f;      // log2 units the running maximum may lag
+
+constexpr int OFF_Q = 0;
+constexpr int OFF_KV = OFF_Q + 8 * QSLAB;
+constexpr int OFF_P = OFF_KV + 8 * SLAB;
+constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
+
+enum Bar { B_FULL = 0, B_EMPTY = 2, B_QFULL = 4, B_QEMPTY, B_VFULL, B_SFULL, B_PREADY, B_OFULL, B_OEMPTY, B_SSYNC,
+           B_CFULL, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
+
+enum TileFlag : int {
+  TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
+  TF_CMP = 16, TF_TOPK = 32, TF_PART0 = 64, TF_PART1 = 128  // PARTn: the piece goes to the CTA's partial n
+};
+
+struct Tile { int flags, row0, nrows, uslot; };
+struct Unit {
+  int b, tok, ctx, thr;      // tok: first token
+  int64_t qrow;              // first row of [T * H]
+  int nrows, roff;           // roff: head of the first row
+  int pos[kMaxTok];          // s of each token, -1: unused
+  uint32_t bits[kMaxTok][kWords];  // drafted rows each token sees
+};
+struct Cut {  // the piece a CTA's range starts with, when it is not its unit's first
+  int64_t ustart, uend, qrow;
+  int nrows, cut;
+};
+struct Misc {
+  uint64_t bars[B_COUNT + (B_COUNT & 1)];
+  sas::CtaCtl ctl;
+  uint32_t tmem;
+  int start_b;
+  int64_t start_prefix, total;
+  int64_t wsum[kThreads / 32];
+  uint32_t vmask[4];
+  float red[3][128];  // row maxima of even and odd tiles, row sums of a unit
+  Tile ring[kRing];
+  Unit units[kUnitSlots];
+  int parents[kMaxTree];
+};
+constexpr int SMEM_BYTES = OFF_MISC + (int)sizeof(Misc) + 1024;
+static_assert(SMEM_BYTES <= 232448, "shared memory over the per-CTA limit");
+
+constexpr size_t kPieceFloats = (size_t)MR * D + 2 * MR;  // O, m (log2 units), l
+
+struct TreeParams {
+  const uint8_t* q;
+  uint8_t* out;
+  float* lse;
+  int T, H, G, R, scenario, K, ratio, win, B, S, layout, split;
+  const int32_t* cu;
+  const int32_t* seqused;
+  const int32_t* parents;
+  const uint8_t* kv[2];  // window pool, compressed pool
+  const int32_t* bt[2];
+  int bs[2], bt_stride[2];
+  int64_t nblk[2];
+  const int32_t* idx;
+  const float* sinks;
+  float scale_log2;
+  float* part;  // [CTAs][2] pieces
+  Cut* cuts;    // [CTAs]
+  int64_t* total;
+  int32_t* status;
+};
+
+// What a request brings: its tokens, and the tiles of each of its units.
+struct Req {
+  int base, slots, n, ctx, thr, units, wtiles, tiles;
+  bool bad;
+  __device__ __forceinline__ int64_t all() const { return (int64_t)units * tiles; }
+};
+__device__ Req request(const TreeParams& p, int b) {
+  Req r;
+  if (p.layout == SAS_LAYOUT_TND) {
+    const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
+    r.base = min(max(c0, 0), p.T);
+    r.n = r.slots = max(min(c1, p.T) - r.base, 0);
+  } else {
+    r.base = b * p.S;
+    r.slots = p.S;
+    r.n = p.cu ? min(max(__ldg(p.cu + b + 1) - __ldg(p.cu + b), 0), p.S) : p.S;
+  }
+  r.ctx = __ldg(p.seqused + b) - r.n;
+  r.bad = r.n > kMaxTree || r.ctx < 0 || r.ctx > kMaxCtx;
+  r.thr = p.scenario == 1 || r.bad ? 0 : r.ctx / p.ratio;
+  r.units = p.scenario == 3 ? r.slots : (int)(((int64_t)r.slots * p.H + MR - 1) / MR);
+  r.wtiles = r.bad || r.n == 0 ? 1 : (min(r.ctx, p.win) + r.n + CH - 1) / CH;
+  r.tiles = r.wtiles + (r.bad || r.n == 0 ? 0 : p.scenario == 2 ? (r.thr + CH - 1) / CH : p.scenario == 3 && r.thr > 0 ? (p.K + CH - 1) / CH : 0);
+  return r;
+}
+__device__ __forceinline__ int64_t range_start(int64_t total, int R, int r) { return total * r / R; }
+// CTAs (per head group) that share the sequence; every range has a tile
+__device__ __forceinline__ int ranges(int64_t total, int R) { return (int)max((int64_t)1, min((int64_t)R, total)); }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sas::smem_u32(bar)) : "memory");
+}
+// D[tmem] (+)= A B^T, M = 64, weight-stationary
+__device__ __forceinline__ void umma_ws(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.ws.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (DT == SAS_DTYPE_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return reinterpret_cast<const uint32_t&>(v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+__device__ __forceinline__ void bad(const TreeParams& p, int code) {
+  if (p.status) atomicCAS(p.status, 0, code);
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
+// The 32 rows from position p0 that a token at position s sees: the cached
+// ones of its window, then the drafted ones of its bitmap.
+__device__ __forceinline__ uint32_t window_bits(int p0, int s, int win, int ctx, const uint32_t* bits) {
+  const int c = ctx - p0;  // cached rows before the drafted ones
+  uint32_t m = low_bits(c) & ~low_bits(s - win - p0);
+  if (c <= 0) {
+    const int j = -c, w = j >> 5, o = j & 31;
+    if (w < kWords) m = __funnelshift_r(bits[w], w + 1 < kWords ? bits[w + 1] : 0u, o);
+  } else if (c < 32) {
+    m |= bits[0] << c;
+  }
+  return m;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_constant__ TreeParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  Misc& ms = *reinterpret_cast<Misc*>(smem + OFF_MISC);
+  uint64_t* bars = ms.bars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = blockIdx.x % p.G, rank = blockIdx.x / p.G;
+  if (tid == 0) {
+    for (int h = 0; h < 2; ++h) {
+      sas::mbar_init(&bars[B_FULL + h], 32 * kLoadWarps);
+      sas::mbar_init(&bars[B_EMPTY + h], 1);
+    }
+    sas::mbar_init(&bars[B_QFULL], 32 * kLoadWarps);
+    sas::mbar_init(&bars[B_QEMPTY], 1);
+    sas::mbar_init(&bars[B_VFULL], kLoadWarps);
+    sas::mbar_init(&bars[B_SFULL], 1);
+    sas::mbar_init(&bars[B_PREADY], 128);
+    sas::mbar_init(&bars[B_OFULL], 1);
+    sas::mbar_init(&bars[B_OEMPTY], 128);
+    sas::mbar_init(&bars[B_SSYNC], 128);
+    for (int i = 0; i < kRing; ++i) {
+      sas::mbar_init(&bars[B_CFULL + i], 1);
+      sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + 4);
+    }
+    sas::mbar_init(&bars[B_DRAIN], 1);
+    sas::fence_mbar_init();
+    ms.ctl.abort = 0;
+    ms.ctl.limit_ns = SAS_WAIT_LIMIT_NS;
+    ms.start_b = p.B;
+    ms.start_prefix = 0;
+  }
+  if (warp == kMmaWarp) {
+    sas::tmem_alloc(&ms.tmem, TM_COLS);
+    sas::tmem_relinquish();
+  }
+  // every thread takes a run of requests; a block scan of their tiles gives the
+  // sequence's length and the request that this CTA's range starts in
+  const int per = (p.B + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += request(p, b).all();
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) ms.wsum[warp] = incl;
+  sas::tc_fence_before();
+  __syncthreads();
+  sas::tc_fence_after();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += ms.wsum[w];
+    total += ms.wsum[w];
+  }
+  const int R = ranges(total, p.R);
+  const int64_t t0 = rank < R ? range_start(total, R, rank) : total;
+  const int64_t t1 = rank < R ? range_start(total, R, rank + 1) : total;
+  {
+    int64_t at = before + incl - mine;
+    for (int b = b0; b < b1; ++b) {
+      const int64_t a = request(p, b).all();
+      if (t0 >= at && t0 < at + a) ms.start_b = b, ms.start_prefix = at;
+      at += a;
+    }
+  }
+  if (p.layout == SAS_LAYOUT_TND) {  // rows that no request holds are zero
+    const int64_t lo = (int64_t)min(max(__ldg(p.cu), 0), p.T) * p.H, hi = (int64_t)min(max(__ldg(p.cu + p.B), 0), p.T) * p.H;
+    const int64_t all = (int64_t)p.T * p.H;
+    for (int64_t r = blockIdx.x; r < all; r += gridDim.x) {
+      if (r >= lo && r < hi) {  // jump over the held rows, staying on this CTA's share
+        r += (hi - r + gridDim.x - 1) / gridDim.x * gridDim.x - gridDim.x;
+        continue;
+      }
+      if (tid < 64) reinterpret_cast<uint4*>(p.out + r * D * 2)[tid] = make_uint4(0, 0, 0, 0);
+      if (tid == 64 && p.lse) p.lse[r] = 0.f;
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) *p.total = total;
+  sas::pdl_launch_dependents();
+  __syncthreads();
+  const uint32_t tmem = ms.tmem;
+  volatile sas::CtaCtl* ctl = &ms.ctl;
+  const uint32_t q_base = sas::smem_u32(smem + OFF_Q), kv_base = sas::smem_u32(smem + OFF_KV),
+                 p_base = sas::smem_u32(smem + OFF_P);
+#define WAIT(bar, par, id) sas::mbar_wait(&bars[bar], (par)&1, ctl, p.status, id)
+
+  if (warp == kCoordWarp) {
+    // ================================================= coordinator
+    int b = ms.start_b, cached = -1;
+    int64_t prefix = ms.start_prefix, t = t0;
+    uint32_t c = 0, uc = 0;
+    bool ok = true, lead_cut = false;
+    auto publish = [&](int flags, int row0, int nrows, int us) -> bool {
+      const int slot = c % kRing;
+      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + slot, (c / kRing) ^ 1u, 20))) return false;
+      if (lane == 0) {
+        ms.ring[slot] = Tile{flags, row0, nrows, us};
+        sas::mbar_arrive(&bars[B_CFULL + slot]);
+      }
+      ++c;
+      return true;
+    };
+    while (ok && t < t1 && b < p.B) {
+      const Req r = request(p, b);
+      if (t >= prefix + r.all()) {
+        prefix += r.all();
+        ++b;
+        continue;
+      }
+      const int u = (int)((t - prefix) / r.tiles);
+      const int64_t ustart = prefix + (int64_t)u * r.tiles, uend = ustart + r.tiles;
+      int k0 = (int)(t - ustart), k1 = (int)min((int64_t)r.tiles, t1 - ustart);
+      if (!p.split) {  // a unit belongs to the range that its first tile is in
+        if (k0 > 0) {
+          t = uend;
+          continue;
+        }
+        k1 = r.tiles;
+      }
+      if (b != cached) {
+        __syncwarp();
+        if (!r.bad)
+          for (int i = lane; i < r.n; i += 32) ms.parents[i] = __ldg(p.parents + r.base + i);
+        else if (lane == 0 && u == 0 && k0 == 0)
+          bad(p, SAS_ERR_BAD_TREE);
+        cached = b;
+        __syncwarp();
+      }
+      const int us = uc % kUnitSlots;
+      Unit& un = ms.units[us];
+      const int64_t row_in = p.scenario == 3 ? (int64_t)u * p.H + g * MR : (int64_t)u * MR;
+      const int nrows = p.scenario == 3 ? min(MR, p.H - g * MR) : (int)min((int64_t)MR, (int64_t)r.slots * p.H - row_in);
+      const int i0 = (int)(row_in / p.H), i1 = (int)((row_in + nrows - 1) / p.H);
+      // the slot's last readers are done: see kUnitSlots; the ring wait below
+      // orders this warp's writes after their reads
+      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + c % kRing, (c / kRing) ^ 1u, 20))) break;
+      int pos = -1;
+      if (lane < kMaxTok) {
+        uint32_t* bits = un.bits[lane];
+        for (int w = 0; w < (min(r.n, kMaxTree) + 31) / 32 || w < 1; ++w) bits[w] = 0;
+        const int i = i0 + lane;
+        if (i <= i1 && i < r.n && !r.bad && ms.parents[i] >= -1) {
+          int j = i, d = 0;
+          bool good = true;
+          while (true) {
+            if (d <= p.win) bits[j >> 5] |= 1u << (j & 31);
+            const int q = ms.parents[j];
+            if (q == -1) break;
+            if (q < -1 || q >= j) {  // after an unused slot, or not before its child
+              good = false;
+              break;
+            }
+            j = q;
+            ++d;
+          }
+          if (good) pos = r.ctx + d;
+          else bad(p, SAS_ERR_BAD_TREE);
+        }
+        // window_bits reads one word past the last one with a bit
+        const int w = (min(r.n, kMaxTree) + 31) / 32;
+        for (int x = max(w, 1); x < min(w + 5, kWords); ++x) bits[x] = 0;
+        un.pos[lane] = pos;
+      }
+      if (lane == 0) {
+        un.b = b;
+        un.tok = r.base + i0;
+        un.ctx = r.ctx;
+        un.thr = r.thr;
+        un.qrow = (int64_t)r.base * p.H + row_in;
+        un.nrows = nrows;
+        un.roff = (int)(row_in % p.H);
+      }
+      const bool any = __any_sync(0xffffffffu, pos >= 0);
+      const bool whole = k0 == 0 && k1 == r.tiles;
+      if (k0 > 0 && any) {
+        lead_cut = true;
+        if (lane == 0) p.cuts[blockIdx.x] = Cut{ustart, uend, un.qrow, nrows, 1};
+      }
+      if (!any) {
+        if (k0 == 0) {
+          ok = publish(TF_ZERO, 0, 0, us);
+          ++uc;
+        }
+      } else {
+        ++uc;
+        const int part = whole ? 0 : (t == t0 ? TF_PART0 : TF_PART1);
+        const int lo = max(r.ctx - p.win, 0);
+        const int wrows = r.ctx - lo + min(i1, r.n - 1) + 1;  // up to the unit's last drafted token
+        for (int k = k0; k < k1 && ok; ++k) {
+          int fl = part | (k == k0 ? TF_FIRST : 0) | (k == k1 - 1 ? TF_LAST : 0), row0, n;
+          if (k < r.wtiles) {
+            row0 = lo + k * CH;
+            n = min(CH, wrows - k * CH);
+          } else {
+            row0 = (k - r.wtiles) * CH;
+            n = min(CH, (p.scenario == 3 ? p.K : r.thr) - row0);
+            fl |= TF_CMP | (p.scenario == 3 ? TF_TOPK : 0);
+          }
+          ok = publish(fl, row0, max(n, 0), us);
+        }
+      }
+      t = ustart + k1;
+    }
+    if (lane == 0 && !lead_cut && rank < R) p.cuts[blockIdx.x].cut = 0;
+    if (ok) publish(TF_END, 0, 0, 0);
+  } else if (warp >= kLoadWarp0) {
+    // ================================================= loaders
+    const int lw = warp - kLoadWarp0;
+    uint32_t c = 0, n = 0, q = 0;
+    int row = -1;
+    Tile t{};
+    // pool row of tile row 16 * lw + lane (-1: none)
+    auto resolve = [&]() -> int {
+      const int r = lw * 16 + lane;
+      if (lane >= 16 || r >= t.nrows || (t.flags & (TF_END | TF_ZERO))) return -1;
+      const Unit& u = ms.units[t.uslot];
+      const int f = (t.flags & TF_CMP) ? 1 : 0;
+      int pos = t.row0 + r;
+      if (t.flags & TF_TOPK) {
+        pos = __ldg(p.idx + (int64_t)u.tok * p.K + pos);
+        if (pos < 0 || pos >= u.thr) return -1;
+      }
+      const int col = pos / p.bs[f];
+      if (col >= p.bt_stride[f]) {
+        bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
+        return -1;
+      }
+      const int blk = __ldg(p.bt[f] + (int64_t)u.b * p.bt_stride[f] + col);
+      if (blk < 0) return -1;
+      if (blk >= p.nblk[f]) {
+        bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
+        return -1;
+      }
+      return blk * p.bs[f] + (pos - col * p.bs[f]);
+    };
+    while (true) {
+      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
+      t = ms.ring[c % kRing];
+      if (t.flags & TF_END) break;
+      if (!(t.flags & TF_ZERO)) {
+        row = resolve();
+        if (t.flags & TF_FIRST) {
+          if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
+          const Unit& u = ms.units[t.uslot];
+          const uint8_t* src = p.q + u.qrow * (D * 2) + lane * 16;
+          const int nr = u.nrows;
+#pragma unroll
+          for (int i = 0; i < MR / kLoadWarps; ++i) {
+            const int r = lw * (MR / kLoadWarps) + i;
+            const uint32_t dst = q_base + r * 128 + (((lane & 7) ^ (r & 7)) << 4) + (lane >> 3) * QSLAB;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              cp16(dst + h * 4 * QSLAB, src + (r < nr ? (int64_t)r * (D * 2) + h * 512 : 0), r < nr ? 16u : 0u);
+          }
+          cp_arrive(&bars[B_QFULL]);
+          ++q;
+        }
+        const int f = (t.flags & TF_CMP) ? 1 : 0;
+        const int top = max(16, (t.nrows + 15) & ~15);
+        const int cnt = min(16, max(0, top - lw * 16));
+        bool ok = true;
+        for (int h = 0; h < 2; ++h) {
+          if (!__all_sync(0xffffffffu, WAIT(B_EMPTY + h, n ^ 1u, 23))) {
+            ok = false;
+            break;
+          }
+          if (h == 0) {  // the rows' mask; its last reader signed off before the tile's slot came free
+            const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
+            if (lane == 0) {
+              reinterpret_cast<uint16_t*>(ms.vmask)[lw] = (uint16_t)vm;
+              sas::mbar_arrive(&bars[B_VFULL]);
+            }
+          }
+          const uint8_t* src = p.kv[f] + h * 512 + lane * 16;
+          const uint32_t dst = kv_base + (h * 4 + (lane >> 3)) * SLAB + lw * 16 * 128;
+#pragma unroll 8
+          for (int i = 0; i < cnt; ++i) {
+            const int ri = __shfl_sync(0xffffffffu, row, i);
+            cp16(dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
+          }
+          cp_arrive(&bars[B_FULL + h]);
+        }
+        if (!ok) break;
+        ++n;
+      }
+      __syncwarp();
+      if (lane == 0) sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
+      ++c;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp) {
+    // ================================================= MMA issuer
+    if (lane == 0) {
+      constexpr int fmt = DT == SAS_DTYPE_BF16 ? 1 : 0;
+      constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, MR, CH, 0, 0);
+      constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, MR, 256, 0, 1);
+      uint32_t c = 0, n = 0, u = 0;
+      while (true) {
+        if (!WAIT(B_CFULL + c % kRing, c / kRing, 24)) break;
+        const Tile t = ms.ring[c % kRing];
+        if (t.flags & TF_END) break;
+        if (!(t.flags & TF_ZERO)) {
+          if ((t.flags & TF_FIRST) && !WAIT(B_QFULL, u, 25)) break;
+          bool ok = true;
+          for (int h = 0; h < 2; ++h) {
+            if (!WAIT(B_FULL + h, n, 26)) {
+              ok = false;
+              break;
+            }
+            sas::fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+            sas::tc_fence_after();
+#pragma unroll
+            for (int s = 4 * h; s < 4 * h + 4; ++s)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma_ws(tmem + TM_S, sas::umma_desc_sw128(q_base + s * QSLAB + kk * 32, 16, 1024),
+                        sas::umma_desc_sw128(kv_base + s * SLAB + kk * 32, 16, 1024), id_s, (s | kk) != 0);
+          }
+          if (!ok) break;
+          sas::umma_commit(&bars[B_SFULL]);
+          if (t.flags & TF_LAST) sas::umma_commit(&bars[B_QEMPTY]);
+          if (!WAIT(B_PREADY, n, 27)) break;
+          if ((t.flags & TF_FIRST) && !WAIT(B_OEMPTY, u ^ 1u, 28)) break;
+          sas::tc_fence_after();
+          const int steps = max(1, (t.nrows + 15) / 16);
+          for (int h = 0; h < 2; ++h) {
+            for (int ks = 0; ks < steps; ++ks)
+              umma_ws(tmem + TM_O + 128 * h,
+                      sas::umma_desc_sw128(p_base + (ks >> 2) * QSLAB + (ks & 3) * 32, 16, 1024),
+                      sas::umma_desc_sw128(kv_base + 4 * h * SLAB + ks * 2048, SLAB, 1024), id_o,
+                      !((t.flags & TF_FIRST) && ks == 0));
+            sas::umma_commit(&bars[B_EMPTY + h]);
+          }
+          if (t.flags & TF_LAST) {
+            sas::umma_commit(&bars[B_OFULL]);
+            ++u;
+          }
+          ++n;
+        }
+        sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
+        ++c;
+      }
+      // nothing may still run on TMEM or shared memory when the CTA leaves
+      sas::umma_commit(&bars[B_DRAIN]);
+      sas::mbar_wait_drain(&bars[B_DRAIN], 0, SAS_WAIT_LIMIT_NS);
+    }
+    __syncwarp();
+  } else {
+    // ================================================= softmax, epilogue
+    const int row = tid & 63, ch = tid >> 6;  // columns [64 ch, 64 ch + 64) of a tile
+    const uint32_t tl = tmem + ((uint32_t)warp << 21);
+    uint32_t c = 0, n = 0, u = 0, sy = 0;
+    float m = -INFINITY, l = 0.f;
+    int pos = -1, tok = 0;
+    bool ok = true;
+    while (ok) {
+      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 29))) break;
+      const Tile t = ms.ring[c % kRing];
+      if (t.flags & TF_END) break;
+      const Unit& un = ms.units[t.uslot];
+      if (t.flags & TF_ZERO) {
+        uint4* o = reinterpret_cast<uint4*>(p.out + un.qrow * (D * 2));
+        for (int i = tid; i < un.nrows * (D / 8); i += 128) o[i] = make_uint4(0, 0, 0, 0);
+        if (p.lse && tid < un.nrows) p.lse[un.qrow + tid] = 0.f;
+      } else {
+        if (t.flags & TF_FIRST) {
+          m = -INFINITY;
+          l = 0.f;
+          tok = p.scenario == 3 ? 0 : min((un.roff + row) / p.H, kMaxTok - 1);
+          pos = row < un.nrows ? un.pos[tok] : -1;
+        }
+        ok = __all_sync(0xffffffffu, WAIT(B_VFULL, n, 30) && WAIT(B_SFULL, n, 31));
+        if (!ok) break;
+        sas::tc_fence_after();
+        float s[64];
+        {
+          uint32_t r[32];
+          sas::tmem_ld32(tl + TM_S, r);
+          sas::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(r[i]);
+          sas::tmem_ld32(tl + TM_S + 32, r);
+          sas::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(r[i]);
+        }
+        // rows that are there, and those of them that this row's token sees
+        const uint32_t v0 = ms.vmask[2 * ch], v1 = ms.vmask[2 * ch + 1];
+        uint32_t k0 = v0, k1 = v1;
+        if (pos < 0) {
+          k0 = k1 = 0;
+        } else if (!(t.flags & TF_CMP)) {
+          const int p0 = t.row0 + 64 * ch;
+          k0 &= window_bits(p0, pos, p.win, un.ctx, un.bits[tok]);
+          k1 &= window_bits(p0 + 32, pos, p.win, un.ctx, un.bits[tok]);
+        }
+        if (!__all_sync(0xffffffffu, (k0 & k1) == 0xffffffffu)) {
+          // A row of KV with infinities or NaN that this token does not see
+          // would reach its sum as 0 * NaN. Its scores are not finite, which
+          // one sum shows; such rows are then cleared before the product. A
+          // token that does see one has a NaN in l, so its result is NaN.
+          float z = 0.f;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const uint32_t v = i < 32 ? v0 : v1, k = i < 32 ? k0 : k1;
+            const bool see = (k >> (i & 31)) & 1u;
+            z = fmaf(((v >> (i & 31)) & 1u) ? s[i] : 0.f, 0.f, z);
+            s[i] = see ? s[i] * p.scale_log2 : -INFINITY;
+          }
+          if (z != 0.f) {
+            for (int i = 0; i < 64; ++i) {
+              const uint32_t v = i < 32 ? v0 : v1;
+              if (!((v >> (i & 31)) & 1u)) continue;
+              const int kr = 64 * ch + i;
+              uint32_t hot = 0;
+              for (int e = 0; e < 64; ++e) {  // 16-byte pieces of the row
+                uint32_t w[4];
+                const uint32_t a = kv_base + (e >> 3) * SLAB + kr * 128 + (e & 7) * 16;
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+                constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
+              }
+              if (hot) {
+                const uint32_t k = i < 32 ? k0 : k1;
+                if ((k >> (i & 31)) & 1u) l = NAN;
+                for (int e = 0; e < 64; ++e) st_shared16(kv_base + (e >> 3) * SLAB + kr * 128 + (e & 7) * 16, 0, 0, 0, 0);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) s[i] *= p.scale_log2;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i]);
+        float* red = ms.red[n & 1];
+        red[tid] = mx;
+        sas::mbar_arrive(&bars[B_SSYNC]);
+        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
+        if (!ok) break;
+        ++sy;
+        mx = fmaxf(mx, red[tid ^ 64]);
+        float fac = 1.f;
+        if (mx > m + kMove || (m == -INFINITY && mx > m)) {
+          fac = sas::ex2(m - mx);
+          m = mx;
+          l *= fac;
+        }
+        // the product before this tile's is complete: its commit came before this tile's scores
+        if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
+#pragma unroll 1
+          for (int x = 0; x < 256; x += 32) {
+            uint32_t r[32];
+            sas::tmem_ld32(tl + TM_O + x, r);
+            sas::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * fac);
+            sas::tmem_st32(tl + TM_O + x, r);
+          }
+          sas::tmem_wait_st();
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float la[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t pd = p_base + ch * QSLAB + row * 128;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float a = sas::ex2(s[8 * e + 2 * x] - ref), b = sas::ex2(s[8 * e + 2 * x + 1] - ref);
+            la[x] += a + b;
+            w[x] = pack2<DT>(a, b);
+          }
+          st_shared16(pd + ((e ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
+        }
+        l += (la[0] + la[1]) + (la[2] + la[3]);
+        sas::fence_proxy_async_smem();
+        sas::tc_fence_before();
+        sas::mbar_arrive(&bars[B_PREADY]);
+        ++n;
+        if (t.flags & TF_LAST) {
+          float* rl = ms.red[2];
+          rl[tid] = l;
+          sas::mbar_arrive(&bars[B_SSYNC]);
+          ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
+          if (!ok) break;
+          ++sy;
+          const float lt = ch ? rl[tid ^ 64] + l : l + rl[tid ^ 64];
+          ok = __all_sync(0xffffffffu, WAIT(B_OFULL, u, 33));
+          if (!ok) break;
+          ++u;
+          sas::tc_fence_after();
+          const bool there = row < un.nrows;
+          if (t.flags & (TF_PART0 | TF_PART1)) {
+            float* o = p.part + ((size_t)blockIdx.x * 2 + ((t.flags & TF_PART1) ? 1 : 0)) * kPieceFloats;
+            if (ch == 0) {
+              o[MR * D + row] = m;
+              o[MR * D + MR + row] = pos < 0 ? -1.f : lt;  // -1: the token is not in use
+            }
+#pragma unroll 1
+            for (int x = 0; x < 8; ++x) {
+              uint32_t r[32];
+              __syncwarp();
+              sas::tmem_ld32(tl + TM_O + 32 * x, r);
+              sas::tmem_wait_ld();
+              float4* d4 = reinterpret_cast<float4*>(o + row * D + (x >> 2) * 256 + ch * 128 + (x & 3) * 32);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                d4[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+            }
+          } else {
+            const float sink = there ? __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e : 0.f;
+            const float top = fmaxf(m, sink);
+            const float a = m == -INFINITY ? 0.f : exp2f(m - top);
+            const float den = lt * a + (sink == -INFINITY ? 0.f : exp2f(sink - top));
+            const float k = pos < 0 || m == -INFINITY && lt == 0.f ? 0.f : a / den;
+            const bool zero = k == 0.f;
+            if (there && ch == 0 && p.lse) p.lse[un.qrow + row] = pos < 0 ? 0.f : (top + log2f(den)) * kLn2;
+            uint8_t* orow = p.out + (un.qrow + row) * (D * 2);
+#pragma unroll 1
+            for (int x = 0; x < 8; ++x) {
+              uint32_t r[32];
+              __syncwarp();
+              sas::tmem_ld32(tl + TM_O + 32 * x, r);
+              sas::tmem_wait_ld();
+              uint4* d4 = reinterpret_cast<uint4*>(orow + ((x >> 2) * 256 + ch * 128 + (x & 3) * 32) * 2);
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                w[i] = zero ? 0u : pack2<DT>(__uint_as_float(r[2 * i]) * k, __uint_as_float(r[2 * i + 1]) * k);
+              if (there)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d4[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            }
+          }
+          sas::tc_fence_before();
+          sas::mbar_arrive(&bars[B_OEMPTY]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
+      ++c;
+    }
+  }
+  sas::tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) sas::tmem_dealloc(tmem, TM_COLS);
+#undef WAIT
+}
+
+// Joins the pieces of a cut unit, in order. The block of CTA c does so when c's
+// range is the first to start inside the unit; blockIdx.y takes 8 of its rows.
+template <int DT>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeParams p) {
+  sas::pdl_wait();
+  const int g = blockIdx.x % p.G, rank = blockIdx.x / p.G;
+  const int64_t total = *p.total;
+  const int R = ranges(total, p.R);
+  if (rank == 0 || rank >= R) return;
+  const Cut c = p.cuts[blockIdx.x];
+  if (!c.cut) return;
+  const int64_t before = range_start(total, R, rank - 1);
+  if (before > c.ustart) return;  // an earlier range starts inside the unit
+  int last = rank;                // the range that holds the unit's last tile
+  while (last + 1 < R && range_start(total, R, last + 1) < c.uend) ++last;
+  // the first piece is partial 0 of its CTA if the unit starts with the range
+  const int first_slot = before == c.ustart ? 0 : 1;
+  auto piece = [&](int r) { return p.part + ((size_t)(r * p.G + g) * 2 + (r == rank - 1 ? first_slot : 0)) * kPieceFloats; };
+  for (int i = threadIdx.x >> 7; i < 8; i += 2) {
+    const int row = blockIdx.y * 8 + i, col = threadIdx.x & 127;
+    if (row >= c.nrows) break;
+    const float sink = __ldg(p.sinks + (c.qrow + row) % p.H) * kLog2e;
+    float top = sink;
+    for (int r = rank - 1; r <= last; ++r) top = fmaxf(top, piece(r)[MR * D + row]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float den = exp2f(sink - base);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool used = true;
+    for (int r = rank - 1; r <= last; ++r) {
+      const float* q = piece(r);
+      const float w = exp2f(q[MR * D + row] - base), l = q[MR * D + MR + row];
+      if (l < 0.f) used = false;
+      const float4 v = reinterpret_cast<const float4*>(q + row * D)[col];
+      den = fmaf(l, w, den);
+      if (w != 0.f) o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+    }
+    const float k = used && top != -INFINITY ? 1.f / den : 0.f;
+    uint2 out = make_uint2(0u, 0u);
+    if (k != 0.f || den != den) out = make_uint2(pack2<DT>(o.x * k, o.y * k), pack2<DT>(o.z * k, o.w * k));
+    if (!used) out = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(p.out + (c.qrow + row) * (D * 2) + col * 8) = out;
+    if (col == 0 && p.lse) p.lse[c.qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
+  }
+}
+
+size_t workspace_bytes(int sms) { return 256 + (size_t)sms * (sizeof(Cut) + 2 * kPieceFloats * sizeof(float)); }
+
+template <int DT>
+int launch(const TreeParams& p, cudaStream_t st) {
+  auto kern = tree_attn_kernel<DT>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return SAS_ERR_CUDA;
+  kern<<<p.R * p.G, kThreads, SMEM_BYTES, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return SAS_ERR_CUDA;
+  if (!p.split) return SAS_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.R * p.G, MR / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<DT>, p) == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
+}
+
+bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+size_t sas_tree_attn_workspace_bytes(int32_t num_sms) { return num_sms > 0 ? workspace_bytes(num_sms) : 0; }
+
+int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim, int32_t dtype, int32_t layout,
+                           int32_t B, int32_t S, const int32_t* cu, const int32_t* seqused, const int32_t* parents,
+                           const void* ori_kv, int64_t ori_nblk, int32_t ori_bs, const int32_t* ori_bt,
+                           int32_t ori_stride, const void* cmp_kv, int64_t cmp_nblk, int32_t cmp_bs,
+                           const int32_t* cmp_bt, int32_t cmp_stride, const int32_t* idx, int32_t K,
+                           const float* sinks, float softmax_scale, int32_t ratio, int32_t win, int32_t scenario,
+                           void* out, float* lse, int32_t num_sms, int32_t* status, void* workspace,
+                           size_t workspace_size, void* stream) {
+  if (dtype != SAS_DTYPE_BF16 && dtype != SAS_DTYPE_FP16) return SAS_ERR_UNSUPPORTED;
+  if (head_dim != D || H <= 0 || H % 8 || T < 0 || B < 0 || win < 0 || num_sms <= 0) return SAS_ERR_INVALID_ARG;
+  if (scenario < 1 || scenario > 3) return SAS_ERR_INVALID_ARG;
+  if (layout == SAS_LAYOUT_TND ? (!cu && B > 0) : (layout != SAS_LAYOUT_BSND || S < 0 || (int64_t)B * S != T))
+    return SAS_ERR_INVALID_ARG;
+  if (T == 0) return SAS_OK;
+  if (!q || !out || !sinks || !parents || B <= 0 || !seqused || !ori_kv || !ori_bt || ori_bs <= 0 || ori_stride <= 0 || ori_nblk < 0)
+    return SAS_ERR_INVALID_ARG;
+  if (scenario >= 2 && (!cmp_kv || !cmp_bt || cmp_bs <= 0 || cmp_stride <= 0 || cmp_nblk < 0 || ratio <= 0))
+    return SAS_ERR_INVALID_ARG;
+  if (scenario == 3 && (!idx || K <= 0)) return SAS_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(ori_kv) || !aligned16(cmp_kv)) return SAS_ERR_INVALID_ARG;
+  if (!workspace || workspace_size < workspace_bytes(num_sms)) return SAS_ERR_WORKSPACE;
+  if (!sas::select_device_of(q)) return SAS_ERR_CUDA;
+  TreeParams p = {};
+  p.q = static_cast<const uint8_t*>(q);
+  p.out = static_cast<uint8_t*>(out);
+  p.lse = lse;
+  p.T = T, p.H = H, p.scenario = scenario, p.K = K, p.ratio = ratio, p.win = win < kMaxCtx ? win : kMaxCtx, p.B = B, p.S = S, p.layout = layout;
+  p.G = scenario == 3 ? (H + MR - 1) / MR : 1;
+  if (p.G > num_sms) return SAS_ERR_UNSUPPORTED;
+  p.R = num_sms / p.G;
+  p.split = 1;
+  p.cu = cu, p.seqused = seqused, p.parents = parents;
+  p.kv[0] = static_cast<const uint8_t*>(ori_kv), p.kv[1] = static_cast<const uint8_t*>(cmp_kv);
+  p.bt[0] = ori_bt, p.bt[1] = cmp_bt;
+  p.bs[0] = ori_bs, p.bs[1] = cmp_bs;
+  p.bt_stride[0] = ori_stride, p.bt_stride[1] = cmp_stride;
+  p.nblk[0] = ori_nblk, p.nblk[1] = cmp_nblk;
+  p.idx = idx, p.sinks = sinks, p.scale_log2 = softmax_scale * kLog2e;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.total = reinterpret_cast<int64_t*>(ws);
+  p.part = reinterpret_cast<float*>(ws + 256);
+  p.cuts = reinterpret_cast<Cut*>(ws + 256 + (size_t)num_sms * 2 * kPieceFloats * sizeof(float));
+  p.status = status;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == SAS_DTYPE_BF16 ? launch<SAS_DTYPE_BF16>(p, st) : launch<SAS_DTYPE_FP16>(p, st);
+}
+
+}  // extern "C"

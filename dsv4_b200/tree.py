@@ -1,0 +1,149 @@
+"""Attention of drafted tokens that form a tree over the paged shared-KV caches.
+
+``tree_attn_sharedkv`` is to a drafted tree what ``sparse_attn_sharedkv`` is to
+a chain of new tokens: the same caches, tables, lengths, sinks and scenarios
+(window only, the whole compressed cache, top-k lists), with each token seeing
+its ancestors instead of everything before it. The reference decodes chains
+only (``sparse_attn_sharedkv_tilelang/api.py:129-397``). No schedule is needed:
+the kernel cuts the work itself. The current stream, no host synchronisation,
+no CPU fallback; errors as in ``sparse_attn_sharedkv``.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from .rope import LAYOUTS, _dtype_code, _i32
+
+HEAD_DIM = 512
+MAX_TREE = 1024
+
+
+def tree_attn_sharedkv(
+    q: torch.Tensor,
+    *,
+    ori_kv: torch.Tensor,
+    ori_block_table: torch.Tensor,
+    tree_parents: torch.Tensor,
+    seqused_kv: torch.Tensor,
+    sinks: torch.Tensor,
+    softmax_scale: float,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    cmp_kv: Optional[torch.Tensor] = None,
+    cmp_sparse_indices: Optional[torch.Tensor] = None,
+    cmp_block_table: Optional[torch.Tensor] = None,
+    cmp_ratio: Optional[int] = None,
+    ori_win_left: int = 127,
+    layout_q: str = "TND",
+    layout_kv: str = "PA_ND",
+    return_softmax_lse: bool = False,
+    out: Optional[torch.Tensor] = None,
+    lse_out: Optional[torch.Tensor] = None,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Returns the output in the layout of ``q`` (``[T, H, 512]`` or ``[B, S, H,
+    512]``), with ``return_softmax_lse`` also the fp32 log-sum-exp, sinks
+    included.
+
+    A request's n drafted tokens are in the window cache at the slots before
+    ``seqused_kv`` (``append_shared_kv`` puts them there). ``tree_parents``
+    (``[T]`` or ``[B, S]``) names for each the token that it follows, by its
+    index among its request's tokens and below its own; -1 follows the cached
+    context, anything less marks an unused slot (zero output and LSE). A token
+    at depth d has position ``ctx + d``, ``ctx = seqused_kv - n``, and attends
+    to its window of ``ori_win_left`` rows before that position (cached rows
+    and ancestors), to itself, and to compressed rows below ``ctx //
+    cmp_ratio``: with ``cmp_kv`` to all of them, with ``cmp_sparse_indices``
+    (``[T, 1, K]`` or ``[B, S, 1, K]``) to its list, where ids outside that
+    range are skipped. A KV row with infinities or NaN makes the output of the
+    tokens that see it NaN, and of no others. A request of over 1024 tokens,
+    with more tokens than ``seqused_kv``, or a token whose parent does not
+    precede it gives zeros and is recorded in the status word.
+    """
+    assert layout_kv == "PA_ND", "only layout_kv=PA_ND supported"
+    assert layout_q in LAYOUTS, f"unsupported layout_q={layout_q!r}"
+    code = _dtype_code(q.dtype)
+    if layout_q == "TND":
+        assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
+        if q.dim() != 3:
+            raise ValueError(f"q must be [T, heads, {HEAD_DIM}] (got {tuple(q.shape)})")
+        B, S = cu_seqlens_q.numel() - 1, 0
+    else:
+        if q.dim() != 4:
+            raise ValueError(f"q must be [B, S, heads, {HEAD_DIM}] (got {tuple(q.shape)})")
+        B, S = q.shape[0], q.shape[1]
+        if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
+            raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
+    H, D = q.shape[-2:]
+    T = q.shape[:-2].numel()
+    if D != HEAD_DIM or H <= 0 or H % 8:
+        raise ValueError(f"only D={HEAD_DIM} and heads a multiple of 8 supported (got {H} heads, D={D})")
+    if ori_win_left < 0:
+        raise ValueError("ori_win_left must not be negative")
+    if tree_parents.numel() != T:
+        raise ValueError(f"tree_parents must have one entry per token (got {tree_parents.numel()} for {T})")
+    if sinks.numel() != H:
+        raise ValueError(f"sinks must have one entry per head (got {sinks.numel()} for {H})")
+    scenario, K, ratio = 1, 0, 1
+    if cmp_kv is not None:
+        scenario, ratio = 2, 4 if cmp_ratio is None else cmp_ratio
+        assert cmp_block_table is not None, "cmp_kv needs cmp_block_table"
+        if ratio < 1:
+            raise ValueError(f"cmp_ratio must be positive (got {ratio})")
+    if cmp_sparse_indices is not None:
+        assert cmp_kv is not None, "cmp_sparse_indices needs cmp_kv"
+        scenario, K = 3, cmp_sparse_indices.shape[-1]
+        if K < 1 or cmp_sparse_indices.numel() != T * K:
+            raise ValueError(f"cmp_sparse_indices must be [tokens, 1, K] (got {tuple(cmp_sparse_indices.shape)})")
+    for name, kv, table in (("ori", ori_kv, ori_block_table), ("cmp", cmp_kv, cmp_block_table)):
+        if kv is None:
+            continue
+        if kv.dim() != 4 or kv.shape[2] != 1 or kv.shape[3] != D or kv.dtype != q.dtype or kv.shape[1] < 1:
+            raise ValueError(f"{name}_kv must be [blocks, block size, 1, {D}] of q's dtype")
+        if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
+            raise ValueError(f"{name}_block_table must be [{B}, blocks] (got {tuple(table.shape)})")
+    if B < 0 or seqused_kv.numel() != B:
+        raise ValueError(f"seqused_kv must have one entry per request (got {seqused_kv.numel()} for {B})")
+    for name, t, shape, dt in (("out", out, q.shape, q.dtype), ("lse_out", lse_out, q.shape[:-1], torch.float32)):
+        if t is not None and (t.shape != shape or t.dtype != dt or t.device != q.device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor of {dt} beside q")
+    if not q.is_cuda:
+        raise RuntimeError("tree_attn_sharedkv needs q on a CUDA device (no CPU path)")
+    dev = q.device
+    q = _aligned(q.detach())
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if lse_out is None and return_softmax_lse:
+        lse_out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
+    if T:
+        lib = _lib.lib()
+        st = _lib.state(dev)
+        cu = _i32(cu_seqlens_q, dev) if cu_seqlens_q is not None else None
+        skv, par = _i32(seqused_kv, dev), _i32(tree_parents, dev)
+        snk = sinks.detach().to(device=dev, dtype=torch.float32).contiguous()
+        ori, obt = _aligned(ori_kv.detach().to(dev)), _i32(ori_block_table, dev)
+        cmp = cbt = idx = None
+        if scenario >= 2:
+            cmp, cbt = _aligned(cmp_kv.detach().to(dev)), _i32(cmp_block_table, dev)
+        if scenario == 3:
+            idx = _i32(cmp_sparse_indices, dev)
+        # from the allocator, so that calls on several streams do not share it
+        ws = torch.empty(lib.sas_tree_attn_workspace_bytes(st.num_sms), dtype=torch.uint8, device=dev)
+        rc = lib.sas_tree_attn_sharedkv(
+            q.data_ptr(), T, H, D, code, LAYOUTS[layout_q], B, S, _lib.ptr(cu), skv.data_ptr(), par.data_ptr(),
+            ori.data_ptr(), ori.shape[0], ori.shape[1], obt.data_ptr(), obt.shape[1], _lib.ptr(cmp),
+            0 if cmp is None else cmp.shape[0], 0 if cmp is None else cmp.shape[1], _lib.ptr(cbt),
+            0 if cbt is None else cbt.shape[1], _lib.ptr(idx), K, snk.data_ptr(), float(softmax_scale), int(ratio),
+            min(int(ori_win_left), 1 << 30), scenario, out.data_ptr(), _lib.ptr(lse_out), st.num_sms,
+            st.status.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+        if rc in (1, 2):
+            raise ValueError(f"tree_attn_sharedkv: {_lib.ERRORS[rc]}")
+        _lib.check(rc, "sas_tree_attn_sharedkv")
+    return (out, lse_out) if return_softmax_lse else out
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -36,6 +36,9 @@ extern "C" {
                                      count was met; those rows were dropped like -1 entries */
 #define SAS_ERR_BAD_POSITION 8    /* device status, non-fatal: a position outside the cos / sin tables (the nearest
                                      row was used) */
+#define SAS_ERR_BAD_TREE 9        /* device status, non-fatal: a tree with a parent that is not before its child or
+                                     is unused, with over 1024 tokens, or with more tokens than seqused_kv; those
+                                     tokens' outputs are zero */
 #define SAS_ERR_TIMEOUT_BASE 16  /* device status: 16 + id of the bounded wait that ran out */
 
 #define SAS_META_SIZE 1024
@@ -300,6 +303,34 @@ int sas_append_sharedkv_bwd(const void* d_pool, int64_t num_blocks, int32_t bloc
                             const float* sin, int32_t P, int32_t R, const float* kv_weight, float* dkv_weight,
                             float eps, int32_t flags, int32_t* status, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of drafted tokens that form a tree over the paged caches (no
+ * counterpart in the reference, whose MTP decode takes a chain). The n new
+ * tokens of request b lie in the window cache at slots [ctx, ctx + n), ctx =
+ * seqused_kv[b] - n. tree_parents [T]: the index, among its request's tokens
+ * and below its own, of the token that it follows; -1: the cached context;
+ * less: an unused slot (zero output and LSE). A token at depth d has the
+ * position s = ctx + d and attends to the cached rows [s - ori_win_left, ctx),
+ * to its ancestors at most ori_win_left back and itself, and to the
+ * compressed rows below ctx // cmp_ratio: none (scenario 1), all (2) or its
+ * cmp_sparse_indices [T, topk] (3; ids outside that range are skipped).
+ * q, out [T, H, 512], lse fp32 [T, H] or NULL, sinks fp32 [H] (-inf: none),
+ * H a multiple of 8; caches, tables and layouts as in the forward. BSND:
+ * max_seqlen_q slots per request, cu_seqlens_q optional.
+ * Rows that no request holds are zeroed. One attention launch and a small one
+ * that joins the sums of rows cut over CTAs.
+ * ---------------------------------------------------------------------- */
+size_t sas_tree_attn_workspace_bytes(int32_t num_sms);
+int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim, int32_t dtype, int32_t layout_q,
+                           int32_t batch, int32_t max_seqlen_q, const int32_t* cu_seqlens_q,
+                           const int32_t* seqused_kv, const int32_t* tree_parents, const void* ori_kv,
+                           int64_t ori_num_blocks, int32_t ori_block_size, const int32_t* ori_block_table,
+                           int32_t ori_table_stride, const void* cmp_kv, int64_t cmp_num_blocks,
+                           int32_t cmp_block_size, const int32_t* cmp_block_table, int32_t cmp_table_stride,
+                           const int32_t* cmp_sparse_indices, int32_t topk, const float* sinks, float softmax_scale,
+                           int32_t cmp_ratio, int32_t ori_win_left, int32_t scenario, void* out, float* lse,
+                           int32_t num_sms, int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Process-wide options of the forward kernel (no counterpart in the
