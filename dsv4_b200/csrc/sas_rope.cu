@@ -156,6 +156,14 @@ __device__ __forceinline__ int table_row(const RopeParams& p, int t, int slot, i
   return (int)pos;
 }
 
+// a * b - c * d to about an ulp of the result however much cancels (Kahan's
+// difference of products): turned values keep their relative accuracy, which
+// the weight's gradient is a product of. Two more FMAs on rotated dims.
+__device__ __forceinline__ float diff_of_products(float a, float b, float c, float d) {
+  const float cd = c * d;
+  return fmaf(a, b, -cd) + fmaf(-c, d, cd);
+}
+
 // cos and sin of vector v's 4 (INTER) or 8 (halves) angles; `first` tells the
 // lower half. Returns false for a vector that is not rotated.
 template <bool INTER>
@@ -184,14 +192,14 @@ struct Angles {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float a = f[2 * i], b = f[2 * i + 1], sn = sgn * s[i];
-        f[2 * i] = a * c[i] - b * sn;
-        f[2 * i + 1] = a * sn + b * c[i];
+        f[2 * i] = diff_of_products(a, c[i], b, sn);
+        f[2 * i + 1] = diff_of_products(b, c[i], -a, sn);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float sn = sgn * s[i % (INTER ? 4 : 8)];
-        f[i] = f[i] * c[i % (INTER ? 4 : 8)] + (first ? -sn : sn) * o[i];
+        f[i] = diff_of_products(f[i], c[i % (INTER ? 4 : 8)], o[i], first ? sn : -sn);
       }
     }
   }
@@ -405,7 +413,8 @@ __global__ void __launch_bounds__(32 * kWarps) rope_bwd_kernel(const __grid_cons
           }
           an[j].turn(g[j], o, sgn);
         }
-        if (rs.w && v < V) weight8(rs.w, v, w);
+        if (v >= V) continue;
+        if (rs.w) weight8(rs.w, v, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           ss = fmaf(x[i], x[i], ss);
