@@ -139,6 +139,11 @@ def state(device: torch.device) -> _DeviceState:
     return st
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream's handle (0.1 us; torch.cuda.current_stream builds an object first, 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 

@@ -11,13 +11,17 @@
 // of the rotated part. All arithmetic is fp32; a value is rounded once, when
 // it is written.
 //
-// Everything here is bound by memory: 4 bytes per value forward (read and
-// written once in 16 bits), 6 backward, for 5-12 operations. A row of D values
-// lies with G lanes of a warp (8 values = 16 bytes per lane and vector), so
-// the sums are a few shuffles and the rotation stays inside a lane (INTER) or
-// takes one more load that hits L1 (halves). A warp takes U heads of ONE token, so the
-// position, the table rows and the slot lookup are fetched once for them, and
-// all U rows' loads are in flight before the first is used.
+// Everything here should be bound by memory: 4 bytes per value forward (read
+// and written once in 16 bits), 6 backward, for 5-12 operations. At the rate of
+// the memory an SM has 88 cycles for a forward row of 512 values, 350 issue
+// slots, so the instructions of a row count: pairs of fp32 operations in one
+// (f32x2), addresses that only advance, weights in registers. A row lies with G
+// lanes of a warp (8 values = 16 bytes per lane and vector), so its sums are a
+// few shuffles and an interleaved pair is in one lane. Warps work alone: each
+// walks runs of heads of one token, which share the position, the table rows
+// and the cache slot, and keeps kStages - 1 rows in flight with cp.async into
+// its own shared memory, which costs no registers, so that enough warps fit.
+// A call with few rows takes short runs, so that they spread over all SMs.
 #include "sas_common.cuh"
 
 namespace {
@@ -32,12 +36,14 @@ struct Rows {
   int64_t dy_ts, dy_hs;
   const float* w;  // [D] or nullptr
   float* dw_part;  // backward: [blocks of this set][D] or nullptr
-  int H, chunks, blocks;  // chunks: warps' shares of a token's heads
+  int H, run, chunks;   // a token's heads are `chunks` shares of `run` rows (a warp's width each)
+  uint32_t most, blocks;  // backward: shares of a warp, blocks
 };
 
 struct RopeParams {
   Rows q, k;
   int T, D, R, P, flags;
+  uint32_t most;  // forward: shares of a warp
   float eps;
   const void* positions;  // [T] int32 / int64, or nullptr: the cache slot (append), no rotation elsewhere
   const float* cos;
@@ -52,37 +58,60 @@ struct RopeParams {
   int32_t* status;
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool on) {  // zeros if not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two fp32 values in a register pair, and operations on both at once.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ float lo() const { return __uint_as_float((uint32_t)v); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float((uint32_t)(v >> 32)); }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
 template <int DT>
-__device__ __forceinline__ void unpack8(const uint4& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& r, F2 (&f)[4]) {
   const uint32_t u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 v;
     if (DT == SAS_DTYPE_BF16) {
-      v = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(u[i]));
+      f[i] = F2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
     } else {
-      v = __half22float2(reinterpret_cast<const __half2&>(u[i]));
+      const float2 v = __half22float2(reinterpret_cast<const __half2&>(u[i]));
+      f[i] = F2(v.x, v.y);
     }
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
   }
 }
 template <int DT>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+__device__ __forceinline__ uint4 pack8(const F2 (&f)[4]) {
   uint32_t u[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (DT == SAS_DTYPE_BF16) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      const __nv_bfloat162 v = __floats2bfloat162_rn(f[i].lo(), f[i].hi());
       u[i] = reinterpret_cast<const uint32_t&>(v);
     } else {
-      const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      const __half2 v = __floats2half2_rn(f[i].lo(), f[i].hi());
       u[i] = reinterpret_cast<const uint32_t&>(v);
     }
   }
@@ -96,49 +125,71 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// Request of token t, its cache slot and the pool row of that slot (-1: no
-// row; the column past the table's width or an entry past the pool is also
-// recorded). Every lane of the warp calls it. TND: a 32-way search of
-// cu_seqlens_q, two rounds up to 1024 requests.
-__device__ __forceinline__ int64_t slot_row(const RopeParams& p, int t, int lane, int& slot, bool want_row) {
-  int b, i, n;
-  if (p.layout == SAS_LAYOUT_TND) {
-    int lo = 0, len = p.B;  // the last b in [lo, lo + len) with cu[b] <= t
-    while (len > 1) {
-      const int step = (len + 31) >> 5;
-      const int c = lo + lane * step;
-      const bool le = c < lo + len && __ldg(p.cu + c) <= t;
-      const int last = 31 - __clz(__ballot_sync(0xffffffffu, le) | 1u);
-      const int at = lo + last * step;
-      len = min(step, lo + len - at);
-      lo = at;
+// The request that a warp's token is in and the page that its slot is in. A
+// warp's tokens are neighbours, so both are mostly those of the token before.
+// Every lane of the warp calls it.
+struct Slots {
+  int b = -1, c0 = 0, n = 0, used = 0, col = -1, blk = -1;
+  // TND: the 31 requests around the one that an even split would give are
+  // looked at first, then cu_seqlens_q is searched 32 ways at a time. The last
+  // round reads the lengths beside it.
+  __device__ __forceinline__ void find(const RopeParams& p, int t, int lane) {
+    if (b >= 0 && t >= c0 && t < c0 + n) return;
+    col = -1;
+    if (p.layout == SAS_LAYOUT_TND) {
+      int len = min(p.B, 31), lo = min(max((int)((int64_t)t * p.B / p.T) - 15, 0), p.B - len);
+      int mine, su;
+      auto read = [&]() {
+        mine = lane <= len ? __ldg(p.cu + lo + lane) : 0x7fffffff;
+        su = lane < len ? __ldg(p.seqused + lo + lane) : 0;
+      };
+      read();
+      if (__shfl_sync(0xffffffffu, mine, 0) > t || __shfl_sync(0xffffffffu, mine, len) <= t) {
+        lo = 0, len = p.B;  // the last request in [lo, lo + len) with cu <= t
+        while (len > 31) {
+          const int stride = (len + 31) >> 5;
+          const int c = lo + lane * stride;
+          const bool le = c < lo + len && __ldg(p.cu + c) <= t;
+          const int last = 31 - __clz(__ballot_sync(0xffffffffu, le) | 1u);
+          const int at = lo + last * stride;
+          len = min(stride, lo + len - at);
+          lo = at;
+        }
+        read();
+      }
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, lane < len && mine <= t) | 1u);
+      c0 = __shfl_sync(0xffffffffu, mine, k);
+      n = __shfl_sync(0xffffffffu, mine, k + 1) - c0;
+      used = __shfl_sync(0xffffffffu, su, k);
+      b = lo + k;
+    } else {
+      b = t / p.S;
+      c0 = b * p.S;
+      n = p.cu ? __ldg(p.cu + b + 1) - __ldg(p.cu + b) : p.S;
+      used = __ldg(p.seqused + b);
     }
-    b = lo;
-    const int c0 = __ldg(p.cu + b);
-    i = t - c0;
-    n = __ldg(p.cu + b + 1) - c0;
-  } else {
-    b = t / p.S;
-    i = t - b * p.S;
-    n = p.cu ? __ldg(p.cu + b + 1) - __ldg(p.cu + b) : p.S;
   }
-  slot = -1;
-  if (i < 0 || i >= n) return -1;  // BSND padding, or a token past cu_seqlens_q's end
-  slot = __ldg(p.seqused + b) - n + i;
-  if (!want_row || slot < 0) return -1;
-  const int col = slot / p.bs;
-  if (col >= p.bt_stride) {
-    if (lane == 0 && p.status) atomicCAS(p.status, 0, SAS_ERR_BAD_BLOCK_ENTRY);
-    return -1;
+  // Slot of token t and, if wanted, the pool row of that slot. -1: none; the
+  // column past the table's width or an entry past the pool is also recorded.
+  __device__ __forceinline__ int64_t row(const RopeParams& p, int t, int lane, int& slot, bool want_row) {
+    find(p, t, lane);
+    const int i = t - c0;
+    slot = -1;
+    if (i < 0 || i >= n) return -1;  // BSND padding, or a token past cu_seqlens_q's end
+    slot = used - n + i;
+    if (!want_row || slot < 0) return -1;
+    const int c = slot / p.bs;
+    if (c != col) {
+      col = c;
+      blk = c < p.bt_stride ? __ldg(p.bt + (int64_t)b * p.bt_stride + c) : 0x7fffffff;
+      if (blk >= p.nblk) {
+        if (lane == 0 && p.status) atomicCAS(p.status, 0, SAS_ERR_BAD_BLOCK_ENTRY);
+        blk = -1;
+      }
+    }
+    return blk < 0 ? -1 : (int64_t)blk * p.bs + (slot - c * p.bs);
   }
-  const int blk = __ldg(p.bt + (int64_t)b * p.bt_stride + col);
-  if (blk < 0) return -1;
-  if (blk >= p.nblk) {
-    if (lane == 0 && p.status) atomicCAS(p.status, 0, SAS_ERR_BAD_BLOCK_ENTRY);
-    return -1;
-  }
-  return (int64_t)blk * p.bs + (slot - col * p.bs);
-}
+};
 
 // Row of the cos / sin tables of token t. A position outside the tables takes
 // the nearest row and is recorded.
@@ -157,303 +208,369 @@ __device__ __forceinline__ int table_row(const RopeParams& p, int t, int slot, i
 }
 
 // a * b - c * d to about an ulp of the result however much cancels (Kahan's
-// difference of products): turned values keep their relative accuracy, which
-// the weight's gradient is a product of. Two more FMAs on rotated dims.
+// difference of products)
 __device__ __forceinline__ float diff_of_products(float a, float b, float c, float d) {
   const float cd = c * d;
   return fmaf(a, b, -cd) + fmaf(-c, d, cd);
 }
 
-// cos and sin of vector v's 4 (INTER) or 8 (halves) angles; `first` tells the
-// lower half. Returns false for a vector that is not rotated.
-template <bool INTER>
-struct Angles {
-  float c[INTER ? 4 : 8], s[INTER ? 4 : 8];
-  bool on, first;
-  __device__ __forceinline__ void load(const RopeParams& p, int v, int row) {
-    const int e = v * 8 - (p.D - p.R);
-    on = e >= 0 && v * 8 < p.D;
-    first = e < p.R / 2;
-    if (!on) return;
-    const int a = INTER ? e / 2 : (first ? e : e - p.R / 2);
-    const float* pc = p.cos + (int64_t)row * (p.R / 2) + a;
-    const float* ps = p.sin + (int64_t)row * (p.R / 2) + a;
-#pragma unroll
-    for (int i = 0; i < (INTER ? 4 : 8); i += 4) {
-      const float4 a4 = __ldg(reinterpret_cast<const float4*>(pc + i));
-      const float4 b4 = __ldg(reinterpret_cast<const float4*>(ps + i));
-      c[i] = a4.x, c[i + 1] = a4.y, c[i + 2] = a4.z, c[i + 3] = a4.w;
-      s[i] = b4.x, s[i + 1] = b4.y, s[i + 2] = b4.z, s[i + 3] = b4.w;
-    }
-  }
-  // f rotated by sgn times the angle; `o`: the partner vector's values (halves only)
-  __device__ __forceinline__ void turn(float (&f)[8], const float (&o)[8], float sgn) const {
-    if (INTER) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = f[2 * i], b = f[2 * i + 1], sn = sgn * s[i];
-        f[2 * i] = diff_of_products(a, c[i], b, sn);
-        f[2 * i + 1] = diff_of_products(b, c[i], -a, sn);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float sn = sgn * s[i % (INTER ? 4 : 8)];
-        f[i] = diff_of_products(f[i], c[i % (INTER ? 4 : 8)], o[i], first ? sn : -sn);
-      }
-    }
-  }
+// Where a lane's vector lies in the rotation, the same for every row.
+struct Place {
+  int angle;    // first angle of the vector, -1: it is not rotated
+  int partner;  // halves: the partner's vector
+  float sgn;    // halves: the sine's sign, down for the lower half
 };
+template <bool INTER>
+__device__ __forceinline__ Place place_of(int v, int D, int R, float sgn) {
+  const int e = v * 8 - (D - R);
+  if (e < 0 || v * 8 >= D) return Place{-1, v, sgn};
+  if (INTER) return Place{e / 2, v, sgn};
+  return e < R / 2 ? Place{e, v + R / 16, -sgn} : Place{e - R / 2, v - R / 16, sgn};
+}
 
-__device__ __forceinline__ void weight8(const float* w, int v, float (&f)[8]) {
+// A rotated vector turned; table: its token's [cos R/2][sin R/2]; o: the
+// partner's values (halves only). EXACT: values that cancel keep their relative
+// accuracy (a weight's gradient is a sum of products of them).
+template <bool INTER, bool EXACT>
+__device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&o)[4], const float* table, const Place& at, int R) {
+  const float4* pc = reinterpret_cast<const float4*>(table + at.angle);
+  const float4* ps = reinterpret_cast<const float4*>(table + at.angle + R / 2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 c4 = pc[INTER ? 0 : i / 2], s4 = ps[INTER ? 0 : i / 2];
+    const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+    const float a = f[i].lo(), b = f[i].hi();
+    if (INTER) {
+      const float c = cs[i], s = at.sgn * ss[i];
+      f[i] = EXACT ? F2(diff_of_products(a, c, b, s), diff_of_products(b, c, -a, s)) : F2(a * c - b * s, a * s + b * c);
+    } else {
+      const float x = o[i].lo(), y = o[i].hi(), s0 = at.sgn * ss[2 * (i & 1)], s1 = at.sgn * ss[2 * (i & 1) + 1];
+      const float c0 = cs[2 * (i & 1)], c1 = cs[2 * (i & 1) + 1];
+      f[i] = EXACT ? F2(diff_of_products(a, c0, -x, s0), diff_of_products(b, c1, -y, s1)) : F2(a * c0 + x * s0, b * c1 + y * s1);
+    }
+  }
+}
+
+__device__ __forceinline__ void weight8(const float* w, int v, F2 (&f)[4]) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(w + v * 8));
   const float4 b = __ldg(reinterpret_cast<const float4*>(w + v * 8 + 4));
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  f[0] = F2(a.x, a.y), f[1] = F2(a.z, a.w), f[2] = F2(b.x, b.y), f[3] = F2(b.z, b.w);
 }
 
 constexpr int kWarps = 8;
+// blocks of an SM, by registers
+__host__ __device__ constexpr int fwd_blocks(int nv) { return nv == 1 ? 3 : 2; }
+__host__ __device__ constexpr int bwd_blocks(int nv) { return nv > 2 ? 1 : 2; }
+__host__ __device__ constexpr int stages_of(int nv) { return nv > 2 ? 2 : 4; }  // rows of a warp in flight or in work
 
-// DT: type; G lanes hold a row, NV vectors of 8 values each; U: rows in flight per group of lanes.
-template <int DT, int G, int NV, int U, bool INTER>
-__global__ void __launch_bounds__(32 * kWarps) rope_fwd_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int HW = 32 / G;  // heads side by side in a warp
-  const int lane = threadIdx.x & 31;
-  const uint32_t cpt = p.q.chunks + p.k.chunks;
-  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const uint32_t t = unit / cpt;
-  if (t >= (uint32_t)p.T) return;
-  int c = (int)(unit - t * cpt);
-  const bool isk = c >= p.q.chunks;
-  const Rows& rs = isk ? p.k : p.q;
-  if (isk) c -= p.q.chunks;
-  const int h0 = c * (U * HW) + lane / G, gl = lane % G;
-  const int V = p.D >> 3;
+// The shares of a warp: every warps-th one, so that the GPU's reads stay close
+// together (353 against 363 us for 16384 x 64 x 512), or `most` neighbours where
+// shares need the token's slot, whose request and page then stay.
+struct Walk {
+  uint32_t first, end, step;
+  __device__ __forceinline__ Walk(uint32_t warp, uint32_t warps, uint32_t all, uint32_t most)
+      : first(most ? min(warp * most, all) : warp), end(most ? min(first + most, all) : all), step(most ? 1 : warps) {}
+};
 
-  uint4 raw[U][NV];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = h0 + u * HW;
-    const uint8_t* xr = rs.x + ((int64_t)t * rs.x_ts + (int64_t)h * rs.x_hs) * 2;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int v = gl + G * j;
-      raw[u][j] = h < rs.H && v < V ? ldg_stream(xr + v * 16) : make_uint4(0, 0, 0, 0);
-    }
-  }
-  const bool append = p.pool != nullptr;
-  int slot = -1;
-  int64_t row = -1;
-  if (append && (isk || !p.positions)) row = slot_row(p, t, lane, slot, isk);
-  Angles<INTER> an[NV];
-  if (p.R > 0) {
-    const int tr = table_row(p, t, slot, lane);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) an[j].load(p, gl + G * j, tr);
-  }
-  const float sgn = (p.flags & SAS_ROPE_INVERSE) ? -1.f : 1.f;
+// A share's result, from the warp's side that loads to the one that computes.
+struct __align__(16) Share {
+  uint8_t* y;  // first row (nullptr: nothing is written)
+  int n, isk;
+};
+
+// DT: type; G lanes hold a row, NV vectors of 8 values each; FULL: D = 8 * G * NV.
+template <int DT, int G, int NV, bool FULL, bool INTER>
+__global__ void __launch_bounds__(32 * kWarps, fwd_blocks(NV)) rope_fwd_kernel(const __grid_constant__ RopeParams p) {
+  constexpr int HW = 32 / G, S = stages_of(NV), STAGE = NV * 512;
+  static_assert(HW == 1 || FULL, "rows side by side are whole");
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Share s_share[kWarps][S];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, sub = lane / G;
+  uint8_t* mine = smem + warp * S * (STAGE + p.R * 4);  // rows, then tables
+  const uint32_t base = sas::smem_u32(mine) + lane * 16, tables = sas::smem_u32(mine) + S * STAGE;
   const float invD = 1.f / (float)p.D;
-  uint8_t* yt = nullptr;
-  if (append && isk) {
-    if (row < 0) return;
-    yt = p.pool + row * p.D * 2;
-  } else {
-    yt = rs.y + (int64_t)t * rs.y_ts * 2;
-  }
-  float rstd[U];
-  if (p.flags & SAS_ROPE_NORM) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float ss = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float f[8];
-        unpack8<DT>(raw[u][j], f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-      }
-      rstd[u] = ss;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) rstd[u] = rsqrtf(group_sum<G>(rstd[u]) * invD + p.eps);
-  } else {
-#pragma unroll
-    for (int u = 0; u < U; ++u) rstd[u] = 1.f;
-  }
-  // halves: the partner vectors, read before any lane of the warp writes (y may be x)
-  uint4 part[INTER ? 1 : U][INTER ? 1 : NV];
-  if (!INTER) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HW;
-      const uint8_t* xr = rs.x + ((int64_t)t * rs.x_ts + (int64_t)h * rs.x_hs) * 2;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int v = gl + G * j + (an[j].first ? p.R / 16 : -(p.R / 16));
-        part[INTER ? 0 : u][INTER ? 0 : j] =
-            p.R > 0 && an[j].on && h < rs.H ? *reinterpret_cast<const uint4*>(xr + v * 16) : make_uint4(0, 0, 0, 0);
-      }
-    }
-    __syncwarp();
-  }
+  const bool norm = p.flags & SAS_ROPE_NORM;
+  bool on[NV];  // the lane has the vector
+  Place at[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int v = gl + G * j;
-    if (v >= V) continue;
-    const bool turn = p.R > 0 && an[j].on;
-    const int pv = v + (an[j].first ? p.R / 16 : -(p.R / 16));
-    float w[8], wp[8];
-    if (rs.w) {
-      weight8(rs.w, v, w);
-      if (!INTER && turn) weight8(rs.w, pv, wp);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HW;
-      if (h >= rs.H) continue;
-      float f[8], o[8];
-      unpack8<DT>(raw[u][j], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= rstd[u];
-      if (rs.w)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= w[i];
-      if (turn) {
-        if (!INTER) {
-          unpack8<DT>(part[INTER ? 0 : u][INTER ? 0 : j], o);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] *= rstd[u];
-          if (rs.w)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] *= wp[i];
-        }
-        an[j].turn(f, o, sgn);
+    on[j] = FULL || (gl + G * j) * 8 < p.D;
+    at[j] = place_of<INTER>(gl + G * j, p.D, p.R, (p.flags & SAS_ROPE_INVERSE) ? -1.f : 1.f);
+  }
+  // ---- the loading side: units of the walk, rows of the unit
+  const uint32_t per = p.q.chunks + p.k.chunks, all = (uint32_t)p.T * per;
+  const Walk walk(blockIdx.x * kWarps + warp, gridDim.x * kWarps, all, p.pool && !p.positions || !p.q.H ? p.most : 0);
+  uint32_t unit = walk.first, share_in = 0, row_in = 0;
+  Slots slots;
+  int left = 0, hleft = 0;
+  const uint8_t* x = nullptr;
+  int64_t xs = 0;
+  const uint8_t* rs0 = p.q.H ? p.q.x : p.k.x;  // a valid address for copies of nothing
+  auto issue = [&]() {
+    if (left == 0 && unit < walk.end) {
+      const uint32_t t = unit / per;
+      int c = (int)(unit - t * per);
+      const bool isk = c >= p.q.chunks;
+      const Rows& rs = isk ? p.k : p.q;
+      if (isk) c -= p.q.chunks;
+      const int h0 = c * rs.run * HW;
+      hleft = rs.H - h0;
+      left = min(rs.run, (hleft + HW - 1) / HW);
+      x = rs.x + ((int64_t)t * rs.x_ts + (int64_t)(h0 + sub) * rs.x_hs) * 2 + gl * 16;
+      xs = rs.x_hs * 2 * HW;
+      int slot = -1;
+      int64_t row = -1;
+      if (p.pool && (isk || !p.positions)) row = slots.row(p, t, lane, slot, isk);
+      if (p.R > 0) {
+        const int64_t tr = (int64_t)table_row(p, t, slot, lane) * (p.R / 2);
+        for (int i = lane; i < p.R / 4; i += 32)
+          cp16(tables + (share_in % S) * p.R * 4 + i * 16, (i < p.R / 8 ? p.cos : p.sin - p.R / 2) + tr + i * 4);
       }
-      *reinterpret_cast<uint4*>(yt + ((int64_t)h * rs.y_hs + v * 8) * 2) = pack8<DT>(f);
+      if (lane == 0) {
+        uint8_t* y = p.pool && isk ? (row < 0 ? nullptr : p.pool + row * p.D * 2)
+                                   : rs.y + ((int64_t)t * rs.y_ts + (int64_t)h0 * rs.y_hs) * 2;
+        s_share[warp][share_in % S] = Share{y, min(hleft, rs.run * HW), isk};
+      }
+      ++share_in;
+      unit += walk.step;
+    }
+    if (left > 0) {
+      const uint32_t dst = base + (row_in % S) * STAGE;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (FULL && HW == 1) {
+          cp16(dst + j * 512, x + G * 16 * j);
+        } else {
+          const bool there = (HW == 1 || sub < hleft) && on[j];
+          cp16_if(dst + j * 512, there ? x + G * 16 * j : rs0, there);
+        }
+      }
+      x += xs;
+      hleft -= HW;
+      ++row_in;
+      --left;
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue();
+  // ---- the computing side
+  F2 w[NV][4];
+  int whose = -1;
+  uint32_t row_out = 0;
+  for (uint32_t u = walk.first, share = 0; u < walk.end; u += walk.step, ++share) {
+    uint8_t* y = nullptr;
+    int64_t ys = 0;
+    int n = 1, hn = 1;
+    bool hasw = false;
+    const float* wt = nullptr;
+    for (int i = 0; i < n; ++i) {
+      issue();
+      cp_wait<S - 1>();
+      __syncwarp();
+      if (i == 0) {
+        const Share sh = s_share[warp][share % S];
+        const Rows& rs = sh.isk ? p.k : p.q;
+        hn = sh.n;
+        n = (hn + HW - 1) / HW;
+        ys = rs.y_hs * 2 * HW;
+        y = sh.y ? sh.y + (int64_t)sub * rs.y_hs * 2 + gl * 16 : nullptr;
+        wt = rs.w;
+        hasw = wt != nullptr;
+        if (hasw && whose != sh.isk) {
+          whose = sh.isk;
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (on[j]) weight8(wt, gl + G * j, w[j]);
+        }
+      }
+      const uint4* xr = reinterpret_cast<const uint4*>(mine + (row_out % S) * STAGE);
+      F2 f[NV][4], ss(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        unpack8<DT>(xr[j * 32 + lane], f[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss = fma2(f[j][e], f[j][e], ss);
+      }
+      if (norm) {
+        const float rstd = rsqrtf(group_sum<G>(ss.lo() + ss.hi()) * invD + p.eps);
+        const F2 rr(rstd, rstd);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[j][e] = mul2(f[j][e], rr);
+        if (hasw)
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[j][e] = mul2(f[j][e], w[j][e]);
+        ss = rr;
+      } else {
+        ss = F2(1.f, 1.f);
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (at[j].angle >= 0) {
+          F2 o[4];
+          if (!INTER) {
+            unpack8<DT>(xr[at[j].partner / G * 32 + sub * G + at[j].partner % G], o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = mul2(o[e], ss);
+            if (hasw) {
+              F2 wp[4];
+              weight8(wt, at[j].partner, wp);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[e] = mul2(o[e], wp[e]);
+            }
+          }
+          turn<INTER, false>(f[j], o, reinterpret_cast<const float*>(mine + S * STAGE) + (share % S) * p.R, at[j], p.R);
+        }
+        if (y && on[j] && (HW == 1 || i * HW + sub < hn)) *reinterpret_cast<uint4*>(y + G * 16 * j) = pack8<DT>(f[j]);
+      }
+      if (y) y += ys;
+      ++row_out;
+      __syncwarp();  // the stage is overwritten next
     }
   }
 }
 
 // Backward. Blocks [0, q.blocks) take the q rows, the rest the k rows; a warp
-// walks tokens' head shares with the stride of its set's warps, and keeps the
-// weight gradient of its columns in registers. Each block adds its warps'
-// sums in order and writes one row of partials; sum_partials_kernel adds the
-// rows in order, so the result does not depend on timing.
-template <int DT, int G, int NV, int U, bool INTER, bool HASW>
-__global__ void __launch_bounds__(32 * kWarps) rope_bwd_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int HW = 32 / G;
-  extern __shared__ float red[];  // [kWarps * HW][D] (HASW)
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool isk = (int)blockIdx.x >= p.q.blocks;
+// keeps the weight gradient of its columns in registers. Each block adds its
+// warps' sums in order and writes one row of partials; sum_partials_kernel
+// adds the rows in order, so the result does not depend on timing.
+template <int DT, int G, int NV, bool FULL, bool INTER, bool HASW>
+__global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(const __grid_constant__ RopeParams p) {
+  constexpr int HW = 32 / G, S = stages_of(NV), STAGE = 2 * NV * 512;
+  static_assert(HW == 1 || FULL, "rows side by side are whole");
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G, sub = lane / G;
+  const bool isk = blockIdx.x >= p.q.blocks;
   const Rows& rs = isk ? p.k : p.q;
-  const int blk = isk ? blockIdx.x - p.q.blocks : blockIdx.x;
-  const int gl = lane % G, V = p.D >> 3;
-  const bool append = p.pool != nullptr;
+  const uint32_t blk = isk ? blockIdx.x - p.q.blocks : blockIdx.x;
+  uint8_t* mine = smem + warp * S * (STAGE + p.R * 4);
+  const uint32_t base = sas::smem_u32(mine) + lane * 16, tables = sas::smem_u32(mine) + S * STAGE;
   const bool norm = p.flags & SAS_ROPE_NORM;
-  const float sgn = (p.flags & SAS_ROPE_INVERSE) ? 1.f : -1.f;  // the transpose turns back
   const float invD = 1.f / (float)p.D;
-  float acc[NV][8];
+  bool on[NV];
+  Place at[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
-  const uint32_t units = (uint32_t)p.T * (uint32_t)rs.chunks;
-  for (uint32_t unit = blk * kWarps + warp; unit < units; unit += rs.blocks * kWarps) {
-    const uint32_t t = unit / rs.chunks;
-    const int h0 = (int)(unit - t * rs.chunks) * (U * HW) + lane / G;
-    uint4 xr[U][NV], dr[U][NV];
-    int slot = -1;
-    int64_t row = -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HW;
-      const uint8_t* xp = rs.x + ((int64_t)t * rs.x_ts + (int64_t)h * rs.x_hs) * 2;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int v = gl + G * j;
-        xr[u][j] = h < rs.H && v < V ? ldg_stream(xp + v * 16) : make_uint4(0, 0, 0, 0);
+  for (int j = 0; j < NV; ++j) {
+    on[j] = FULL || (gl + G * j) * 8 < p.D;
+    at[j] = place_of<INTER>(gl + G * j, p.D, p.R, (p.flags & SAS_ROPE_INVERSE) ? 1.f : -1.f);  // the transpose turns back
+  }
+  const uint32_t per = rs.chunks, all = (uint32_t)p.T * per;
+  const Walk walk(blk * kWarps + warp, rs.blocks * kWarps, all, p.pool ? rs.most : 0);
+  Slots slots;
+  uint32_t unit = walk.first, share_in = 0, row_in = 0;
+  int left = 0, hleft = 0;
+  bool have = true;
+  const uint8_t *x = nullptr, *dy = nullptr;
+  const int64_t xs = rs.x_hs * 2 * HW, ds = rs.dy_hs * 2 * HW, ys = rs.y_hs * 2 * HW;
+  auto issue = [&]() {
+    if (left == 0 && unit < walk.end) {
+      const uint32_t t = unit / per;
+      const int h0 = (int)(unit - t * per) * rs.run * HW;
+      hleft = rs.H - h0;
+      left = min(rs.run, (hleft + HW - 1) / HW);
+      int slot = -1;
+      int64_t row = 0;
+      x = rs.x + ((int64_t)t * rs.x_ts + (int64_t)(h0 + sub) * rs.x_hs) * 2 + gl * 16;
+      if (p.pool) row = slots.row(p, t, lane, slot, true);
+      have = row >= 0;
+      dy = (p.pool ? p.pool + (have ? row : 0) * p.D * 2 : rs.dy + (int64_t)t * rs.dy_ts * 2) +
+           (int64_t)(h0 + sub) * rs.dy_hs * 2 + gl * 16;
+      if (p.R > 0) {
+        const int64_t tr = (int64_t)table_row(p, t, slot, lane) * (p.R / 2);
+        for (int i = lane; i < p.R / 4; i += 32)
+          cp16(tables + (share_in % S) * p.R * 4 + i * 16, (i < p.R / 8 ? p.cos : p.sin - p.R / 2) + tr + i * 4);
       }
+      ++share_in;
+      unit += walk.step;
     }
-    if (append) row = slot_row(p, t, lane, slot, true);
-    const uint8_t* db = append ? p.pool + (row < 0 ? 0 : row) * p.D * 2 : rs.dy + (int64_t)t * rs.dy_ts * 2;
-    const bool have = !append || row >= 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HW;
+    if (left > 0) {
+      const uint32_t dst = base + (row_in % S) * STAGE;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int v = gl + G * j;
-        dr[u][j] = have && h < rs.H && v < V ? *reinterpret_cast<const uint4*>(db + ((int64_t)h * rs.dy_hs + v * 8) * 2)
-                                             : make_uint4(0, 0, 0, 0);
+        const bool there = (HW == 1 || sub < hleft) && on[j];
+        if (FULL && HW == 1) cp16(dst + j * 512, x + G * 16 * j);
+        else cp16_if(dst + j * 512, there ? x + G * 16 * j : rs.x, there);
+        cp16_if(dst + (NV + j) * 512, there ? dy + G * 16 * j : rs.x, there && have);
       }
+      x += xs;
+      dy += ds;
+      hleft -= HW;
+      ++row_in;
+      --left;
     }
-    Angles<INTER> an[NV];
-    if (p.R > 0) {
-      const int tr = table_row(p, t, slot, lane);
+    cp_commit();
+  };
 #pragma unroll
-      for (int j = 0; j < NV; ++j) an[j].load(p, gl + G * j, tr);
-    }
+  for (int i = 0; i < S - 1; ++i) issue();
+  const bool hasw = rs.w != nullptr;
+  F2 acc[NV][4], w[NV][4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HW;
-      float ss = 0.f, gx = 0.f;
-      float g[NV][8];
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = F2(0.f, 0.f), w[j][e] = F2(1.f, 1.f);
+    if (hasw && on[j]) weight8(rs.w, gl + G * j, w[j]);
+  }
+  uint32_t row_out = 0, share = 0;
+  for (uint32_t u = walk.first; u < walk.end; u += walk.step, ++share) {
+    const uint32_t t = u / per;
+    const int h0 = (int)(u - t * per) * rs.run * HW, hn = min(rs.H - h0, rs.run * HW);
+    uint8_t* y = rs.y + ((int64_t)t * rs.y_ts + (int64_t)(h0 + sub) * rs.y_hs) * 2 + gl * 16;
+    for (int i = 0; i * HW < hn; ++i) {
+      issue();
+      cp_wait<S - 1>();
+      __syncwarp();
+      const uint4* xr = reinterpret_cast<const uint4*>(mine + (row_out % S) * STAGE);
+      const uint4* dr = xr + NV * 32;
+      F2 f[NV][4], g[NV][4], ss(0.f, 0.f), gx(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int v = gl + G * j;
-        float x[8], o[8], w[8];
-        unpack8<DT>(xr[u][j], x);
-        unpack8<DT>(dr[u][j], g[j]);
-        if (p.R > 0 && an[j].on) {
-          if (!INTER) {
-            const int pv = v + (an[j].first ? p.R / 16 : -(p.R / 16));
-            const uint4 pr = have && h < rs.H
-                                 ? *reinterpret_cast<const uint4*>(db + ((int64_t)h * rs.dy_hs + pv * 8) * 2)
-                                 : make_uint4(0, 0, 0, 0);
-            unpack8<DT>(pr, o);
-          }
-          an[j].turn(g[j], o, sgn);
+        unpack8<DT>(xr[j * 32 + lane], f[j]);
+        unpack8<DT>(dr[j * 32 + lane], g[j]);
+        if (at[j].angle >= 0) {
+          F2 o[4];
+          if (!INTER) unpack8<DT>(dr[at[j].partner / G * 32 + sub * G + at[j].partner % G], o);
+          turn<INTER, true>(g[j], o, reinterpret_cast<const float*>(mine + S * STAGE) + (share % S) * p.R, at[j], p.R);
         }
-        if (v >= V) continue;
-        if (rs.w) weight8(rs.w, v, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss = fmaf(x[i], x[i], ss);
-          gx = fmaf(rs.w ? g[j][i] * w[i] : g[j][i], x[i], gx);
+        for (int e = 0; e < 4; ++e) {
+          ss = fma2(f[j][e], f[j][e], ss);
+          gx = fma2(mul2(g[j][e], w[j][e]), f[j][e], gx);
         }
       }
-      float rstd = 1.f, mean = 0.f;
+      float rstd = 1.f, mean = 0.f;  // mean of g * xhat
       if (norm) {
-        ss = group_sum<G>(ss);
-        gx = group_sum<G>(gx);
-        rstd = rsqrtf(ss * invD + p.eps);
-        mean = rstd * gx * invD;  // of g * xhat
+        rstd = rsqrtf(group_sum<G>(ss.lo() + ss.hi()) * invD + p.eps);
+        mean = rstd * group_sum<G>(gx.lo() + gx.hi()) * invD;
       }
-      uint8_t* yp = rs.y + ((int64_t)t * rs.y_ts + (int64_t)h * rs.y_hs) * 2;
+      const F2 r2(rstd, rstd), m2(-mean, -mean);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int v = gl + G * j;
-        if (v >= V) continue;
-        float x[8], w[8], o[8];
-        unpack8<DT>(xr[u][j], x);
-        if (rs.w) weight8(rs.w, v, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float xh = x[i] * rstd;
-          if (HASW) acc[j][i] = fmaf(g[j][i], xh, acc[j][i]);
-          o[i] = rstd * ((rs.w ? g[j][i] * w[i] : g[j][i]) - xh * mean);
+        for (int e = 0; e < 4; ++e) {
+          const F2 xh = mul2(f[j][e], r2);
+          if (HASW) acc[j][e] = fma2(g[j][e], xh, acc[j][e]);
+          f[j][e] = mul2(r2, fma2(xh, m2, mul2(g[j][e], w[j][e])));
         }
-        if (h < rs.H) *reinterpret_cast<uint4*>(yp + v * 16) = pack8<DT>(o);
+        if (on[j] && (HW == 1 || i * HW + sub < hn)) *reinterpret_cast<uint4*>(y + G * 16 * j) = pack8<DT>(f[j]);
       }
+      y += ys;
+      ++row_out;
+      __syncwarp();  // the stage is overwritten next
     }
   }
   if (HASW && rs.dw_part) {
-    float* mine = red + (warp * HW + lane / G) * p.D;
+    __syncthreads();  // every warp is done with its stages
+    float* red = reinterpret_cast<float*>(smem);  // [kWarps * HW][D]
+    float* my = red + (warp * HW + sub) * p.D;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int v = gl + G * j;
-      if (v < V)
+      if (!on[j]) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine[v * 8 + i] = acc[j][i];
+      for (int e = 0; e < 4; ++e) my[(gl + G * j) * 8 + 2 * e] = acc[j][e].lo(), my[(gl + G * j) * 8 + 2 * e + 1] = acc[j][e].hi();
     }
     __syncthreads();
     for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
@@ -491,7 +608,7 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* qp, floa
 }
 
 // --------------------------------------------------------------- host side
-int lanes_of(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : 32); }
+int lanes_of(int D) { return D == 64 ? 8 : (D == 128 ? 16 : 32); }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -522,55 +639,87 @@ int check_paged(const RopeParams& p) {
   return SAS_OK;
 }
 
-#define ROPE_SHAPES(F)                       \
-  if (g == 8) F(8, 1)                        \
-  else if (g == 16) F(16, 1)                 \
-  else if (nv == 1) F(32, 1)                 \
-  else if (nv == 2) F(32, 2)                 \
-  else F(32, 4)
+#define ROPE_SHAPES(F)                      \
+  if (D == 64) F(8, 1, true)                \
+  else if (D == 128) F(16, 1, true)         \
+  else if (D == 256) F(32, 1, true)         \
+  else if (D == 512) F(32, 2, true)         \
+  else if (D < 256) F(32, 1, false)         \
+  else if (D < 512) F(32, 2, false)         \
+  else F(32, 4, false)
 
-template <int DT, int U, bool INTER>
-void launch_fwd(const RopeParams& p, int blocks, cudaStream_t st) {
-  const int g = lanes_of(p.D), nv = (p.D / 8 + g - 1) / g;
-#define F(G, NV) rope_fwd_kernel<DT, G, NV, U, INTER><<<blocks, 32 * kWarps, 0, st>>>(p);
+int vectors_of(int D) {
+  const int nv = (D / 8 + lanes_of(D) - 1) / lanes_of(D);
+  return nv == 3 ? 4 : nv;
+}
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+  return n;
+}
+
+// How T tokens of the sets a and b (b may be nullptr) are shared out over at
+// most `warps` warps: rows of a share (up to most_rows) and shares of a warp. The
+// slowest warp's time counts: its rows, and about two rows' more per share.
+// Measured for 16384 x 64 x 512 forward: up to 8 rows 335 us, 6 377, 16 371;
+// 8192 x 64 x 512 backward: up to 4 rows 250 us, 3 257, 8 293.
+bool share_out(int64_t T, Rows* a, Rows* b, int hw, int64_t warps, int most_rows, uint32_t* most) {
+  double best = 0;
+  for (int run = most_rows; run >= 1; --run) {
+    const int64_t ca = (a->H + run * hw - 1) / (run * hw), cb = b ? (b->H + run * hw - 1) / (run * hw) : 0;
+    const int64_t units = T * (ca + cb), per = (units + warps - 1) / warps;
+    if (units >= (1ll << 31) || per * warps >= (1ll << 32)) return false;
+    const int64_t widest = a->H > (b ? b->H : 0) ? a->H : b ? b->H : a->H;
+    const int64_t rows = (widest + hw - 1) / hw < run ? (widest + hw - 1) / hw : run;
+    const double cost = (double)per * ((double)rows + 2);
+    if (best == 0 || cost < best) {
+      best = cost;
+      a->run = run, a->chunks = (int)ca;
+      if (b) b->run = run, b->chunks = (int)cb;
+      *most = (uint32_t)(per > 0 ? per : 1);
+    }
+  }
+  return true;
+}
+
+template <typename K>
+int launch(K kern, const RopeParams& p, int blocks, int smem, cudaStream_t st) {
+  if (smem > 47 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return SAS_ERR_CUDA;
+  kern<<<blocks, 32 * kWarps, smem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
+}
+
+template <int DT, bool INTER>
+int launch_fwd(const RopeParams& p, int blocks, int smem, cudaStream_t st) {
+  const int D = p.D;
+#define F(G, NV, FULL) return launch(rope_fwd_kernel<DT, G, NV, FULL, INTER>, p, blocks, smem, st);
   ROPE_SHAPES(F)
 #undef F
 }
 
-// Rows in flight per lane group: 4 once the call has enough warps to fill the
-// GPU that way, else 1, so that a decode step's few rows spread over all SMs.
 int fwd(RopeParams& p, int dtype, cudaStream_t st) {
   if (p.T == 0) return SAS_OK;
-  const int hw = 32 / lanes_of(p.D);
-  const int64_t rows = (int64_t)p.T * ((p.q.H + hw - 1) / hw);
-  const int U = rows >= 148 * 64 * 4 ? 4 : 1;
-  p.q.chunks = (p.q.H + U * hw - 1) / (U * hw);
-  p.k.chunks = (p.k.H + U * hw - 1) / (U * hw);
-  const int64_t blocks = ((int64_t)p.T * (p.q.chunks + p.k.chunks) + kWarps - 1) / kWarps;
-  if (blocks * kWarps >= (1ll << 31)) return SAS_ERR_UNSUPPORTED;
+  const int hw = 32 / lanes_of(p.D), nv = vectors_of(p.D);
   const bool inter = p.flags & SAS_ROPE_INTERLEAVED;
-#define GO(DT, U_)                                       \
-  (inter ? launch_fwd<DT, U_, true>(p, (int)blocks, st)  \
-         : launch_fwd<DT, U_, false>(p, (int)blocks, st))
-  if (dtype == SAS_DTYPE_BF16) {
-    if (U == 4) GO(SAS_DTYPE_BF16, 4); else GO(SAS_DTYPE_BF16, 1);
-  } else {
-    if (U == 4) GO(SAS_DTYPE_FP16, 4); else GO(SAS_DTYPE_FP16, 1);
-  }
-#undef GO
-  return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
+  const int64_t most = (int64_t)sm_count() * fwd_blocks(nv);
+  if (!share_out(p.T, &p.q, &p.k, hw, most * kWarps, 8, &p.most)) return SAS_ERR_UNSUPPORTED;
+  const int64_t fit = ((int64_t)p.T * (p.q.chunks + p.k.chunks) + kWarps - 1) / kWarps;
+  const int blocks = (int)(fit < most ? fit : most);
+  const int smem = kWarps * stages_of(nv) * (nv * 512 + p.R * 4);
+  if (dtype == SAS_DTYPE_BF16)
+    return inter ? launch_fwd<SAS_DTYPE_BF16, true>(p, blocks, smem, st) : launch_fwd<SAS_DTYPE_BF16, false>(p, blocks, smem, st);
+  return inter ? launch_fwd<SAS_DTYPE_FP16, true>(p, blocks, smem, st) : launch_fwd<SAS_DTYPE_FP16, false>(p, blocks, smem, st);
 }
 
-constexpr int kBwdBlocks = 148 * 4;  // most blocks of a set of rows; its partials are one row of D floats per block
+constexpr int kBwdBlocks = 148 * 2;  // most blocks of a set of rows; its partials are one row of D floats per block
 
 template <int DT, bool INTER, bool HASW>
-int launch_bwd(const RopeParams& p, cudaStream_t st) {
-  const int g = lanes_of(p.D), nv = (p.D / 8 + g - 1) / g;
-  const size_t smem = HASW ? (size_t)kWarps * (32 / g) * p.D * 4 : 0;  // at most 32 KB
-#define F(G, NV) rope_bwd_kernel<DT, G, NV, 1, INTER, HASW><<<p.q.blocks + p.k.blocks, 32 * kWarps, smem, st>>>(p);
+int launch_bwd(const RopeParams& p, int smem, cudaStream_t st) {
+  const int D = p.D;
+#define F(G, NV, FULL) return launch(rope_bwd_kernel<DT, G, NV, FULL, INTER, HASW>, p, p.q.blocks + p.k.blocks, smem, st);
   ROPE_SHAPES(F)
 #undef F
-  return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
 
 int bwd(RopeParams& p, int dtype, float* dqw, float* dkw, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -582,20 +731,21 @@ int bwd(RopeParams& p, int dtype, float* dqw, float* dkw, void* ws, size_t ws_by
     if (dkw && cudaMemsetAsync(dkw, 0, p.D * 4, st) != cudaSuccess) return SAS_ERR_CUDA;
     return SAS_OK;
   }
-  const int hw = 32 / lanes_of(p.D);
+  const int hw = 32 / lanes_of(p.D), nv = vectors_of(p.D);
   for (Rows* r : {&p.q, &p.k}) {
-    r->chunks = (r->H + hw - 1) / hw;
-    const int64_t units = (int64_t)p.T * r->chunks;
-    if (units >= (1ll << 31) - kBwdBlocks * kWarps) return SAS_ERR_UNSUPPORTED;
-    r->blocks = (int)((units + kWarps - 1) / kWarps < kBwdBlocks ? (units + kWarps - 1) / kWarps : kBwdBlocks);
+    if (!share_out(p.T, r, nullptr, hw, kBwdBlocks * kWarps, 4, &r->most)) return SAS_ERR_UNSUPPORTED;
+    const int64_t fit = ((int64_t)p.T * r->chunks + kWarps - 1) / kWarps;
+    r->blocks = (uint32_t)(fit < kBwdBlocks ? fit : kBwdBlocks);
   }
   p.q.dw_part = dqw ? static_cast<float*>(ws) : nullptr;
   p.k.dw_part = dkw ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part) : nullptr;
   const bool inter = p.flags & SAS_ROPE_INTERLEAVED, hasw = dqw || dkw;
+  int smem = kWarps * stages_of(nv) * (2 * nv * 512 + p.R * 4);
+  if (hasw && smem < kWarps * hw * p.D * 4) smem = kWarps * hw * p.D * 4;
   int rc;
-#define GO(DT)                                                                                              \
-  rc = inter ? (hasw ? launch_bwd<DT, true, true>(p, st) : launch_bwd<DT, true, false>(p, st))             \
-             : (hasw ? launch_bwd<DT, false, true>(p, st) : launch_bwd<DT, false, false>(p, st))
+#define GO(DT)                                                                                                          \
+  rc = inter ? (hasw ? launch_bwd<DT, true, true>(p, smem, st) : launch_bwd<DT, true, false>(p, smem, st))             \
+             : (hasw ? launch_bwd<DT, false, true>(p, smem, st) : launch_bwd<DT, false, false>(p, smem, st))
   if (dtype == SAS_DTYPE_BF16) GO(SAS_DTYPE_BF16); else GO(SAS_DTYPE_FP16);
 #undef GO
   if (rc != SAS_OK || !hasw) return rc;
@@ -614,8 +764,8 @@ int sas_head_norm_rope_fwd(const void* q, int64_t q_ts, int64_t q_hs, void* q_ou
                            const float* cos, const float* sin, int32_t P, int32_t R, const float* q_weight,
                            const float* k_weight, float eps, int32_t flags, int32_t* status, void* stream) {
   RopeParams p = {};
-  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(q_out), qo_ts, qo_hs, nullptr, 0, 0, q_weight, nullptr, H, 0, 0};
-  p.k = {static_cast<const uint8_t*>(k), k_ts, k_hs, static_cast<uint8_t*>(k_out), ko_ts, ko_hs, nullptr, 0, 0, k_weight, nullptr, Hk, 0, 0};
+  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(q_out), qo_ts, qo_hs, nullptr, 0, 0, q_weight, nullptr, H};
+  p.k = {static_cast<const uint8_t*>(k), k_ts, k_hs, static_cast<uint8_t*>(k_out), ko_ts, ko_hs, nullptr, 0, 0, k_weight, nullptr, Hk};
   p.T = T, p.D = D, p.R = R, p.P = P, p.flags = flags, p.eps = eps;
   p.positions = positions, p.cos = cos, p.sin = sin, p.status = status;
   const int rc = check(p, dtype, false);
@@ -636,8 +786,8 @@ int sas_head_norm_rope_bwd(const void* dq_out, int64_t dqo_ts, int64_t dqo_hs, c
                            size_t workspace_bytes, void* stream) {
   RopeParams p = {};
   const int64_t ts = (int64_t)H * D, tsk = (int64_t)Hk * D;  // dq, dk are dense
-  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(dq), ts, D, static_cast<const uint8_t*>(dq_out), dqo_ts, dqo_hs, q_weight, nullptr, H, 0, 0};
-  p.k = {static_cast<const uint8_t*>(k), k_ts, k_hs, static_cast<uint8_t*>(dk), tsk, D, static_cast<const uint8_t*>(dk_out), dko_ts, dko_hs, k_weight, nullptr, Hk, 0, 0};
+  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(dq), ts, D, static_cast<const uint8_t*>(dq_out), dqo_ts, dqo_hs, q_weight, nullptr, H};
+  p.k = {static_cast<const uint8_t*>(k), k_ts, k_hs, static_cast<uint8_t*>(dk), tsk, D, static_cast<const uint8_t*>(dk_out), dko_ts, dko_hs, k_weight, nullptr, Hk};
   p.T = T, p.D = D, p.R = R, p.P = P, p.flags = flags, p.eps = eps;
   p.positions = positions, p.cos = cos, p.sin = sin, p.status = status;
   const int rc = check(p, dtype, true);
@@ -654,8 +804,8 @@ int sas_append_sharedkv(const void* kv, int64_t kv_ts, void* pool, int64_t nblk,
                         const float* cos, const float* sin, int32_t P, int32_t R, const float* kv_weight,
                         const float* q_weight, float eps, int32_t flags, int32_t* status, void* stream) {
   RopeParams p = {};
-  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(q_out), qo_ts, qo_hs, nullptr, 0, 0, q_weight, nullptr, H, 0, 0};
-  p.k = {static_cast<const uint8_t*>(kv), kv_ts, 0, nullptr, 0, 0, nullptr, 0, 0, kv_weight, nullptr, 1, 0, 0};
+  p.q = {static_cast<const uint8_t*>(q), q_ts, q_hs, static_cast<uint8_t*>(q_out), qo_ts, qo_hs, nullptr, 0, 0, q_weight, nullptr, H};
+  p.k = {static_cast<const uint8_t*>(kv), kv_ts, 0, nullptr, 0, 0, nullptr, 0, 0, kv_weight, nullptr, 1};
   p.T = T, p.D = D, p.R = R, p.P = P, p.flags = flags, p.eps = eps;
   p.positions = positions, p.cos = cos, p.sin = sin, p.status = status;
   p.pool = static_cast<uint8_t*>(pool), p.nblk = nblk, p.bs = bs, p.bt = block_table, p.bt_stride = bt_stride;
@@ -675,7 +825,7 @@ int sas_append_sharedkv_bwd(const void* d_pool, int64_t nblk, int32_t bs, const 
                             int32_t R, const float* kv_weight, float* dkv_weight, float eps, int32_t flags,
                             int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
   RopeParams p = {};
-  p.k = {static_cast<const uint8_t*>(kv), kv_ts, 0, static_cast<uint8_t*>(dkv), D, 0, nullptr, 0, 0, kv_weight, nullptr, 1, 0, 0};
+  p.k = {static_cast<const uint8_t*>(kv), kv_ts, 0, static_cast<uint8_t*>(dkv), D, 0, nullptr, 0, 0, kv_weight, nullptr, 1};
   p.T = T, p.D = D, p.R = R, p.P = P, p.flags = flags, p.eps = eps;
   p.positions = positions, p.cos = cos, p.sin = sin, p.status = status;
   p.pool = const_cast<uint8_t*>(static_cast<const uint8_t*>(d_pool));  // read only here

@@ -42,41 +42,52 @@ def _dtype_code(t: torch.dtype) -> int:
 
 
 def _i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
+        return t
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _f32(t: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    t = t.detach().to(device=dev, dtype=torch.float32).contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
+        t = t.to(device=dev, dtype=torch.float32).contiguous()
+    return t if t.data_ptr() & 15 == 0 else t.clone()
 
 
-class _Rows:
-    """[..., H, D] as [T, H, D] with the strides the kernel takes; copied only where it cannot take them."""
+_NO_ROWS = (0, 0, 0)
 
-    def __init__(self, t: Optional[torch.Tensor], name: str, out: bool = False):
-        if t is None:
-            self.t, self.T, self.H, self.args = None, 0, 0, (0, 0, 0)
-            return
-        T, H, D = t.numel() // (t.shape[-2] * t.shape[-1]) if t.numel() else 0, t.shape[-2], t.shape[-1]
-        r = t
-        if T:
-            try:
-                r = t.view(T, H, D)
-            except RuntimeError:
-                if out:
-                    raise ValueError(f"{name}: the token dims must have one stride") from None
-                r = t.reshape(T, H, D)
-            bad = (D > 1 and r.stride(2) != 1) or r.data_ptr() % 16 or (H > 1 and r.stride(1) % 8) or \
-                (T > 1 and r.stride(0) % 8)
-            if bad:
-                if out:
-                    raise ValueError(f"{name} must have a contiguous last dim and 16-byte aligned rows")
-                r = r.contiguous() if not r.is_contiguous() else r.clone()
-        self.t, self.T, self.H = r, T, H
-        ts, hs = (r.stride(0) if T > 1 else H * D, r.stride(1) if H > 1 else D) if T else (H * D, D)
-        self.args = (r.data_ptr(), ts, hs)
+
+def _rows(t: torch.Tensor, name: str, out: bool = False):
+    """``t [..., H, D]`` as the kernel takes it, ``(tensor, (pointer, token stride, head stride))``: copied only
+    where a stride or an address does not fit."""
+    shape = t.shape
+    H, D = shape[-2], shape[-1]
+    at = t.data_ptr()
+    if at & 15 == 0 and t.is_contiguous():
+        return t, (at, H * D, D)
+    T = shape[:-2].numel()
+    if T == 0:
+        return t, (at, H * D, D)
+    try:
+        r = t.view(T, H, D)
+    except RuntimeError:
+        if out:
+            raise ValueError(f"{name}: the token dims must have one stride") from None
+        r = t.reshape(T, H, D)
+    ts, hs = (r.stride(0) if T > 1 else H * D), (r.stride(1) if H > 1 else D)
+    if r.stride(2) != 1 or r.data_ptr() & 15 or (ts | hs) & 7:
+        if out:
+            raise ValueError(f"{name} must have a contiguous last dim and 16-byte aligned rows")
+        r = r.clone(memory_format=torch.contiguous_format)
+        ts, hs = H * D, D
+    return r, (r.data_ptr(), ts, hs)
+
+
+def _new(like: torch.Tensor) -> torch.Tensor:
+    if like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
 def _rope_args(dev, D, T, positions, cos, sin, norm, inverse, interleaved, slots=False):
@@ -104,7 +115,7 @@ def _rope_args(dev, D, T, positions, cos, sin, norm, inverse, interleaved, slots
 
 
 def _to_dev(dev, positions, cos, sin):
-    if positions is not None:
+    if positions is not None and (positions.device != dev or not positions.is_contiguous()):
         positions = positions.to(dev).contiguous()
     return positions, _f32(cos, dev), _f32(sin, dev)
 
@@ -121,8 +132,8 @@ def _check_pair(q, k):
     if q.dim() < 2 or q.shape[-2] < 1:
         raise ValueError(f"q must be [..., heads, D] (got {tuple(q.shape)})")
     if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]
-                          or k.shape[-2] < 1 or k.dtype != q.dtype):
-        raise ValueError("k must have q's token dims, head dim and dtype")
+                          or k.shape[-2] < 1 or k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("k must have q's token dims, head dim, dtype and device")
 
 
 def _check_out(out, like, name):
@@ -175,18 +186,23 @@ def head_norm_rope(
         raise RuntimeError("head_norm_rope needs CUDA tensors (no CPU path)")
     dev = q.device
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        q_out = _new(q)
     if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        k_out = _new(k)
     if T:
         positions, cos, sin = _to_dev(dev, positions, cos, sin)
         qw, kw = _f32(q_weight, dev), _f32(k_weight if k is not None else None, dev)
-        a, b = _Rows(q.detach(), "q"), _Rows(q_out, "q_out", out=True)
-        c, d = _Rows(k.detach() if k is not None else None, "k"), _Rows(k_out if k is not None else None, "k_out", out=True)
+        q, qa = _rows(q, "q")
+        _, qo = _rows(q_out, "q_out", out=True)
+        ka = ko = _NO_ROWS
+        Hk = 0
+        if k is not None:
+            Hk = k.shape[-2]
+            k, ka = _rows(k, "k")
+            _, ko = _rows(k_out, "k_out", out=True)
         rc = _lib.lib().sas_head_norm_rope_fwd(
-            *a.args, *b.args, a.H, *c.args, *d.args, c.H, T, D, code, _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin),
-            P, R, _lib.ptr(qw), _lib.ptr(kw), float(eps), flags, _lib.state(dev).status.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream)
+            *qa, *qo, q.shape[-2], *ka, *ko, Hk, T, D, code, _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), P, R,
+            _lib.ptr(qw), _lib.ptr(kw), float(eps), flags, _lib.state(dev).status.data_ptr(), _lib.raw_stream(dev))
         _raise(rc, "head_norm_rope", "sas_head_norm_rope_fwd")
     return q_out if k is None else (q_out, k_out)
 
@@ -219,11 +235,13 @@ def head_norm_rope_backward(
     positions, cos, sin, P, R, flags = _rope_args(q.device, D, T, positions, cos, sin, norm, inverse, interleaved)
     if dq_out.shape != q.shape or (k is not None and (dk_out is None or dk_out.shape != k.shape)):
         raise ValueError("dq_out and dk_out must have the shapes of q and k")
+    if dq_out.device != q.device or (k is not None and dk_out.device != q.device):
+        raise ValueError("dq_out and dk_out must be on the device of q and k")
     if not q.is_cuda:
         raise RuntimeError("head_norm_rope_backward needs CUDA tensors (no CPU path)")
     dev = q.device
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if k is not None else None
+    dq = _new(q)
+    dk = _new(k) if k is not None else None
     qw = _f32(q_weight, dev)
     kw = _f32(k_weight, dev) if k is not None else None
     dqw = torch.empty(D, dtype=torch.float32, device=dev) if qw is not None else None
@@ -231,16 +249,20 @@ def head_norm_rope_backward(
     lib = _lib.lib()
     st = _lib.state(dev)
     positions, cos, sin = _to_dev(dev, positions, cos, sin)
-    a, da = _Rows(q.detach(), "q"), _Rows(dq_out.to(q.dtype), "dq_out")
-    b = _Rows(k.detach() if k is not None else None, "k")
-    db = _Rows(dk_out.to(q.dtype) if k is not None else None, "dk_out")
+    q, qa = _rows(q, "q")
+    dq_out, da = _rows(dq_out.to(q.dtype), "dq_out")
+    ka = db = _NO_ROWS
+    Hk = 0
+    if k is not None:
+        Hk = k.shape[-2]
+        k, ka = _rows(k, "k")
+        dk_out, db = _rows(dk_out.to(q.dtype), "dk_out")
     ws = torch.empty(lib.sas_head_norm_rope_bwd_workspace_bytes(D), dtype=torch.uint8, device=dev) \
         if qw is not None or kw is not None else None
     rc = lib.sas_head_norm_rope_bwd(
-        *da.args, *a.args, dq.data_ptr(), a.H, *db.args, *b.args, _lib.ptr(dk), b.H, T, D, code, _lib.ptr(positions),
-        _lib.ptr(cos), _lib.ptr(sin), P, R, _lib.ptr(qw), _lib.ptr(kw), _lib.ptr(dqw), _lib.ptr(dkw), float(eps), flags,
-        st.status.data_ptr(), _lib.ptr(ws), ws.numel() if ws is not None else 0,
-        torch.cuda.current_stream(dev).cuda_stream) if T else 0
+        *da, *qa, dq.data_ptr(), q.shape[-2], *db, *ka, _lib.ptr(dk), Hk, T, D, code, _lib.ptr(positions), _lib.ptr(cos),
+        _lib.ptr(sin), P, R, _lib.ptr(qw), _lib.ptr(kw), _lib.ptr(dqw), _lib.ptr(dkw), float(eps), flags, st.status.data_ptr(),
+        _lib.ptr(ws), ws.numel() if ws is not None else 0, _lib.raw_stream(dev)) if T else 0
     _raise(rc, "head_norm_rope_backward", "sas_head_norm_rope_bwd")
     if not T:
         dqw, dkw = (None if w is None else w.zero_() for w in (dqw, dkw))
@@ -358,18 +380,22 @@ def append_shared_kv(
     if ori_kv.device != dev or (q is not None and q.device != dev):
         raise ValueError("kv, ori_kv and q must be on one device")
     if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        q_out = _new(q)
     if T:
         p.put(dev)
         positions, cos, sin = _to_dev(dev, positions, cos, sin)
         w, qw = _f32(weight, dev), _f32(q_weight if q is not None else None, dev)
-        r = _Rows(p.kv.detach(), "kv")
-        a = _Rows(q.detach() if q is not None else None, "q")
-        b = _Rows(q_out if q is not None else None, "q_out", out=True)
+        r, ra = _rows(p.kv, "kv")
+        qa = qo = _NO_ROWS
+        H = 0
+        if q is not None:
+            H = q.shape[-2]
+            q, qa = _rows(q, "q")
+            _, qo = _rows(q_out, "q_out", out=True)
         rc = _lib.lib().sas_append_sharedkv(
-            *r.args[:2], ori_kv.data_ptr(), *p.args(), *a.args, *b.args, a.H, T, D, code, _lib.ptr(positions),
-            _lib.ptr(cos), _lib.ptr(sin), P, R, _lib.ptr(w), _lib.ptr(qw), float(eps), flags,
-            _lib.state(dev).status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+            *ra[:2], ori_kv.data_ptr(), *p.args(), *qa, *qo, H, T, D, code, _lib.ptr(positions), _lib.ptr(cos),
+            _lib.ptr(sin), P, R, _lib.ptr(w), _lib.ptr(qw), float(eps), flags, _lib.state(dev).status.data_ptr(),
+            _lib.raw_stream(dev))
         _raise(rc, "append_shared_kv", "sas_append_sharedkv")
     return ori_kv if q is None else (ori_kv, q_out)
 
@@ -405,7 +431,7 @@ def append_shared_kv_backward(
     dev = kv.device
     if d_ori_kv.device != dev:
         raise ValueError("kv and d_ori_kv must be on one device")
-    dkv = torch.empty(kv.shape, dtype=kv.dtype, device=dev)
+    dkv = _new(kv)
     w = _f32(weight, dev)
     dw = torch.zeros(D, dtype=torch.float32, device=dev) if w is not None and not T else \
         torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None
@@ -413,12 +439,12 @@ def append_shared_kv_backward(
         lib = _lib.lib()
         p.put(dev)
         positions, cos, sin = _to_dev(dev, positions, cos, sin)
-        r = _Rows(p.kv.detach(), "kv")
+        r, ra = _rows(p.kv, "kv")
         ws = torch.empty(lib.sas_head_norm_rope_bwd_workspace_bytes(D), dtype=torch.uint8, device=dev) \
             if w is not None else None
         rc = lib.sas_append_sharedkv_bwd(
-            d_ori_kv.data_ptr(), *p.args(), *r.args[:2], dkv.data_ptr(), T, D, code, _lib.ptr(positions), _lib.ptr(cos),
+            d_ori_kv.data_ptr(), *p.args(), *ra[:2], dkv.data_ptr(), T, D, code, _lib.ptr(positions), _lib.ptr(cos),
             _lib.ptr(sin), P, R, _lib.ptr(w), _lib.ptr(dw), float(eps), flags, _lib.state(dev).status.data_ptr(),
-            _lib.ptr(ws), ws.numel() if ws is not None else 0, torch.cuda.current_stream(dev).cuda_stream)
+            _lib.ptr(ws), ws.numel() if ws is not None else 0, _lib.raw_stream(dev))
         _raise(rc, "append_shared_kv_backward", "sas_append_sharedkv_bwd")
     return dkv, dw

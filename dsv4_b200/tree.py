@@ -16,7 +16,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .rope import LAYOUTS, _dtype_code, _i32
+from .rope import LAYOUTS, _dtype_code, _f32, _i32
 
 HEAD_DIM = 512
 MAX_TREE = 1024
@@ -112,9 +112,9 @@ def tree_attn_sharedkv(
     if not q.is_cuda:
         raise RuntimeError("tree_attn_sharedkv needs q on a CUDA device (no CPU path)")
     dev = q.device
-    q = _aligned(q.detach())
+    q = _aligned(q)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q)
     if lse_out is None and return_softmax_lse:
         lse_out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
     if T:
@@ -122,11 +122,11 @@ def tree_attn_sharedkv(
         st = _lib.state(dev)
         cu = _i32(cu_seqlens_q, dev) if cu_seqlens_q is not None else None
         skv, par = _i32(seqused_kv, dev), _i32(tree_parents, dev)
-        snk = sinks.detach().to(device=dev, dtype=torch.float32).contiguous()
-        ori, obt = _aligned(ori_kv.detach().to(dev)), _i32(ori_block_table, dev)
+        snk = _f32(sinks, dev)
+        ori, obt = _aligned(ori_kv.to(dev)), _i32(ori_block_table, dev)
         cmp = cbt = idx = None
         if scenario >= 2:
-            cmp, cbt = _aligned(cmp_kv.detach().to(dev)), _i32(cmp_block_table, dev)
+            cmp, cbt = _aligned(cmp_kv.to(dev)), _i32(cmp_block_table, dev)
         if scenario == 3:
             idx = _i32(cmp_sparse_indices, dev)
         # from the allocator, so that calls on several streams do not share it
@@ -137,7 +137,7 @@ def tree_attn_sharedkv(
             0 if cmp is None else cmp.shape[0], 0 if cmp is None else cmp.shape[1], _lib.ptr(cbt),
             0 if cbt is None else cbt.shape[1], _lib.ptr(idx), K, snk.data_ptr(), float(softmax_scale), int(ratio),
             min(int(ori_win_left), 1 << 30), scenario, out.data_ptr(), _lib.ptr(lse_out), st.num_sms,
-            st.status.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+            st.status.data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(dev))
         if rc in (1, 2):
             raise ValueError(f"tree_attn_sharedkv: {_lib.ERRORS[rc]}")
         _lib.check(rc, "sas_tree_attn_sharedkv")
@@ -146,4 +146,4 @@ def tree_attn_sharedkv(
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() & 15 == 0 else t.clone()

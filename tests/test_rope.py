@@ -191,6 +191,10 @@ CASES = [  # T, H, Hk, D, R, interleaved, q weight, k weight
     (700, 56, 1, 512, 64, True, True, True),  # several rows in flight, many partial sums
     (701, 57, 1, 512, 64, False, True, True),
     (3, 1, 1, 768, 96, False, False, True),
+    (310, 40, 8, 128, 128, False, True, True),
+    (2, 3, 1, 1024, 1024, False, True, True),  # the most shared memory
+    (50, 9, 2, 256, 64, True, True, False),
+    (4, 2, 0, 320, 48, True, True, False),
 ]
 
 
