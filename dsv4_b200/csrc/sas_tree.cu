@@ -8,41 +8,50 @@
 //   compressed rows below ctx // ratio: all of them, or its top-k list.
 // o = sum_j p_j v_j / (sum_j p_j + e^sink),  p_j = e^(scale q.k_j),  K = V.
 //
-// Work: one unit is 64 (token, head) rows of one request, in order, so a
-// request's units read the same rows; with top-k lists a unit is 64 heads of
+// Work: one unit is 128 (token, head) rows of one request, in order, so a
+// request's units read the same rows; with top-k lists a unit is 128 heads of
 // one token. A unit's rows of KV come in tiles of 128: the window (cached and
 // drafted rows together), then the compressed ones. All tiles of all units
-// form one sequence that is cut into equal ranges, one per CTA; a unit cut by
-// a range's end leaves partial sums that tree_combine_kernel joins in order.
+// form one sequence that is cut into equal ranges, one per pair of CTAs; a unit
+// cut by a range's end leaves partial sums that tree_combine_kernel joins in order.
 //
-// Per tile, S[64 x 128] = Q K^T and O[64 x 512] += P V are tcgen05.mma.ws with
-// M = 64: weight-stationary because its M = 64 accumulators use all 128 TMEM
-// lanes (lanes 64-127 hold the upper half of the columns), so O takes 256
-// columns and the next scores fit beside it, and because it runs at 0.66
-// (N = 128) to 0.80 (N = 256) of the full rate where plain M = 64 stops at 0.5
-// (48.2 and 80.2 cycles measured). A tile's 128 KB are resident once and read
-// as K (K-major) and as V (MN-major). The softmax is one pass with a running
-// maximum that moves, and rescales O, only when a row's maximum rises by more
-// than 2^8: P then stays below 2^8, and P, l and O keep one common scale.
-// P is rounded to the I/O type for the product, l sums it unrounded (as the
-// framework's forward does).
+// A pair of CTAs (one cluster) works on a unit, 64 rows each, with tcgen05.mma
+// over both SMs (cta_group::2, M = 128): S[128 x 128] = Q K^T, each CTA
+// bringing 64 of the tile's rows as K, and O[128 x 512] += P V, each bringing
+// 256 of the 512 columns as V. Why: O of 128 rows fills the tensor memory of
+// one SM, of 64 rows half of it, but one SM's M = 64 runs at half rate (64
+// cycles for N = 128; 48 in the weight-stationary form), where the pair runs at
+// 45.6 (N = 128) and the full rate of 64 (N = 256), all measured; and K and V,
+// 64 KB each, are then separate buffers, so that the next tile's K is copied
+// and multiplied while this tile's softmax runs. The accumulators use all 128
+// TMEM lanes (lanes 64-127 hold the upper half of the columns): O takes 256
+// columns, two buffers of S 64 each.
+// The softmax is one pass with a running maximum that moves, and rescales O,
+// only when a row's maximum rises by more than 2^8: P then stays below 2^8, and
+// P, l and O keep one common scale. P is rounded to the I/O type for the
+// product, l sums it unrounded (as the framework's forward does).
 //
 // Roles (14 warps): 0-3 softmax and epilogue (thread = row, half of the tile's
-// columns), 4 MMA issuer, 5 coordinator (walks the range and the trees and
-// publishes tiles in a ring), 6-13 loaders (cp.async, 16 rows of a tile each).
+// columns), 4 MMA issuer (in the pair's second CTA it passes on that its copies
+// have landed), 5 coordinator (walks the range and the trees and publishes
+// tiles in a ring; the pair's two coordinators take the same steps), 6-13
+// loaders (cp.async; 8 K rows and 16 V half rows of a tile each).
 #include "sas_common.cuh"
 
 namespace {
 
 constexpr int D = 512;
-constexpr int MR = 64;    // rows of a unit
+constexpr int MR = 64;    // rows of a CTA
+constexpr int UR = 128;   // rows of a unit
 constexpr int CH = 128;   // KV rows of a tile
-constexpr int kMaxTok = 8;      // tokens of a unit: heads are a multiple of 8
+constexpr int kMaxTok = 8;      // tokens of a CTA's rows: heads are a multiple of 8
+constexpr int kMaxUnitTok = 16;
 constexpr int kMaxTree = 1024;  // drafted tokens of a request
 constexpr int kWords = kMaxTree / 32;
 constexpr int kMaxCtx = 1 << 30;  // rows cached before them
-constexpr int SLAB = CH * 128;    // 64 columns of a tile
-constexpr int QSLAB = MR * 128;   // 64 columns of Q, or 64 rows' P
+constexpr int KSLAB = 64 * 128;   // 64 columns of the CTA's 64 K rows
+constexpr int VSLAB = CH * 128;   // 64 columns of the tile's V rows
+constexpr int QSLAB = MR * 128;   // 64 columns of Q, or of P
 constexpr int kMmaWarp = 4, kCoordWarp = 5, kLoadWarp0 = 6, kLoadWarps = 8;
 constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
 constexpr int kRing = 4;          // tiles the coordinator may be ahead
@@ -52,12 +61,15 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMove = 8.f;      // log2 units the running maximum may lag
 
 constexpr int OFF_Q = 0;
-constexpr int OFF_KV = OFF_Q + 8 * QSLAB;
-constexpr int OFF_P = OFF_KV + 8 * SLAB;
+constexpr int OFF_K = OFF_Q + 8 * QSLAB;
+constexpr int OFF_V = OFF_K + 8 * KSLAB;
+constexpr int OFF_P = OFF_V + 4 * VSLAB;
 constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
 
-enum Bar { B_FULL = 0, B_EMPTY = 2, B_QFULL = 4, B_QEMPTY, B_VFULL, B_SFULL, B_PREADY, B_OFULL, B_OEMPTY, B_SSYNC,
-           B_CFULL, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
+// *FULL and the others that both CTAs' threads arrive on count in the first
+// CTA, whose MMA thread waits; X* are the second CTA's copies having landed.
+enum Bar { B_KFULL = 0, B_VFULL, B_QFULL, B_XK, B_XV, B_XQ, B_KEMPTY, B_VEMPTY, B_QEMPTY, B_MASK, B_SFULL = B_MASK + 3, B_PREADY = B_SFULL + 2,
+           B_OFULL, B_OEMPTY, B_SSYNC, B_CFULL, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
 
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
@@ -83,7 +95,7 @@ struct Misc {
   int start_b;
   int64_t start_prefix, total;
   int64_t wsum[kThreads / 32];
-  uint32_t vmask[4];
+  uint32_t vmask[3][4];  // tile n in n % 3
   float red[3][128];  // row maxima of even and odd tiles, row sums of a unit
   Tile ring[kRing];
   Unit units[kUnitSlots];
@@ -98,7 +110,8 @@ struct TreeParams {
   const uint8_t* q;
   uint8_t* out;
   float* lse;
-  int T, H, G, R, scenario, K, ratio, win, B, S, layout, split;
+  int T, H, G, R, scenario,  // G: head groups of 128, R: pairs of CTAs per group
+       K, ratio, win, B, S, layout, split;
   const int32_t* cu;
   const int32_t* seqused;
   const int32_t* parents;
@@ -135,7 +148,7 @@ __device__ Req request(const TreeParams& p, int b) {
   r.ctx = __ldg(p.seqused + b) - r.n;
   r.bad = r.n > kMaxTree || r.ctx < 0 || r.ctx > kMaxCtx;
   r.thr = p.scenario == 1 || r.bad ? 0 : r.ctx / p.ratio;
-  r.units = p.scenario == 3 ? r.slots : (int)(((int64_t)r.slots * p.H + MR - 1) / MR);
+  r.units = p.scenario == 3 ? r.slots : (int)(((int64_t)r.slots * p.H + UR - 1) / UR);
   r.wtiles = r.bad || r.n == 0 ? 1 : (min(r.ctx, p.win) + r.n + CH - 1) / CH;
   r.tiles = r.wtiles + (r.bad || r.n == 0 ? 0 : p.scenario == 2 ? (r.thr + CH - 1) / CH : p.scenario == 3 && r.thr > 0 ? (p.K + CH - 1) / CH : 0);
   return r;
@@ -150,12 +163,57 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t byt
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sas::smem_u32(bar)) : "memory");
 }
-// D[tmem] (+)= A B^T, M = 64, weight-stationary
-__device__ __forceinline__ void umma_ws(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D[tmem of both CTAs] (+)= A B^T over the pair
+__device__ __forceinline__ void umma2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.ws.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
+}
+// Arrive on `bar` of both CTAs once every MMA issued before is complete.
+__device__ __forceinline__ void commit2(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          sas::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Arrive on `bar` of the pair's first CTA, with cluster scope.
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(sas::smem_u32(bar))
+      : "memory");
+}
+// sas::mbar_wait for a barrier that the other CTA's threads arrive on
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(sas::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = sas::globaltimer(), lim = ctl->limit_ns;
+  for (uint32_t n = 1;; ++n) {
+    if (try_wait_cluster(bar, parity)) return true;
+    if ((n & 63u) == 0) {
+      if (ctl->abort) return false;
+      if (sas::globaltimer() - t0 > lim) {
+        ctl->abort = 1;
+        if (status) atomicCAS(status, 0, SAS_ERR_TIMEOUT_BASE + where);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -189,31 +247,28 @@ __device__ __forceinline__ uint32_t window_bits(int p0, int s, int win, int ctx,
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Misc& ms = *reinterpret_cast<Misc*>(smem + OFF_MISC);
   uint64_t* bars = ms.bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = blockIdx.x % p.G, rank = blockIdx.x / p.G;
+  const int side = blockIdx.x & 1;  // the CTA's place in its pair
+  const int g = (blockIdx.x >> 1) % p.G, rank = (blockIdx.x >> 1) / p.G;
   if (tid == 0) {
-    for (int h = 0; h < 2; ++h) {
-      sas::mbar_init(&bars[B_FULL + h], 32 * kLoadWarps);
-      sas::mbar_init(&bars[B_EMPTY + h], 1);
-    }
+    sas::mbar_init(&bars[B_KFULL], 32 * kLoadWarps);
+    sas::mbar_init(&bars[B_VFULL], 32 * kLoadWarps);
     sas::mbar_init(&bars[B_QFULL], 32 * kLoadWarps);
-    sas::mbar_init(&bars[B_QEMPTY], 1);
-    sas::mbar_init(&bars[B_VFULL], kLoadWarps);
-    sas::mbar_init(&bars[B_SFULL], 1);
-    sas::mbar_init(&bars[B_PREADY], 128);
-    sas::mbar_init(&bars[B_OFULL], 1);
-    sas::mbar_init(&bars[B_OEMPTY], 128);
+    for (int i : {(int)B_XK, (int)B_XV, (int)B_XQ, (int)B_KEMPTY, (int)B_VEMPTY, (int)B_QEMPTY, (int)B_SFULL, B_SFULL + 1, (int)B_OFULL, (int)B_DRAIN})
+      sas::mbar_init(&bars[i], 1);
+    for (int i = 0; i < 3; ++i) sas::mbar_init(&bars[B_MASK + i], kLoadWarps);
+    sas::mbar_init(&bars[B_PREADY], 8);  // softmax warps of both CTAs
+    sas::mbar_init(&bars[B_OEMPTY], 8);
     sas::mbar_init(&bars[B_SSYNC], 128);
     for (int i = 0; i < kRing; ++i) {
       sas::mbar_init(&bars[B_CFULL + i], 1);
       sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + 4);
     }
-    sas::mbar_init(&bars[B_DRAIN], 1);
     sas::fence_mbar_init();
     ms.ctl.abort = 0;
     ms.ctl.limit_ns = SAS_WAIT_LIMIT_NS;
@@ -221,8 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
     ms.start_prefix = 0;
   }
   if (warp == kMmaWarp) {
-    sas::tmem_alloc(&ms.tmem, TM_COLS);
-    sas::tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sas::smem_u32(&ms.tmem)), "r"(TM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   // every thread takes a run of requests; a block scan of their tiles gives the
   // sequence's length and the request that this CTA's range starts in
@@ -271,12 +326,16 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
   }
   if (blockIdx.x == 0 && tid == 0) *p.total = total;
   sas::pdl_launch_dependents();
+  sas::tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the other CTA's barriers and tensor memory are there
+  sas::tc_fence_after();
   const uint32_t tmem = ms.tmem;
   volatile sas::CtaCtl* ctl = &ms.ctl;
-  const uint32_t q_base = sas::smem_u32(smem + OFF_Q), kv_base = sas::smem_u32(smem + OFF_KV),
-                 p_base = sas::smem_u32(smem + OFF_P);
+  const uint32_t q_base = sas::smem_u32(smem + OFF_Q), k_base = sas::smem_u32(smem + OFF_K),
+                 v_base = sas::smem_u32(smem + OFF_V), p_base = sas::smem_u32(smem + OFF_P);
 #define WAIT(bar, par, id) sas::mbar_wait(&bars[bar], (par)&1, ctl, p.status, id)
+#define WAIT_PAIR(bar, par, id) wait_cluster(&bars[bar], (par)&1, ctl, p.status, id)
 
   if (warp == kCoordWarp) {
     // ================================================= coordinator
@@ -322,22 +381,30 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
       }
       const int us = uc % kUnitSlots;
       Unit& un = ms.units[us];
-      const int64_t row_in = p.scenario == 3 ? (int64_t)u * p.H + g * MR : (int64_t)u * MR;
-      const int nrows = p.scenario == 3 ? min(MR, p.H - g * MR) : (int)min((int64_t)MR, (int64_t)r.slots * p.H - row_in);
-      const int i0 = (int)(row_in / p.H), i1 = (int)((row_in + nrows - 1) / p.H);
+      // the unit's rows among the request's, and this CTA's half of them
+      const int64_t first = p.scenario == 3 ? (int64_t)u * p.H + g * UR : (int64_t)u * UR;
+      const int64_t end = p.scenario == 3 ? min(first + UR, (int64_t)(u + 1) * p.H) : min(first + UR, (int64_t)r.slots * p.H);
+      const int64_t row_in = first + side * MR;
+      const int nrows = (int)max((int64_t)0, min((int64_t)MR, end - row_in));
+      const int i0 = (int)(first / p.H), i1 = (int)((end - 1) / p.H);
+      const int mine = nrows ? (int)(row_in / p.H) - i0 : 0;  // this CTA's first token among the unit's
       // the slot's last readers are done: see kUnitSlots; the ring wait below
       // orders this warp's writes after their reads
       if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + c % kRing, (c / kRing) ^ 1u, 20))) break;
       int pos = -1;
-      if (lane < kMaxTok) {
-        uint32_t* bits = un.bits[lane];
-        for (int w = 0; w < (min(r.n, kMaxTree) + 31) / 32 || w < 1; ++w) bits[w] = 0;
+      if (lane < kMaxUnitTok) {
+        const int slot = lane - mine;
+        uint32_t* bits = slot >= 0 && slot < kMaxTok ? un.bits[slot] : nullptr;
+        const int words = max((min(r.n, kMaxTree) + 31) / 32, 1);
+        // window_bits reads up to five words past the last one with a bit
+        if (bits)
+          for (int w = 0; w < min(words + 5, kWords); ++w) bits[w] = 0;
         const int i = i0 + lane;
         if (i <= i1 && i < r.n && !r.bad && ms.parents[i] >= -1) {
           int j = i, d = 0;
           bool good = true;
           while (true) {
-            if (d <= p.win) bits[j >> 5] |= 1u << (j & 31);
+            if (bits && d <= p.win) bits[j >> 5] |= 1u << (j & 31);
             const int q = ms.parents[j];
             if (q == -1) break;
             if (q < -1 || q >= j) {  // after an unused slot, or not before its child
@@ -350,10 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
           if (good) pos = r.ctx + d;
           else bad(p, SAS_ERR_BAD_TREE);
         }
-        // window_bits reads one word past the last one with a bit
-        const int w = (min(r.n, kMaxTree) + 31) / 32;
-        for (int x = max(w, 1); x < min(w + 5, kWords); ++x) bits[x] = 0;
-        un.pos[lane] = pos;
+        if (bits) un.pos[slot] = pos;
       }
       if (lane == 0) {
         un.b = b;
@@ -368,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
       const bool whole = k0 == 0 && k1 == r.tiles;
       if (k0 > 0 && any) {
         lead_cut = true;
-        if (lane == 0) p.cuts[blockIdx.x] = Cut{ustart, uend, un.qrow, nrows, 1};
+        if (lane == 0) p.cuts[blockIdx.x] = Cut{ustart, uend, (int64_t)r.base * p.H + row_in, nrows, 1};
       }
       if (!any) {
         if (k0 == 0) {
@@ -399,17 +463,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
     if (ok) publish(TF_END, 0, 0, 0);
   } else if (warp >= kLoadWarp0) {
     // ================================================= loaders
+    // K of a tile, then V of the tile before: the order in which the buffers
+    // come free (K after the scores, V after the product).
     const int lw = warp - kLoadWarp0;
     uint32_t c = 0, n = 0, q = 0;
-    int row = -1;
+    // Lanes 0-7: tile rows [64 side + 8 lw, + 8), which are also this warp's K
+    // rows; lanes 8-15: the same of the other CTA's half.
+    const int my_row = (lane < 8 ? side : side ^ 1) * 64 + lw * 8 + (lane & 7);
     Tile t{};
-    // pool row of tile row 16 * lw + lane (-1: none)
-    auto resolve = [&]() -> int {
-      const int r = lw * 16 + lane;
-      if (lane >= 16 || r >= t.nrows || (t.flags & (TF_END | TF_ZERO))) return -1;
+    auto resolve = [&]() -> int {  // pool row of tile row my_row (-1: none)
+      if (lane >= 16 || my_row >= t.nrows) return -1;
       const Unit& u = ms.units[t.uslot];
       const int f = (t.flags & TF_CMP) ? 1 : 0;
-      int pos = t.row0 + r;
+      int pos = t.row0 + my_row;
       if (t.flags & TF_TOPK) {
         pos = __ldg(p.idx + (int64_t)u.tok * p.K + pos);
         if (pos < 0 || pos >= u.thr) return -1;
@@ -427,17 +493,41 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
       }
       return blk * p.bs[f] + (pos - col * p.bs[f]);
     };
-    while (true) {
+    // rows of a tile that are copied (others stay as they are): whole K steps of the product
+    auto top = [](const Tile& x) { return max(16, (x.nrows + 15) & ~15); };
+    int v_row = -1, v_top = 0;
+    bool v_due = false;  // V of tile n - 1 is not copied yet
+    const uint8_t* v_pool = nullptr;
+    // V of tile m: 512 bytes (this CTA's 256 columns) of rows my_row of lanes 0-15
+    auto load_v = [&](uint32_t m) -> bool {
+      if (!__all_sync(0xffffffffu, WAIT(B_VEMPTY, m ^ 1u, 23))) return false;
+      const uint8_t* src = v_pool + side * 512 + lane * 16;
+      const uint32_t dst = v_base + (lane >> 3) * VSLAB;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int ri = __shfl_sync(0xffffffffu, v_row, i);
+        const int r = (i < 8 ? side : side ^ 1) * 64 + lw * 8 + (i & 7);
+        if (r < v_top)
+          cp16(dst + r * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
+      }
+      cp_arrive(&bars[B_VFULL]);
+      return true;
+    };
+    bool ok = true;
+    while (ok) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
       t = ms.ring[c % kRing];
-      if (t.flags & TF_END) break;
-      if (!(t.flags & TF_ZERO)) {
-        row = resolve();
+      if (t.flags & (TF_END | TF_ZERO)) {  // no K to go first (and a unit may end here: see the MMA issuer)
+        if (v_due) ok = load_v(n - 1);
+        v_due = false;
+        if (t.flags & TF_END) break;
+      } else {
+        const int row = resolve();
         if (t.flags & TF_FIRST) {
           if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
           const Unit& u = ms.units[t.uslot];
-          const uint8_t* src = p.q + u.qrow * (D * 2) + lane * 16;
           const int nr = u.nrows;
+          const uint8_t* src = p.q + (nr ? u.qrow : 0) * (D * 2) + lane * 16;
 #pragma unroll
           for (int i = 0; i < MR / kLoadWarps; ++i) {
             const int r = lw * (MR / kLoadWarps) + i;
@@ -449,32 +539,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
           cp_arrive(&bars[B_QFULL]);
           ++q;
         }
-        const int f = (t.flags & TF_CMP) ? 1 : 0;
-        const int top = max(16, (t.nrows + 15) & ~15);
-        const int cnt = min(16, max(0, top - lw * 16));
-        bool ok = true;
-        for (int h = 0; h < 2; ++h) {
-          if (!__all_sync(0xffffffffu, WAIT(B_EMPTY + h, n ^ 1u, 23))) {
-            ok = false;
-            break;
-          }
-          if (h == 0) {  // the rows' mask; its last reader signed off before the tile's slot came free
-            const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
-            if (lane == 0) {
-              reinterpret_cast<uint16_t*>(ms.vmask)[lw] = (uint16_t)vm;
-              sas::mbar_arrive(&bars[B_VFULL]);
-            }
-          }
-          const uint8_t* src = p.kv[f] + h * 512 + lane * 16;
-          const uint32_t dst = kv_base + (h * 4 + (lane >> 3)) * SLAB + lw * 16 * 128;
-#pragma unroll 8
-          for (int i = 0; i < cnt; ++i) {
-            const int ri = __shfl_sync(0xffffffffu, row, i);
-            cp16(dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
-          }
-          cp_arrive(&bars[B_FULL + h]);
+        if (!__all_sync(0xffffffffu, WAIT(B_KEMPTY, n ^ 1u, 34))) break;
+        // The rows' mask. Its place was tile n - 3's, which is done with: the
+        // scores of n - 1, after which K came free, were issued after its product.
+        const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane == 0) {
+          uint8_t* bytes = reinterpret_cast<uint8_t*>(ms.vmask[n % 3]);
+          bytes[side * 8 + lw] = (uint8_t)vm;
+          bytes[(side ^ 1) * 8 + lw] = (uint8_t)(vm >> 8);
+          sas::mbar_arrive(&bars[B_MASK + n % 3]);
         }
-        if (!ok) break;
+        const uint8_t* pool = p.kv[(t.flags & TF_CMP) ? 1 : 0];
+        const uint8_t* src = pool + lane * 16;
+        const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 8 * 128;
+        const int cnt = min(8, max(0, top(t) - side * 64 - lw * 8));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int ri = __shfl_sync(0xffffffffu, row, i);
+          if (i < cnt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              cp16(dst + h * 4 * KSLAB + i * 128 + (((lane & 7) ^ (i & 7)) << 4),
+                   src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
+        }
+        cp_arrive(&bars[B_KFULL]);
+        if (v_due) ok = load_v(n - 1);
+        v_row = row, v_top = top(t), v_pool = pool, v_due = true;
         ++n;
       }
       __syncwarp();
@@ -484,59 +574,84 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMmaWarp) {
     // ================================================= MMA issuer
+    // First CTA: scores of tile n, then the product of tile n - 1. Second CTA:
+    // tells the first, in the loaders' order, that its copies have landed.
     if (lane == 0) {
       constexpr int fmt = DT == SAS_DTYPE_BF16 ? 1 : 0;
-      constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, MR, CH, 0, 0);
-      constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, MR, 256, 0, 1);
-      uint32_t c = 0, n = 0, u = 0;
+      constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, UR, CH, 0, 0);
+      constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
+      uint32_t c = 0, n = 0, u = 0, vu = 0;
+      Tile last{};  // tile n - 1
+      bool due = false;  // its product is not issued yet
+      auto pass_on = [&](int bar, int to, uint32_t par) -> bool {
+        if (!WAIT(bar, par, 26)) return false;
+        sas::fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+        arrive_first(&bars[to]);
+        return true;
+      };
+      auto product = [&](uint32_t m) -> bool {
+        if (side) return pass_on(B_VFULL, B_XV, m);
+        if (!WAIT_PAIR(B_PREADY, m, 27) || !WAIT(B_VFULL, m, 35) || !WAIT_PAIR(B_XV, m, 36)) return false;
+        if ((last.flags & TF_FIRST) && !WAIT_PAIR(B_OEMPTY, vu ^ 1u, 28)) return false;
+        sas::fence_proxy_async_smem();
+        sas::tc_fence_after();
+        const int steps = max(1, (last.nrows + 15) / 16);
+        for (int h = 0; h < 2; ++h)
+          for (int ks = 0; ks < steps; ++ks)
+            umma2(tmem + TM_O + 128 * h, sas::umma_desc_sw128(p_base + (ks >> 2) * QSLAB + (ks & 3) * 32, 16, 1024),
+                  sas::umma_desc_sw128(v_base + 2 * h * VSLAB + ks * 2048, VSLAB, 1024), id_o,
+                  !((last.flags & TF_FIRST) && ks == 0));
+        commit2(&bars[B_VEMPTY]);
+        if (last.flags & TF_LAST) {
+          commit2(&bars[B_OFULL]);
+          ++vu;
+        }
+        return true;
+      };
       while (true) {
         if (!WAIT(B_CFULL + c % kRing, c / kRing, 24)) break;
         const Tile t = ms.ring[c % kRing];
-        if (t.flags & TF_END) break;
-        if (!(t.flags & TF_ZERO)) {
-          if ((t.flags & TF_FIRST) && !WAIT(B_QFULL, u, 25)) break;
-          bool ok = true;
-          for (int h = 0; h < 2; ++h) {
-            if (!WAIT(B_FULL + h, n, 26)) {
-              ok = false;
-              break;
+        if (t.flags & (TF_END | TF_ZERO)) {
+          // The product may not wait for a next tile with rows: the softmax
+          // warps wait for it before they release the ring's next entries.
+          if (due && !product(n - 1)) break;
+          due = false;
+          if (t.flags & TF_END) break;
+        } else {
+          if (side) {
+            if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
+            if (!pass_on(B_KFULL, B_XK, n)) break;
+          } else {
+            if (t.flags & TF_FIRST) {
+              if (!WAIT(B_QFULL, u, 25) || !WAIT_PAIR(B_XQ, u, 37)) break;
+              ++u;
             }
-            sas::fence_proxy_async_smem();  // cp.async writes -> tensor core reads
+            if (!WAIT(B_KFULL, n, 26) || !WAIT_PAIR(B_XK, n, 38)) break;
+            sas::fence_proxy_async_smem();
             sas::tc_fence_after();
 #pragma unroll
-            for (int s = 4 * h; s < 4 * h + 4; ++s)
+            for (int s = 0; s < 8; ++s)
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                umma_ws(tmem + TM_S, sas::umma_desc_sw128(q_base + s * QSLAB + kk * 32, 16, 1024),
-                        sas::umma_desc_sw128(kv_base + s * SLAB + kk * 32, 16, 1024), id_s, (s | kk) != 0);
+                umma2(tmem + TM_S + 64 * (n & 1), sas::umma_desc_sw128(q_base + s * QSLAB + kk * 32, 16, 1024),
+                      sas::umma_desc_sw128(k_base + s * KSLAB + kk * 32, 16, 1024), id_s, (s | kk) != 0);
+            commit2(&bars[B_SFULL + (n & 1)]);
+            commit2(&bars[B_KEMPTY]);
+            if (t.flags & TF_LAST) commit2(&bars[B_QEMPTY]);
           }
-          if (!ok) break;
-          sas::umma_commit(&bars[B_SFULL]);
-          if (t.flags & TF_LAST) sas::umma_commit(&bars[B_QEMPTY]);
-          if (!WAIT(B_PREADY, n, 27)) break;
-          if ((t.flags & TF_FIRST) && !WAIT(B_OEMPTY, u ^ 1u, 28)) break;
-          sas::tc_fence_after();
-          const int steps = max(1, (t.nrows + 15) / 16);
-          for (int h = 0; h < 2; ++h) {
-            for (int ks = 0; ks < steps; ++ks)
-              umma_ws(tmem + TM_O + 128 * h,
-                      sas::umma_desc_sw128(p_base + (ks >> 2) * QSLAB + (ks & 3) * 32, 16, 1024),
-                      sas::umma_desc_sw128(kv_base + 4 * h * SLAB + ks * 2048, SLAB, 1024), id_o,
-                      !((t.flags & TF_FIRST) && ks == 0));
-            sas::umma_commit(&bars[B_EMPTY + h]);
-          }
-          if (t.flags & TF_LAST) {
-            sas::umma_commit(&bars[B_OFULL]);
-            ++u;
-          }
+          if (due && !product(n - 1)) break;
+          last = t;
+          due = true;
           ++n;
         }
         sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
         ++c;
       }
-      // nothing may still run on TMEM or shared memory when the CTA leaves
-      sas::umma_commit(&bars[B_DRAIN]);
-      sas::mbar_wait_drain(&bars[B_DRAIN], 0, SAS_WAIT_LIMIT_NS);
+      // nothing may still run on TMEM or shared memory when the pair leaves
+      if (!side) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sas::smem_u32(&bars[B_DRAIN])) : "memory");
+        sas::mbar_wait_drain(&bars[B_DRAIN], 0, SAS_WAIT_LIMIT_NS);
+      }
     }
     __syncwarp();
   } else {
@@ -563,23 +678,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
           tok = p.scenario == 3 ? 0 : min((un.roff + row) / p.H, kMaxTok - 1);
           pos = row < un.nrows ? un.pos[tok] : -1;
         }
-        ok = __all_sync(0xffffffffu, WAIT(B_VFULL, n, 30) && WAIT(B_SFULL, n, 31));
+        ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30) && WAIT(B_SFULL + (n & 1), n >> 1, 31));
         if (!ok) break;
         sas::tc_fence_after();
+        const uint32_t ts = tl + TM_S + 64 * (n & 1);
         float s[64];
         {
           uint32_t r[32];
-          sas::tmem_ld32(tl + TM_S, r);
+          sas::tmem_ld32(ts, r);
           sas::tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(r[i]);
-          sas::tmem_ld32(tl + TM_S + 32, r);
+          sas::tmem_ld32(ts + 32, r);
           sas::tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(r[i]);
         }
         // rows that are there, and those of them that this row's token sees
-        const uint32_t v0 = ms.vmask[2 * ch], v1 = ms.vmask[2 * ch + 1];
+        const uint32_t v0 = ms.vmask[n % 3][2 * ch], v1 = ms.vmask[n % 3][2 * ch + 1];
         uint32_t k0 = v0, k1 = v1;
         if (pos < 0) {
           k0 = k1 = 0;
@@ -588,11 +704,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
           k0 &= window_bits(p0, pos, p.win, un.ctx, un.bits[tok]);
           k1 &= window_bits(p0 + 32, pos, p.win, un.ctx, un.bits[tok]);
         }
-        if (!__all_sync(0xffffffffu, (k0 & k1) == 0xffffffffu)) {
-          // A row of KV with infinities or NaN that this token does not see
-          // would reach its sum as 0 * NaN. Its scores are not finite, which
-          // one sum shows; such rows are then cleared before the product. A
-          // token that does see one has a NaN in l, so its result is NaN.
+        const bool window = !(t.flags & TF_CMP);
+        if (window || !__all_sync(0xffffffffu, (k0 & k1) == 0xffffffffu)) {
+          // In the window a row may be seen by some tokens only, and one with
+          // infinities or NaN would reach the others' sums as 0 * NaN. All rows'
+          // scores with it are not finite, in both CTAs, which one sum shows;
+          // each CTA then clears what it holds of such a row's V. A token that
+          // sees it has a NaN in l, so its result is NaN.
           float z = 0.f;
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
@@ -601,26 +719,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
             z = fmaf(((v >> (i & 31)) & 1u) ? s[i] : 0.f, 0.f, z);
             s[i] = see ? s[i] * p.scale_log2 : -INFINITY;
           }
-          if (z != 0.f) {
-            for (int i = 0; i < 64; ++i) {
-              const uint32_t v = i < 32 ? v0 : v1;
-              if (!((v >> (i & 31)) & 1u)) continue;
-              const int kr = 64 * ch + i;
-              uint32_t hot = 0;
-              for (int e = 0; e < 64; ++e) {  // 16-byte pieces of the row
-                uint32_t w[4];
-                const uint32_t a = kv_base + (e >> 3) * SLAB + kr * 128 + (e & 7) * 16;
-                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-                constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+          if (window && z != 0.f) {
+            // The tile's V has to be there, after the one before it was done with
+            // (its copy alone could be two phases back). A wait that fails shows
+            // at the next one.
+            if (WAIT(B_VEMPTY, n ^ 1u, 40) && WAIT(B_VFULL, n, 39))
+              for (int i = 0; i < 64; ++i) {
+                const uint32_t v = i < 32 ? v0 : v1;
+                if (!((v >> (i & 31)) & 1u)) continue;
+                const int vr = 64 * ch + i;
+                uint32_t hot = 0;
+                for (int e = 0; e < 32; ++e) {  // 16-byte pieces of the half row
+                  uint32_t w[4];
+                  const uint32_t a = v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16;
+                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+                  constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
+                  for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
+                }
+                if (hot)
+                  for (int e = 0; e < 32; ++e) st_shared16(v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16, 0, 0, 0, 0);
               }
-              if (hot) {
-                const uint32_t k = i < 32 ? k0 : k1;
-                if ((k >> (i & 31)) & 1u) l = NAN;
-                for (int e = 0; e < 64; ++e) st_shared16(kv_base + (e >> 3) * SLAB + kr * 128 + (e & 7) * 16, 0, 0, 0, 0);
-              }
-            }
+            // a score of -inf weighs nothing, but its row is not finite
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (((i < 32 ? k0 : k1) >> (i & 31)) & 1u) l = s[i] == -INFINITY ? NAN : l;
           }
         } else {
 #pragma unroll
@@ -642,7 +765,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
           m = mx;
           l *= fac;
         }
-        // the product before this tile's is complete: its commit came before this tile's scores
+        // the product before this tile's is complete, and P may be written
+        ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40));
+        if (!ok) break;
+        sas::tc_fence_after();
         if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
 #pragma unroll 1
           for (int x = 0; x < 256; x += 32) {
@@ -672,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
         l += (la[0] + la[1]) + (la[2] + la[3]);
         sas::fence_proxy_async_smem();
         sas::tc_fence_before();
-        sas::mbar_arrive(&bars[B_PREADY]);
+        __syncwarp();
+        if (lane == 0) arrive_first(&bars[B_PREADY]);
         ++n;
         if (t.flags & TF_LAST) {
           float* rl = ms.red[2];
@@ -699,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
               __syncwarp();
               sas::tmem_ld32(tl + TM_O + 32 * x, r);
               sas::tmem_wait_ld();
-              float4* d4 = reinterpret_cast<float4*>(o + row * D + (x >> 2) * 256 + ch * 128 + (x & 3) * 32);
+              float4* d4 = reinterpret_cast<float4*>(o + row * D + ch * 256 + x * 32);
 #pragma unroll
               for (int i = 0; i < 8; ++i)
                 d4[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
@@ -719,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
               __syncwarp();
               sas::tmem_ld32(tl + TM_O + 32 * x, r);
               sas::tmem_wait_ld();
-              uint4* d4 = reinterpret_cast<uint4*>(orow + ((x >> 2) * 256 + ch * 128 + (x & 3) * 32) * 2);
+              uint4* d4 = reinterpret_cast<uint4*>(orow + (ch * 256 + x * 32) * 2);
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i)
@@ -730,7 +857,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
             }
           }
           sas::tc_fence_before();
-          sas::mbar_arrive(&bars[B_OEMPTY]);
+          __syncwarp();
+          if (lane == 0) arrive_first(&bars[B_OEMPTY]);
         }
       }
       __syncwarp();
@@ -740,8 +868,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
   }
   sas::tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) sas::tmem_dealloc(tmem, TM_COLS);
+  cluster_sync();  // the other CTA no longer reads this one's shared memory or arrives on it
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
 #undef WAIT
+#undef WAIT_PAIR
 }
 
 // Joins the pieces of a cut unit, in order. The block of CTA c does so when c's
@@ -749,7 +879,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_con
 template <int DT>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeParams p) {
   sas::pdl_wait();
-  const int g = blockIdx.x % p.G, rank = blockIdx.x / p.G;
+  const int ctas = 2 * p.G;  // of a range
+  const int g = blockIdx.x % ctas, rank = blockIdx.x / ctas;
   const int64_t total = *p.total;
   const int R = ranges(total, p.R);
   if (rank == 0 || rank >= R) return;
@@ -761,7 +892,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   while (last + 1 < R && range_start(total, R, last + 1) < c.uend) ++last;
   // the first piece is partial 0 of its CTA if the unit starts with the range
   const int first_slot = before == c.ustart ? 0 : 1;
-  auto piece = [&](int r) { return p.part + ((size_t)(r * p.G + g) * 2 + (r == rank - 1 ? first_slot : 0)) * kPieceFloats; };
+  auto piece = [&](int r) { return p.part + ((size_t)(r * ctas + g) * 2 + (r == rank - 1 ? first_slot : 0)) * kPieceFloats; };
   for (int i = threadIdx.x >> 7; i < 8; i += 2) {
     const int row = blockIdx.y * 8 + i, col = threadIdx.x & 127;
     if (row >= c.nrows) break;
@@ -795,11 +926,11 @@ template <int DT>
 int launch(const TreeParams& p, cudaStream_t st) {
   auto kern = tree_attn_kernel<DT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return SAS_ERR_CUDA;
-  kern<<<p.R * p.G, kThreads, SMEM_BYTES, st>>>(p);
+  kern<<<2 * p.R * p.G, kThreads, SMEM_BYTES, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SAS_ERR_CUDA;
   if (!p.split) return SAS_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.R * p.G, MR / 8);
+  cfg.gridDim = dim3(2 * p.R * p.G, MR / 8);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -845,9 +976,9 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.out = static_cast<uint8_t*>(out);
   p.lse = lse;
   p.T = T, p.H = H, p.scenario = scenario, p.K = K, p.ratio = ratio, p.win = win < kMaxCtx ? win : kMaxCtx, p.B = B, p.S = S, p.layout = layout;
-  p.G = scenario == 3 ? (H + MR - 1) / MR : 1;
-  if (p.G > num_sms) return SAS_ERR_UNSUPPORTED;
-  p.R = num_sms / p.G;
+  p.G = scenario == 3 ? (H + UR - 1) / UR : 1;
+  if (2 * p.G > num_sms) return SAS_ERR_UNSUPPORTED;
+  p.R = num_sms / (2 * p.G);
   p.split = 1;
   p.cu = cu, p.seqused = seqused, p.parents = parents;
   p.kv[0] = static_cast<const uint8_t*>(ori_kv), p.kv[1] = static_cast<const uint8_t*>(cmp_kv);

@@ -199,6 +199,9 @@ CASES = {
     "empty requests": dict(lens=[0, 2, 0, 0, 3, 0], ctx=[5, 70, 0, 9, 200, 1], H=16, scenario=2),
     "rows of no request": dict(lens=[2, 2], ctx=[70, 10], H=16, pad=5, lead=3),
     "padded": dict(lens=[4, 4, 4], ctx=[30, 300, 128], H=64, layout="BSND", trees=[[-1, 0], [-2, -1, -2, 1], [-2] * 4]),
+    "long runs of unused slots": dict(lens=[24] * 6, ctx=[30, 300, 128, 2, 400, 260], H=64, layout="BSND", scenario=2,
+                                      trees=[[-1] + [-2] * 23, [-2] * 20 + [-1, -1, 20, -2], [-2] * 24, [-1, 0] + [-2] * 22,
+                                             [-2] * 23 + [-1], [-1] * 24]),
     "ragged bsnd": dict(lens=[2, 5, 0], ctx=[30, 300, 128], H=16, layout="BSND", scenario=2, ratio=16),
     "dense": dict(lens=[5, 1], ctx=[1000, 37], H=64, scenario=2),
     "dense odd": dict(lens=[3, 8, 2], ctx=[515, 4099, 3], H=24, scenario=2, ratio=4, bs=48, dt=FP, win=63),
