@@ -31,10 +31,10 @@
 // P, l and O keep one common scale. P is rounded to the I/O type for the
 // product, l sums it unrounded (as the framework's forward does).
 //
-// Roles (14 warps): 0-3 softmax and epilogue (thread = row, half of the tile's
-// columns), 4 MMA issuer (in the pair's second CTA it passes on that its copies
-// have landed), 5 coordinator (walks the range and the trees and publishes
-// tiles in a ring; the pair's two coordinators take the same steps), 6-13
+// Roles (18 warps): 0-7 softmax and epilogue (thread = row, 32 of the tile's
+// columns), 8 MMA issuer (in the pair's second CTA it passes on that its copies
+// have landed), 9 coordinator (walks the range and the trees and publishes
+// tiles in a ring; the pair's two coordinators take the same steps), 10-17
 // loaders (cp.async; 8 K rows and 16 V half rows of a tile each).
 #include "sas_common.cuh"
 
@@ -52,7 +52,7 @@ constexpr int kMaxCtx = 1 << 30;  // rows cached before them
 constexpr int KSLAB = 64 * 128;   // 64 columns of the CTA's 64 K rows
 constexpr int VSLAB = CH * 128;   // 64 columns of the tile's V rows
 constexpr int QSLAB = MR * 128;   // 64 columns of Q, or of P
-constexpr int kMmaWarp = 4, kCoordWarp = 5, kLoadWarp0 = 6, kLoadWarps = 8;
+constexpr int kSmWarps = 8, kMmaWarp = 8, kCoordWarp = 9, kLoadWarp0 = 10, kLoadWarps = 8;
 constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
 constexpr int kRing = 4;          // tiles the coordinator may be ahead
 constexpr int kUnitSlots = 6;     // > kRing + 1: no slot is rewritten while a published tile names it
@@ -96,7 +96,7 @@ struct Misc {
   int64_t start_prefix, total;
   int64_t wsum[kThreads / 32];
   uint32_t vmask[3][4];  // tile n in n % 3
-  float red[3][128];  // row maxima of even and odd tiles, row sums of a unit
+  float red[3][32 * kSmWarps];  // row maxima of even and odd tiles, row sums of a unit
   Tile ring[kRing];
   Unit units[kUnitSlots];
   int parents[kMaxTree];
@@ -227,6 +227,35 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return reinterpret_cast<const uint32_t&>(v);
 }
+// Two fp32 values in a register pair, and operations on both at once.
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ float lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pair(__float_as_uint(a), __float_as_uint(a)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ void bad(const TreeParams& p, int code) {
   if (p.status) atomicCAS(p.status, 0, code);
 }
@@ -262,12 +291,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     for (int i : {(int)B_XK, (int)B_XV, (int)B_XQ, (int)B_KEMPTY, (int)B_VEMPTY, (int)B_QEMPTY, (int)B_SFULL, B_SFULL + 1, (int)B_OFULL, (int)B_DRAIN})
       sas::mbar_init(&bars[i], 1);
     for (int i = 0; i < 3; ++i) sas::mbar_init(&bars[B_MASK + i], kLoadWarps);
-    sas::mbar_init(&bars[B_PREADY], 8);  // softmax warps of both CTAs
-    sas::mbar_init(&bars[B_OEMPTY], 8);
-    sas::mbar_init(&bars[B_SSYNC], 128);
+    sas::mbar_init(&bars[B_PREADY], 2 * kSmWarps);  // softmax warps of both CTAs
+    sas::mbar_init(&bars[B_OEMPTY], 2 * kSmWarps);
+    sas::mbar_init(&bars[B_SSYNC], 32 * kSmWarps);
     for (int i = 0; i < kRing; ++i) {
       sas::mbar_init(&bars[B_CFULL + i], 1);
-      sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + 4);
+      sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + kSmWarps);
     }
     sas::fence_mbar_init();
     ms.ctl.abort = 0;
@@ -493,7 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       }
       return blk * p.bs[f] + (pos - col * p.bs[f]);
     };
-    // rows of a tile that are copied (others stay as they are): whole K steps of the product
+    // V rows of a tile that are copied (others stay as they are): whole K steps of the product
     auto top = [](const Tile& x) { return max(16, (x.nrows + 15) & ~15); };
     int v_row = -1, v_top = 0;
     bool v_due = false;  // V of tile n - 1 is not copied yet
@@ -552,15 +581,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         const uint8_t* pool = p.kv[(t.flags & TF_CMP) ? 1 : 0];
         const uint8_t* src = pool + lane * 16;
         const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 8 * 128;
-        const int cnt = min(8, max(0, top(t) - side * 64 - lw * 8));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i) {  // all 64 rows: absent ones are zero, so that their scores are finite
           const int ri = __shfl_sync(0xffffffffu, row, i);
-          if (i < cnt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              cp16(dst + h * 4 * KSLAB + i * 128 + (((lane & 7) ^ (i & 7)) << 4),
-                   src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
+          for (int h = 0; h < 2; ++h)
+            cp16(dst + h * 4 * KSLAB + i * 128 + (((lane & 7) ^ (i & 7)) << 4),
+                 src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
         }
         cp_arrive(&bars[B_KFULL]);
         if (v_due) ok = load_v(n - 1);
@@ -656,8 +683,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     __syncwarp();
   } else {
     // ================================================= softmax, epilogue
-    const int row = tid & 63, ch = tid >> 6;  // columns [64 ch, 64 ch + 64) of a tile
-    const uint32_t tl = tmem + ((uint32_t)warp << 21);
+    // Warps w and w + 4 share TMEM lanes: thread = row, columns [32 part, + 32)
+    // of a tile's 128, and 128 of the row's output columns.
+    const int row = (warp & 1) * 32 + lane, ch = (warp >> 1) & 1, gr = warp >> 2, part = 2 * ch + gr;
+    const uint32_t tl = tmem + ((uint32_t)(warp & 3) << 21);
+    float* const red_row = &ms.red[0][row];
+    constexpr int RED = 32 * kSmWarps;
+    const bool flip = p.scale_log2 < 0.f;
+    const float scale = flip ? -p.scale_log2 : p.scale_log2;
     uint32_t c = 0, n = 0, u = 0, sy = 0;
     float m = -INFINITY, l = 0.f;
     int pos = -1, tok = 0;
@@ -669,7 +702,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const Unit& un = ms.units[t.uslot];
       if (t.flags & TF_ZERO) {
         uint4* o = reinterpret_cast<uint4*>(p.out + un.qrow * (D * 2));
-        for (int i = tid; i < un.nrows * (D / 8); i += 128) o[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < un.nrows * (D / 8); i += 32 * kSmWarps) o[i] = make_uint4(0, 0, 0, 0);
         if (p.lse && tid < un.nrows) p.lse[un.qrow + tid] = 0.f;
       } else {
         if (t.flags & TF_FIRST) {
@@ -678,100 +711,107 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           tok = p.scenario == 3 ? 0 : min((un.roff + row) / p.H, kMaxTok - 1);
           pos = row < un.nrows ? un.pos[tok] : -1;
         }
-        ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30) && WAIT(B_SFULL + (n & 1), n >> 1, 31));
+        // rows of the tile that are there, and those that this row's token sees
+        ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30));
+        if (!ok) break;
+        const bool window = !(t.flags & TF_CMP);
+        const uint32_t there32 = ms.vmask[n % 3][part];
+        uint32_t see = there32;
+        if (pos < 0) see = 0;
+        else if (window) see &= window_bits(t.row0 + 32 * part, pos, p.win, un.ctx, un.bits[tok]);
+        ok = __all_sync(0xffffffffu, WAIT(B_SFULL + (n & 1), n >> 1, 31));
         if (!ok) break;
         sas::tc_fence_after();
-        const uint32_t ts = tl + TM_S + 64 * (n & 1);
-        float s[64];
+        uint64_t s[16];
         {
           uint32_t r[32];
-          sas::tmem_ld32(ts, r);
+          sas::tmem_ld32(tl + TM_S + 64 * (n & 1) + 32 * gr, r);
           sas::tmem_wait_ld();
+          if (flip)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(r[i]);
-          sas::tmem_ld32(ts + 32, r);
-          sas::tmem_wait_ld();
+            for (int i = 0; i < 32; ++i) r[i] ^= 0x80000000u;
+          if (window || !__all_sync(0xffffffffu, see == 0xffffffffu)) {
+            if (window) {
+              // In the window a row may be seen by some tokens only, and one with
+              // infinities or NaN would reach the others' sums as 0 * NaN. All
+              // rows' scores with it are not finite, in both CTAs, which their
+              // sum shows; each CTA then clears what it holds of such a row's V.
+              // A token that sees it has a NaN in l, so its result is NaN.
+              uint64_t z[2] = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(r[i]);
-        }
-        // rows that are there, and those of them that this row's token sees
-        const uint32_t v0 = ms.vmask[n % 3][2 * ch], v1 = ms.vmask[n % 3][2 * ch + 1];
-        uint32_t k0 = v0, k1 = v1;
-        if (pos < 0) {
-          k0 = k1 = 0;
-        } else if (!(t.flags & TF_CMP)) {
-          const int p0 = t.row0 + 64 * ch;
-          k0 &= window_bits(p0, pos, p.win, un.ctx, un.bits[tok]);
-          k1 &= window_bits(p0 + 32, pos, p.win, un.ctx, un.bits[tok]);
-        }
-        const bool window = !(t.flags & TF_CMP);
-        if (window || !__all_sync(0xffffffffu, (k0 & k1) == 0xffffffffu)) {
-          // In the window a row may be seen by some tokens only, and one with
-          // infinities or NaN would reach the others' sums as 0 * NaN. All rows'
-          // scores with it are not finite, in both CTAs, which one sum shows;
-          // each CTA then clears what it holds of such a row's V. A token that
-          // sees it has a NaN in l, so its result is NaN.
-          float z = 0.f;
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const uint32_t v = i < 32 ? v0 : v1, k = i < 32 ? k0 : k1;
-            const bool see = (k >> (i & 31)) & 1u;
-            z = fmaf(((v >> (i & 31)) & 1u) ? s[i] : 0.f, 0.f, z);
-            s[i] = see ? s[i] * p.scale_log2 : -INFINITY;
-          }
-          if (window && z != 0.f) {
-            // The tile's V has to be there, after the one before it was done with
-            // (its copy alone could be two phases back). A wait that fails shows
-            // at the next one.
-            if (WAIT(B_VEMPTY, n ^ 1u, 40) && WAIT(B_VFULL, n, 39))
-              for (int i = 0; i < 64; ++i) {
-                const uint32_t v = i < 32 ? v0 : v1;
-                if (!((v >> (i & 31)) & 1u)) continue;
-                const int vr = 64 * ch + i;
-                uint32_t hot = 0;
-                for (int e = 0; e < 32; ++e) {  // 16-byte pieces of the half row
-                  uint32_t w[4];
-                  const uint32_t a = v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16;
-                  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-                  constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                  for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
-                }
-                if (hot)
-                  for (int e = 0; e < 32; ++e) st_shared16(v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16, 0, 0, 0, 0);
+              for (int i = 0; i < 32; i += 4) {
+                z[0] = add2(z[0], pair(r[i], r[i + 1]));
+                z[1] = add2(z[1], pair(r[i + 2], r[i + 3]));
               }
-            // a score of -inf weighs nothing, but its row is not finite
+              const float zs = (lo(z[0]) + hi(z[0])) + (lo(z[1]) + hi(z[1]));
+              // The tile's V has to be there, after the one before it was done
+              // with (its copy alone could be two phases back). A wait that fails
+              // shows at the next one.
+              if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY, n ^ 1u, 40) && WAIT(B_VFULL, n, 39)) {
+                for (int i = 0; i < 32; ++i) {
+                  if (!((there32 >> i) & 1u)) continue;
+                  const int vr = 32 * part + i;
+                  uint32_t hot = 0;
+                  for (int e = 0; e < 32; ++e) {  // 16-byte pieces of the half row
+                    uint32_t w[4];
+                    const uint32_t a = v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+                    constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (((i < 32 ? k0 : k1) >> (i & 31)) & 1u) l = s[i] == -INFINITY ? NAN : l;
+                    for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
+                  }
+                  if (hot)
+                    for (int e = 0; e < 32; ++e) st_shared16(v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16, 0, 0, 0, 0);
+                }
+                // a score of -inf weighs nothing, but its row is not finite
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (((see >> i) & 1u) && __uint_as_float(r[i]) == -INFINITY) l = NAN;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((see >> i) & 1u)) r[i] = 0xff800000u;  // -inf
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] *= p.scale_log2;
+          for (int i = 0; i < 16; ++i) s[i] = pair(r[2 * i], r[2 * i + 1]);
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i]);
-        float* red = ms.red[n & 1];
-        red[tid] = mx;
+        for (int i = 0; i < 16; ++i) mx = max3(mx, lo(s[i]), hi(s[i]));
+        float* const red = red_row + (n & 1) * RED;
+        red[part * 64] = mx;
         sas::mbar_arrive(&bars[B_SSYNC]);
         ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
         if (!ok) break;
         ++sy;
-        mx = fmaxf(mx, red[tid ^ 64]);
+        mx = fmaxf(fmaxf(red[0], red[64]), fmaxf(red[128], red[192])) * scale;
         float fac = 1.f;
         if (mx > m + kMove || (m == -INFINITY && mx > m)) {
           fac = sas::ex2(m - mx);
           m = mx;
           l *= fac;
         }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t sc2 = twice(scale), rf2 = twice(-ref);
+        uint64_t la[2] = {0, 0};
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t x = fma2(s[i], sc2, rf2);
+          const float a = sas::ex2(lo(x)), b = sas::ex2(hi(x));
+          la[i & 1] = add2(la[i & 1], pair(__float_as_uint(a), __float_as_uint(b)));
+          w[i] = pack2<DT>(a, b);
+        }
+        la[0] = add2(la[0], la[1]);
+        l += lo(la[0]) + hi(la[0]);
         // the product before this tile's is complete, and P may be written
         ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40));
         if (!ok) break;
         sas::tc_fence_after();
         if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
 #pragma unroll 1
-          for (int x = 0; x < 256; x += 32) {
+          for (int x = 128 * gr; x < 128 * gr + 128; x += 32) {
             uint32_t r[32];
             sas::tmem_ld32(tl + TM_O + x, r);
             sas::tmem_wait_ld();
@@ -781,79 +821,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           }
           sas::tmem_wait_st();
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float la[4] = {0.f, 0.f, 0.f, 0.f};
         const uint32_t pd = p_base + ch * QSLAB + row * 128;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint32_t w[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float a = sas::ex2(s[8 * e + 2 * x] - ref), b = sas::ex2(s[8 * e + 2 * x + 1] - ref);
-            la[x] += a + b;
-            w[x] = pack2<DT>(a, b);
-          }
-          st_shared16(pd + ((e ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
-        l += (la[0] + la[1]) + (la[2] + la[3]);
+        for (int e = 0; e < 4; ++e)
+          st_shared16(pd + (((4 * gr + e) ^ (row & 7)) << 4), w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
         sas::fence_proxy_async_smem();
         sas::tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_first(&bars[B_PREADY]);
         ++n;
         if (t.flags & TF_LAST) {
-          float* rl = ms.red[2];
-          rl[tid] = l;
+          float* const rl = red_row + 2 * RED;
+          rl[part * 64] = l;
           sas::mbar_arrive(&bars[B_SSYNC]);
           ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
           if (!ok) break;
           ++sy;
-          const float lt = ch ? rl[tid ^ 64] + l : l + rl[tid ^ 64];
+          const float lt = (rl[0] + rl[64]) + (rl[128] + rl[192]);
           ok = __all_sync(0xffffffffu, WAIT(B_OFULL, u, 33));
           if (!ok) break;
           ++u;
           sas::tc_fence_after();
-          const bool there = row < un.nrows;
+          const int col0 = ch * 256 + gr * 128;  // this thread's output columns
           if (t.flags & (TF_PART0 | TF_PART1)) {
+            // [D / 4][64 rows] of float4: a warp's stores are contiguous
             float* o = p.part + ((size_t)blockIdx.x * 2 + ((t.flags & TF_PART1) ? 1 : 0)) * kPieceFloats;
-            if (ch == 0) {
+            if (part == 0) {
               o[MR * D + row] = m;
               o[MR * D + MR + row] = pos < 0 ? -1.f : lt;  // -1: the token is not in use
             }
 #pragma unroll 1
-            for (int x = 0; x < 8; ++x) {
+            for (int x = 0; x < 4; ++x) {
               uint32_t r[32];
               __syncwarp();
-              sas::tmem_ld32(tl + TM_O + 32 * x, r);
+              sas::tmem_ld32(tl + TM_O + 128 * gr + 32 * x, r);
               sas::tmem_wait_ld();
-              float4* d4 = reinterpret_cast<float4*>(o + row * D + ch * 256 + x * 32);
+              uint4* d4 = reinterpret_cast<uint4*>(o) + (size_t)((col0 + 32 * x) / 4) * MR + row;
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                d4[i] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+              for (int i = 0; i < 8; ++i) d4[i * MR] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
             }
           } else {
-            const float sink = there ? __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e : 0.f;
+            const float sink = row < un.nrows ? __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e : 0.f;
             const float top = fmaxf(m, sink);
             const float a = m == -INFINITY ? 0.f : exp2f(m - top);
             const float den = lt * a + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-            const float k = pos < 0 || m == -INFINITY && lt == 0.f ? 0.f : a / den;
+            const float k = pos < 0 || (m == -INFINITY && lt == 0.f) ? 0.f : a / den;
             const bool zero = k == 0.f;
-            if (there && ch == 0 && p.lse) p.lse[un.qrow + row] = pos < 0 ? 0.f : (top + log2f(den)) * kLn2;
-            uint8_t* orow = p.out + (un.qrow + row) * (D * 2);
+            if (row < un.nrows && part == 0 && p.lse) p.lse[un.qrow + row] = pos < 0 ? 0.f : (top + log2f(den)) * kLn2;
+            // 32 columns at a time through this warp's 2 KB of P, which is free
+            // now, so that a store instruction writes whole sectors of 8 rows
+            const uint32_t box = p_base + warp * 2048;
+            const int nr = min(32, un.nrows - (warp & 1) * 32);
+            uint8_t* out = p.out + (un.qrow + (warp & 1) * 32) * (D * 2) + col0 * 2 + (lane & 3) * 16;
+            const uint64_t k2 = twice(k);
 #pragma unroll 1
-            for (int x = 0; x < 8; ++x) {
+            for (int x = 0; x < 4; ++x) {
               uint32_t r[32];
               __syncwarp();
-              sas::tmem_ld32(tl + TM_O + 32 * x, r);
+              sas::tmem_ld32(tl + TM_O + 128 * gr + 32 * x, r);
               sas::tmem_wait_ld();
-              uint4* d4 = reinterpret_cast<uint4*>(orow + (ch * 256 + x * 32) * 2);
-              uint32_t w[16];
+              uint32_t v[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                w[i] = zero ? 0u : pack2<DT>(__uint_as_float(r[2 * i]) * k, __uint_as_float(r[2 * i + 1]) * k);
-              if (there)
+              for (int i = 0; i < 16; ++i) {
+                const uint64_t y = mul2(pair(r[2 * i], r[2 * i + 1]), k2);
+                v[i] = zero ? 0u : pack2<DT>(lo(y), hi(y));
+              }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d4[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              for (int i = 0; i < 4; ++i)
+                st_shared16(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4), v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int rr = 8 * i + (lane >> 2);
+                uint4 q4;
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(q4.x), "=r"(q4.y), "=r"(q4.z), "=r"(q4.w)
+                             : "r"(box + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4)));
+                if (rr < nr) *reinterpret_cast<uint4*>(out + (int64_t)rr * (D * 2) + x * 64) = q4;
+              }
             }
           }
           sas::tc_fence_before();
@@ -875,7 +920,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
 }
 
 // Joins the pieces of a cut unit, in order. The block of CTA c does so when c's
-// range is the first to start inside the unit; blockIdx.y takes 8 of its rows.
+// range is the first to start inside the unit; blockIdx.y takes 64 columns.
 template <int DT>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeParams p) {
   sas::pdl_wait();
@@ -893,31 +938,45 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   // the first piece is partial 0 of its CTA if the unit starts with the range
   const int first_slot = before == c.ustart ? 0 : 1;
   auto piece = [&](int r) { return p.part + ((size_t)(r * ctas + g) * 2 + (r == rank - 1 ? first_slot : 0)) * kPieceFloats; };
-  for (int i = threadIdx.x >> 7; i < 8; i += 2) {
-    const int row = blockIdx.y * 8 + i, col = threadIdx.x & 127;
-    if (row >= c.nrows) break;
+  // 64 of the 512 columns: thread = row, 16 of them
+  __shared__ __align__(16) uint8_t tile[MR * 128];
+  const int row = threadIdx.x & 63, c4 = (threadIdx.x >> 6) * 4, d4 = blockIdx.y * 16 + c4;
+  if (row < c.nrows) {
     const float sink = __ldg(p.sinks + (c.qrow + row) % p.H) * kLog2e;
     float top = sink;
     for (int r = rank - 1; r <= last; ++r) top = fmaxf(top, piece(r)[MR * D + row]);
     const float base = top == -INFINITY ? 0.f : top;
     float den = exp2f(sink - base);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
     bool used = true;
     for (int r = rank - 1; r <= last; ++r) {
       const float* q = piece(r);
       const float w = exp2f(q[MR * D + row] - base), l = q[MR * D + MR + row];
       if (l < 0.f) used = false;
-      const float4 v = reinterpret_cast<const float4*>(q + row * D)[col];
       den = fmaf(l, w, den);
-      if (w != 0.f) o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+      if (w != 0.f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 v = reinterpret_cast<const float4*>(q)[(size_t)(d4 + i) * MR + row];
+          o[4 * i] = fmaf(v.x, w, o[4 * i]), o[4 * i + 1] = fmaf(v.y, w, o[4 * i + 1]);
+          o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2]), o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3]);
+        }
     }
     const float k = used && top != -INFINITY ? 1.f / den : 0.f;
-    uint2 out = make_uint2(0u, 0u);
-    if (k != 0.f || den != den) out = make_uint2(pack2<DT>(o.x * k, o.y * k), pack2<DT>(o.z * k, o.w * k));
-    if (!used) out = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(p.out + (c.qrow + row) * (D * 2) + col * 8) = out;
-    if (col == 0 && p.lse) p.lse[c.qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = used && (k != 0.f || den != den) ? pack2<DT>(o[2 * i] * k, o[2 * i + 1] * k) : 0u;
+    uint4* to = reinterpret_cast<uint4*>(tile + row * 128 + c4 * 8);
+    to[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    to[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    if (blockIdx.y == 0 && c4 == 0 && p.lse) p.lse[c.qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < c.nrows * 8; i += 256)
+    *reinterpret_cast<uint4*>(p.out + (c.qrow + (i >> 3)) * (D * 2) + blockIdx.y * 128 + (i & 7) * 16) =
+        *reinterpret_cast<const uint4*>(tile + (i >> 3) * 128 + (i & 7) * 16);
 }
 
 size_t workspace_bytes(int sms) { return 256 + (size_t)sms * (sizeof(Cut) + 2 * kPieceFloats * sizeof(float)); }
@@ -930,7 +989,7 @@ int launch(const TreeParams& p, cudaStream_t st) {
   if (cudaGetLastError() != cudaSuccess) return SAS_ERR_CUDA;
   if (!p.split) return SAS_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * p.R * p.G, MR / 8);
+  cfg.gridDim = dim3(2 * p.R * p.G, D / 64);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -986,7 +1045,7 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.bs[0] = ori_bs, p.bs[1] = cmp_bs;
   p.bt_stride[0] = ori_stride, p.bt_stride[1] = cmp_stride;
   p.nblk[0] = ori_nblk, p.nblk[1] = cmp_nblk;
-  p.idx = idx, p.sinks = sinks, p.scale_log2 = softmax_scale * kLog2e;
+  p.idx = idx, p.sinks = sinks, p.scale_log2 = softmax_scale == 0.f ? 1e-30f : softmax_scale * kLog2e;  // 0 * -inf would not mask
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.total = reinterpret_cast<int64_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + 256);
