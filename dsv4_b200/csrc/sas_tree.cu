@@ -69,7 +69,7 @@ constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
 // *FULL and the others that both CTAs' threads arrive on count in the first
 // CTA, whose MMA thread waits; X* are the second CTA's copies having landed.
 enum Bar { B_KFULL = 0, B_VFULL, B_QFULL, B_XK, B_XV, B_XQ, B_KEMPTY, B_VEMPTY, B_QEMPTY, B_MASK, B_SFULL = B_MASK + 3, B_PREADY = B_SFULL + 2,
-           B_OFULL, B_OEMPTY, B_SSYNC, B_CFULL, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
+           B_OFULL, B_OEMPTY, B_SSYNC, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
 
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
@@ -178,11 +178,14 @@ __device__ __forceinline__ void commit2(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-// Arrive on `bar` of the pair's first CTA, with cluster scope.
+// Arrive on `bar` of the pair's first CTA. What it announces is in this CTA's
+// shared or tensor memory, written before a proxy or tcgen05 fence of the
+// writers, and read there by the pair's MMAs: CTA scope is enough, and a cluster-scope
+// release would wait for the warp's global stores too.
 __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(sas::smem_u32(bar))
+      "mbarrier.arrive.release.cta.shared::cluster.b64 _, [a];\n\t}" ::"r"(sas::smem_u32(bar))
       : "memory");
 }
 // sas::mbar_wait for a barrier that the other CTA's threads arrive on
@@ -293,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     for (int i = 0; i < 3; ++i) sas::mbar_init(&bars[B_MASK + i], kLoadWarps);
     sas::mbar_init(&bars[B_PREADY], 2 * kSmWarps);  // softmax warps of both CTAs
     sas::mbar_init(&bars[B_OEMPTY], 2 * kSmWarps);
-    sas::mbar_init(&bars[B_SSYNC], 32 * kSmWarps);
+    for (int i = 0; i < 2; ++i) sas::mbar_init(&bars[B_SSYNC + i], kSmWarps / 2);  // the warps of 32 rows
     for (int i = 0; i < kRing; ++i) {
       sas::mbar_init(&bars[B_CFULL + i], 1);
       sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + kSmWarps);
@@ -781,8 +784,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         for (int i = 0; i < 16; ++i) mx = max3(mx, lo(s[i]), hi(s[i]));
         float* const red = red_row + (n & 1) * RED;
         red[part * 64] = mx;
-        sas::mbar_arrive(&bars[B_SSYNC]);
-        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
+        __syncwarp();
+        if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
+        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
         if (!ok) break;
         ++sy;
         mx = fmaxf(fmaxf(red[0], red[64]), fmaxf(red[128], red[192])) * scale;
@@ -833,8 +837,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (t.flags & TF_LAST) {
           float* const rl = red_row + 2 * RED;
           rl[part * 64] = l;
-          sas::mbar_arrive(&bars[B_SSYNC]);
-          ok = __all_sync(0xffffffffu, WAIT(B_SSYNC, sy, 32));
+          __syncwarp();
+          if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
+          ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
           if (!ok) break;
           ++sy;
           const float lt = (rl[0] + rl[64]) + (rl[128] + rl[192]);
