@@ -134,7 +134,7 @@ struct Req {
   bool bad;
   __device__ __forceinline__ int64_t all() const { return (int64_t)units * tiles; }
 };
-__device__ Req request(const TreeParams& p, int b) {
+__device__ __noinline__ Req request(const TreeParams& p, int b) {
   Req r;
   if (p.layout == SAS_LAYOUT_TND) {
     const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
@@ -188,8 +188,13 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
       "mbarrier.arrive.release.cta.shared::cluster.b64 _, [a];\n\t}" ::"r"(sas::smem_u32(bar))
       : "memory");
 }
-// sas::mbar_wait for a barrier that the other CTA's threads arrive on
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+// Bounded waits, as sas::mbar_wait. Only the first try is inlined: with the
+// loops in every place the kernel had 159 KB of code, and its warps, each in
+// another part of it, waited for instructions. PAIR: the other CTA's threads
+// arrive on the barrier.
+template <bool PAIR>
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+  if (!PAIR) return sas::mbar_try_wait(bar, parity);
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -200,11 +205,11 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
-  if (try_wait_cluster(bar, parity)) return true;
+template <bool PAIR>
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
   const uint64_t t0 = sas::globaltimer(), lim = ctl->limit_ns;
   for (uint32_t n = 1;; ++n) {
-    if (try_wait_cluster(bar, parity)) return true;
+    if (try_wait<PAIR>(bar, parity)) return true;
     if ((n & 63u) == 0) {
       if (ctl->abort) return false;
       if (sas::globaltimer() - t0 > lim) {
@@ -214,6 +219,10 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, vol
       }
     }
   }
+}
+template <bool PAIR>
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
+  return try_wait<PAIR>(bar, parity) || wait_on<PAIR>(bar, parity, ctl, status, where);
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -266,7 +275,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >=
 
 // The 32 rows from position p0 that a token at position s sees: the cached
 // ones of its window, then the drafted ones of its bitmap.
-__device__ __forceinline__ uint32_t window_bits(int p0, int s, int win, int ctx, const uint32_t* bits) {
+__device__ __noinline__ uint32_t window_bits(int p0, int s, int win, int ctx, const uint32_t* bits) {
   const int c = ctx - p0;  // cached rows before the drafted ones
   uint32_t m = low_bits(c) & ~low_bits(s - win - p0);
   if (c <= 0) {
@@ -276,6 +285,26 @@ __device__ __forceinline__ uint32_t window_bits(int p0, int s, int win, int ctx,
     m |= bits[0] << c;
   }
   return m;
+}
+
+// Zeroes the half rows [row0, row0 + 32) of a tile's V, of those in `there`,
+// that hold infinities or NaN.
+template <int DT>
+__device__ __noinline__ void clear_rows(uint32_t v_base, uint32_t there, int row0) {
+  constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;  // the exponent's bits
+  for (; there; there &= there - 1) {
+    const uint32_t at = v_base + (row0 + __ffs(there) - 1) * 128;
+    uint32_t hot = 0;
+#pragma unroll 1
+    for (int e = 0; e < 32; ++e) {  // 16-byte pieces
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + (e >> 3) * VSLAB + (e & 7) * 16));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
+    }
+#pragma unroll 1
+    for (int e = 0; hot && e < 32; ++e) st_shared16(at + (e >> 3) * VSLAB + (e & 7) * 16, 0, 0, 0, 0);
+  }
 }
 
 template <int DT>
@@ -366,8 +395,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   volatile sas::CtaCtl* ctl = &ms.ctl;
   const uint32_t q_base = sas::smem_u32(smem + OFF_Q), k_base = sas::smem_u32(smem + OFF_K),
                  v_base = sas::smem_u32(smem + OFF_V), p_base = sas::smem_u32(smem + OFF_P);
-#define WAIT(bar, par, id) sas::mbar_wait(&bars[bar], (par)&1, ctl, p.status, id)
-#define WAIT_PAIR(bar, par, id) wait_cluster(&bars[bar], (par)&1, ctl, p.status, id)
+#define WAIT(bar, par, id) wait<false>(&bars[bar], (par)&1, ctl, p.status, id)
+#define WAIT_PAIR(bar, par, id) wait<true>(&bars[bar], (par)&1, ctl, p.status, id)
 
   if (warp == kCoordWarp) {
     // ================================================= coordinator
@@ -535,7 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       if (!__all_sync(0xffffffffu, WAIT(B_VEMPTY, m ^ 1u, 23))) return false;
       const uint8_t* src = v_pool + side * 512 + lane * 16;
       const uint32_t dst = v_base + (lane >> 3) * VSLAB;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 16; ++i) {
         const int ri = __shfl_sync(0xffffffffu, v_row, i);
         const int r = (i < 8 ? side : side ^ 1) * 64 + lw * 8 + (i & 7);
@@ -545,22 +574,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       cp_arrive(&bars[B_VFULL]);
       return true;
     };
-    bool ok = true;
-    while (ok) {
+    while (true) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
       t = ms.ring[c % kRing];
-      if (t.flags & (TF_END | TF_ZERO)) {  // no K to go first (and a unit may end here: see the MMA issuer)
-        if (v_due) ok = load_v(n - 1);
-        v_due = false;
-        if (t.flags & TF_END) break;
-      } else {
-        const int row = resolve();
+      const bool rows = !(t.flags & (TF_END | TF_ZERO));
+      int row = -1;
+      const uint8_t* pool = nullptr;
+      if (rows) {
+        row = resolve();
         if (t.flags & TF_FIRST) {
           if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
           const Unit& u = ms.units[t.uslot];
           const int nr = u.nrows;
           const uint8_t* src = p.q + (nr ? u.qrow : 0) * (D * 2) + lane * 16;
-#pragma unroll
+#pragma unroll 2
           for (int i = 0; i < MR / kLoadWarps; ++i) {
             const int r = lw * (MR / kLoadWarps) + i;
             const uint32_t dst = q_base + r * 128 + (((lane & 7) ^ (r & 7)) << 4) + (lane >> 3) * QSLAB;
@@ -581,10 +608,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           bytes[(side ^ 1) * 8 + lw] = (uint8_t)(vm >> 8);
           sas::mbar_arrive(&bars[B_MASK + n % 3]);
         }
-        const uint8_t* pool = p.kv[(t.flags & TF_CMP) ? 1 : 0];
+        pool = p.kv[(t.flags & TF_CMP) ? 1 : 0];
         const uint8_t* src = pool + lane * 16;
         const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 8 * 128;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 8; ++i) {  // all 64 rows: absent ones are zero, so that their scores are finite
           const int ri = __shfl_sync(0xffffffffu, row, i);
 #pragma unroll
@@ -593,8 +620,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
                  src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
         }
         cp_arrive(&bars[B_KFULL]);
-        if (v_due) ok = load_v(n - 1);
-        v_row = row, v_top = top(t), v_pool = pool, v_due = true;
+      }
+      if (v_due && !load_v(n - 1)) break;
+      v_due = rows;
+      if (t.flags & TF_END) break;
+      if (rows) {
+        v_row = row, v_top = top(t), v_pool = pool;
         ++n;
       }
       __syncwarp();
@@ -610,6 +641,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       constexpr int fmt = DT == SAS_DTYPE_BF16 ? 1 : 0;
       constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, UR, CH, 0, 0);
       constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
+      const uint64_t q_desc = sas::umma_desc_sw128(q_base, 16, 1024), k_desc = sas::umma_desc_sw128(k_base, 16, 1024);
+      const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
       uint32_t c = 0, n = 0, u = 0, vu = 0;
       Tile last{};  // tile n - 1
       bool due = false;  // its product is not issued yet
@@ -626,11 +659,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         sas::fence_proxy_async_smem();
         sas::tc_fence_after();
         const int steps = max(1, (last.nrows + 15) / 16);
+#pragma unroll 1
         for (int h = 0; h < 2; ++h)
+#pragma unroll 1
           for (int ks = 0; ks < steps; ++ks)
-            umma2(tmem + TM_O + 128 * h, sas::umma_desc_sw128(p_base + (ks >> 2) * QSLAB + (ks & 3) * 32, 16, 1024),
-                  sas::umma_desc_sw128(v_base + 2 * h * VSLAB + ks * 2048, VSLAB, 1024), id_o,
-                  !((last.flags & TF_FIRST) && ks == 0));
+            umma2(tmem + TM_O + 128 * h, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
+                  v_desc + ((2 * h * VSLAB + ks * 2048) >> 4), id_o, !((last.flags & TF_FIRST) && ks == 0));
         commit2(&bars[B_VEMPTY]);
         if (last.flags & TF_LAST) {
           commit2(&bars[B_OFULL]);
@@ -641,13 +675,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       while (true) {
         if (!WAIT(B_CFULL + c % kRing, c / kRing, 24)) break;
         const Tile t = ms.ring[c % kRing];
-        if (t.flags & (TF_END | TF_ZERO)) {
-          // The product may not wait for a next tile with rows: the softmax
-          // warps wait for it before they release the ring's next entries.
-          if (due && !product(n - 1)) break;
-          due = false;
-          if (t.flags & TF_END) break;
-        } else {
+        const bool rows = !(t.flags & (TF_END | TF_ZERO));
+        if (rows) {
           if (side) {
             if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
             if (!pass_on(B_KFULL, B_XK, n)) break;
@@ -659,19 +688,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             if (!WAIT(B_KFULL, n, 26) || !WAIT_PAIR(B_XK, n, 38)) break;
             sas::fence_proxy_async_smem();
             sas::tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int s = 0; s < 8; ++s)
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                umma2(tmem + TM_S + 64 * (n & 1), sas::umma_desc_sw128(q_base + s * QSLAB + kk * 32, 16, 1024),
-                      sas::umma_desc_sw128(k_base + s * KSLAB + kk * 32, 16, 1024), id_s, (s | kk) != 0);
+                umma2(tmem + TM_S + 64 * (n & 1), q_desc + ((s * QSLAB + kk * 32) >> 4), k_desc + ((s * KSLAB + kk * 32) >> 4), id_s,
+                      (s | kk) != 0);
             commit2(&bars[B_SFULL + (n & 1)]);
             commit2(&bars[B_KEMPTY]);
             if (t.flags & TF_LAST) commit2(&bars[B_QEMPTY]);
           }
-          if (due && !product(n - 1)) break;
+        }
+        // Also where no tile with rows follows: the softmax warps wait for the
+        // product of a unit's end before they release the ring's next entries.
+        if (due && !product(n - 1)) break;
+        due = rows;
+        if (t.flags & TF_END) break;
+        if (rows) {
           last = t;
-          due = true;
           ++n;
         }
         sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
@@ -751,21 +785,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
               // with (its copy alone could be two phases back). A wait that fails
               // shows at the next one.
               if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY, n ^ 1u, 40) && WAIT(B_VFULL, n, 39)) {
-                for (int i = 0; i < 32; ++i) {
-                  if (!((there32 >> i) & 1u)) continue;
-                  const int vr = 32 * part + i;
-                  uint32_t hot = 0;
-                  for (int e = 0; e < 32; ++e) {  // 16-byte pieces of the half row
-                    uint32_t w[4];
-                    const uint32_t a = v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16;
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-                    constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) hot |= ((w[x] & ex) == ex) | (((w[x] >> 16) & ex) == ex);
-                  }
-                  if (hot)
-                    for (int e = 0; e < 32; ++e) st_shared16(v_base + (e >> 3) * VSLAB + vr * 128 + (e & 7) * 16, 0, 0, 0, 0);
-                }
+                clear_rows<DT>(v_base, there32, 32 * part);
                 // a score of -inf weighs nothing, but its row is not finite
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
