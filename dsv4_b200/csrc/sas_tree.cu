@@ -98,6 +98,7 @@ struct Misc {
   uint32_t vmask[3][4];  // tile n in n % 3
   float red[3][32 * kSmWarps];  // row maxima of even and odd tiles, row sums of a unit
   Tile ring[kRing];
+  uint32_t vis[kRing][kMaxTok][4];  // a published tile's 128 rows: those that each token sees
   Unit units[kUnitSlots];
   int parents[kMaxTree];
 };
@@ -407,6 +408,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     auto publish = [&](int flags, int row0, int nrows, int us) -> bool {
       const int slot = c % kRing;
       if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + slot, (c / kRing) ^ 1u, 20))) return false;
+      if (!(flags & (TF_END | TF_ZERO))) {  // lane: token, 32 rows
+        const Unit& un = ms.units[us];
+        const int tok = lane >> 2, pos = un.pos[tok];
+        uint32_t m = 0;
+        if (pos >= 0) m = flags & TF_CMP ? 0xffffffffu : window_bits(row0 + 32 * (lane & 3), pos, p.win, un.ctx, un.bits[tok]);
+        ms.vis[slot][tok][lane & 3] = m;
+        __syncwarp();
+      }
       if (lane == 0) {
         ms.ring[slot] = Tile{flags, row0, nrows, us};
         sas::mbar_arrive(&bars[B_CFULL + slot]);
@@ -489,6 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         un.nrows = nrows;
         un.roff = (int)(row_in % p.H);
       }
+      __syncwarp();
       const bool any = __any_sync(0xffffffffu, pos >= 0);
       const bool whole = k0 == 0 && k1 == r.tiles;
       if (k0 > 0 && any) {
@@ -730,8 +740,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     const float scale = flip ? -p.scale_log2 : p.scale_log2;
     uint32_t c = 0, n = 0, u = 0, sy = 0;
     float m = -INFINITY, l = 0.f;
-    int pos = -1, tok = 0;
-    bool ok = true;
+    int tok = 0;
+    bool used = false, ok = true;
+    float sink = 0.f;
     while (ok) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 29))) break;
       const Tile t = ms.ring[c % kRing];
@@ -746,16 +757,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           m = -INFINITY;
           l = 0.f;
           tok = p.scenario == 3 ? 0 : min((un.roff + row) / p.H, kMaxTok - 1);
-          pos = row < un.nrows ? un.pos[tok] : -1;
+          used = row < un.nrows && un.pos[tok] >= 0;
+          sink = __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e;
         }
+        uint32_t see = used ? ms.vis[c % kRing][tok][part] : 0u;
         // rows of the tile that are there, and those that this row's token sees
         ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30));
         if (!ok) break;
         const bool window = !(t.flags & TF_CMP);
         const uint32_t there32 = ms.vmask[n % 3][part];
-        uint32_t see = there32;
-        if (pos < 0) see = 0;
-        else if (window) see &= window_bits(t.row0 + 32 * part, pos, p.win, un.ctx, un.bits[tok]);
+        see &= there32;
         ok = __all_sync(0xffffffffu, WAIT(B_SFULL + (n & 1), n >> 1, 31));
         if (!ok) break;
         sas::tc_fence_after();
@@ -806,29 +817,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         red[part * 64] = mx;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
-        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
-        if (!ok) break;
-        ++sy;
-        mx = fmaxf(fmaxf(red[0], red[64]), fmaxf(red[128], red[192])) * scale;
-        float fac = 1.f;
-        if (mx > m + kMove || (m == -INFINITY && mx > m)) {
-          fac = sas::ex2(m - mx);
-          m = mx;
-          l *= fac;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        const uint64_t sc2 = twice(scale), rf2 = twice(-ref);
-        uint64_t la[2] = {0, 0};
+        // P with the reference as it stands, while the row's other maxima come;
+        // again if one of the warp's rows moves
+        const uint64_t sc2 = twice(scale);
         uint32_t w[16];
+        float sum = 0.f;
+        auto exps = [&]() {
+          const uint64_t rf2 = twice(m == -INFINITY ? 0.f : -m);
+          uint64_t la[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint64_t x = fma2(s[i], sc2, rf2);
-          const float a = sas::ex2(lo(x)), b = sas::ex2(hi(x));
-          la[i & 1] = add2(la[i & 1], pair(__float_as_uint(a), __float_as_uint(b)));
-          w[i] = pack2<DT>(a, b);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x = fma2(s[i], sc2, rf2);
+            const float a = sas::ex2(lo(x)), b = sas::ex2(hi(x));
+            la[i & 1] = add2(la[i & 1], pair(__float_as_uint(a), __float_as_uint(b)));
+            w[i] = pack2<DT>(a, b);
+          }
+          la[0] = add2(la[0], la[1]);
+          sum = lo(la[0]) + hi(la[0]);
+        };
+        bool redo = t.flags & TF_FIRST;
+        float fac = 1.f;
+#pragma unroll 1
+        for (int pass = redo; pass < 2; ++pass) {
+          if (pass == 1) {
+            ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
+            if (!ok) break;
+            ++sy;
+            mx = fmaxf(fmaxf(red[0], red[64]), fmaxf(red[128], red[192])) * scale;
+            if (mx > m + kMove || (m == -INFINITY && mx > m)) {
+              fac = sas::ex2(m - mx);
+              m = mx;
+              l *= fac;
+            }
+            if (!redo && !__any_sync(0xffffffffu, fac != 1.f)) break;
+          }
+          exps();
         }
-        la[0] = add2(la[0], la[1]);
-        l += lo(la[0]) + hi(la[0]);
+        if (!ok) break;
+        l += sum;
         // the product before this tile's is complete, and P may be written
         ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40));
         if (!ok) break;
@@ -873,7 +899,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             float* o = p.part + ((size_t)blockIdx.x * 2 + ((t.flags & TF_PART1) ? 1 : 0)) * kPieceFloats;
             if (part == 0) {
               o[MR * D + row] = m;
-              o[MR * D + MR + row] = pos < 0 ? -1.f : lt;  // -1: the token is not in use
+              o[MR * D + MR + row] = used ? lt : -1.f;  // -1: the token is not in use
             }
 #pragma unroll 1
             for (int x = 0; x < 4; ++x) {
@@ -886,13 +912,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
               for (int i = 0; i < 8; ++i) d4[i * MR] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
             }
           } else {
-            const float sink = row < un.nrows ? __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e : 0.f;
             const float top = fmaxf(m, sink);
             const float a = m == -INFINITY ? 0.f : exp2f(m - top);
             const float den = lt * a + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-            const float k = pos < 0 || (m == -INFINITY && lt == 0.f) ? 0.f : a / den;
+            const float k = !used || (m == -INFINITY && lt == 0.f) ? 0.f : a / den;
             const bool zero = k == 0.f;
-            if (row < un.nrows && part == 0 && p.lse) p.lse[un.qrow + row] = pos < 0 ? 0.f : (top + log2f(den)) * kLn2;
+            if (row < un.nrows && part == 0 && p.lse) p.lse[un.qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
             // 32 columns at a time through this warp's 2 KB of P, which is free
             // now, so that a store instruction writes whole sectors of 8 rows
             const uint32_t box = p_base + warp * 2048;
