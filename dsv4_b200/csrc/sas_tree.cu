@@ -31,11 +31,14 @@
 // P, l and O keep one common scale. P is rounded to the I/O type for the
 // product, l sums it unrounded (as the framework's forward does).
 //
-// Roles (18 warps): 0-7 softmax and epilogue (thread = row, 32 of the tile's
-// columns), 8 MMA issuer (in the pair's second CTA it passes on that its copies
-// have landed), 9 coordinator (walks the range and the trees and publishes
-// tiles in a ring; the pair's two coordinators take the same steps), 10-17
-// loaders (cp.async; 8 K rows and 16 V half rows of a tile each).
+// Roles (23 warps), each of which walks the ring of published tiles by itself:
+//   0-7    softmax: thread = row, 32 of the tile's columns;
+//   8-11   epilogue: O of a finished unit leaves while the next one runs;
+//   12, 13 issue the scores and the products (first CTA), or tell the first CTA
+//          that this one's K and Q, or V, have landed (second CTA);
+//   14     coordinator: walks the range and the trees, works out which rows each
+//          token sees and publishes tiles (the pair's two take the same steps);
+//   15-18  copy Q and K, 19-22 V (cp.async, one row's 512 bytes at a time).
 #include "sas_common.cuh"
 
 namespace {
@@ -52,10 +55,11 @@ constexpr int kMaxCtx = 1 << 30;  // rows cached before them
 constexpr int KSLAB = 64 * 128;   // 64 columns of the CTA's 64 K rows
 constexpr int VSLAB = CH * 128;   // 64 columns of the tile's V rows
 constexpr int QSLAB = MR * 128;   // 64 columns of Q, or of P
-constexpr int kSmWarps = 8, kMmaWarp = 8, kCoordWarp = 9, kLoadWarp0 = 10, kLoadWarps = 8;
-constexpr int kThreads = 32 * (kLoadWarp0 + kLoadWarps);
-constexpr int kRing = 4;          // tiles the coordinator may be ahead
-constexpr int kUnitSlots = 6;     // > kRing + 1: no slot is rewritten while a published tile names it
+constexpr int kSmWarps = 8, kEpiWarp0 = 8, kEpiWarps = 4, kQkWarp = 12, kPvWarp = 13, kCoordWarp = 14, kKWarp0 = 15, kVWarp0 = 19,
+              kLoadWarps = 4;
+constexpr int kThreads = 32 * 23;
+constexpr int kRing = 5;          // tiles the coordinator may be ahead
+constexpr int kUnitSlots = 7;     // > kRing + 1: no slot is rewritten while a published tile names it
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMove = 8.f;      // log2 units the running maximum may lag
@@ -66,10 +70,11 @@ constexpr int OFF_V = OFF_K + 8 * KSLAB;
 constexpr int OFF_P = OFF_V + 4 * VSLAB;
 constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
 
-// *FULL and the others that both CTAs' threads arrive on count in the first
-// CTA, whose MMA thread waits; X* are the second CTA's copies having landed.
-enum Bar { B_KFULL = 0, B_VFULL, B_QFULL, B_XK, B_XV, B_XQ, B_KEMPTY, B_VEMPTY, B_QEMPTY, B_MASK, B_SFULL = B_MASK + 3, B_PREADY = B_SFULL + 2,
-           B_OFULL, B_OEMPTY, B_SSYNC, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT };
+// X* count in the first CTA: the second's copies have landed. So do SEMPTY (the
+// scores are read), PREADY and OEMPTY, on which both CTAs' warps arrive.
+enum Bar { B_KFULL = 0, B_VFULL, B_QFULL, B_XK, B_XV, B_XQ, B_KEMPTY, B_VEMPTY, B_QEMPTY, B_MASK, B_SFULL = B_MASK + 3,
+           B_SEMPTY = B_SFULL + 2, B_PREADY = B_SEMPTY + 2, B_OFULL, B_OEMPTY, B_FIN, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2,
+           B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
 
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
@@ -82,7 +87,11 @@ struct Unit {
   int64_t qrow;              // first row of [T * H]
   int nrows, roff;           // roff: head of the first row
   int pos[kMaxTok];          // s of each token, -1: unused
-  uint32_t bits[kMaxTok][kWords];  // drafted rows each token sees
+};
+struct Fin {  // a finished unit, from the softmax warps to the epilogue
+  float m[MR], l[4][MR];     // l: of a quarter of the columns; < 0 in the first: the row's token is not in use
+  int64_t qrow;
+  int nrows, roff, part;     // part: -1, or the CTA's partial
 };
 struct Cut {  // the piece a CTA's range starts with, when it is not its unit's first
   int64_t ustart, uend, qrow;
@@ -95,12 +104,15 @@ struct Misc {
   int start_b;
   int64_t start_prefix, total;
   int64_t wsum[kThreads / 32];
-  uint32_t vmask[3][4];  // tile n in n % 3
-  float red[3][32 * kSmWarps];  // row maxima of even and odd tiles, row sums of a unit
+  uint32_t vmask[3][4];  // rows of tile n that are there, in n % 3
+  float red[2][4][MR];   // row maxima of even and odd tiles, by quarter
   Tile ring[kRing];
   uint32_t vis[kRing][kMaxTok][4];  // a published tile's 128 rows: those that each token sees
   Unit units[kUnitSlots];
-  int parents[kMaxTree];
+  Fin fin[2];            // of even and odd units
+  uint32_t bits[kMaxTok][kWords];   // coordinator: drafted rows each token of its unit sees
+  int16_t parents[kMaxTree];        // coordinator: its request's, -2: not a drafted token's index
+  uint4 box[kEpiWarps][128];        // epilogue: 32 rows x 64 bytes per warp
 };
 constexpr int SMEM_BYTES = OFF_MISC + (int)sizeof(Misc) + 1024;
 static_assert(SMEM_BYTES <= 232448, "shared memory over the per-CTA limit");
@@ -326,26 +338,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   const int side = blockIdx.x & 1;  // the CTA's place in its pair
   const int g = (blockIdx.x >> 1) % p.G, rank = (blockIdx.x >> 1) / p.G;
   if (tid == 0) {
-    sas::mbar_init(&bars[B_KFULL], 32 * kLoadWarps);
-    sas::mbar_init(&bars[B_VFULL], 32 * kLoadWarps);
-    sas::mbar_init(&bars[B_QFULL], 32 * kLoadWarps);
-    for (int i : {(int)B_XK, (int)B_XV, (int)B_XQ, (int)B_KEMPTY, (int)B_VEMPTY, (int)B_QEMPTY, (int)B_SFULL, B_SFULL + 1, (int)B_OFULL, (int)B_DRAIN})
-      sas::mbar_init(&bars[i], 1);
-    for (int i = 0; i < 3; ++i) sas::mbar_init(&bars[B_MASK + i], kLoadWarps);
-    sas::mbar_init(&bars[B_PREADY], 2 * kSmWarps);  // softmax warps of both CTAs
-    sas::mbar_init(&bars[B_OEMPTY], 2 * kSmWarps);
-    for (int i = 0; i < 2; ++i) sas::mbar_init(&bars[B_SSYNC + i], kSmWarps / 2);  // the warps of 32 rows
-    for (int i = 0; i < kRing; ++i) {
-      sas::mbar_init(&bars[B_CFULL + i], 1);
-      sas::mbar_init(&bars[B_CEMPTY + i], kLoadWarps + 1 + kSmWarps);
-    }
+    auto init = [&](int bar, int n, int count) {
+      for (int i = 0; i < n; ++i) sas::mbar_init(&bars[bar + i], count);
+    };
+    init(B_KFULL, 3, 32 * kLoadWarps);  // and V, Q
+    init(B_XK, 6, 1);                   // XK, XV, XQ, KEMPTY, VEMPTY, QEMPTY
+    init(B_MASK, 3, kLoadWarps);
+    init(B_SFULL, 2, 1);
+    init(B_SEMPTY, 3, 2 * kSmWarps);    // and PREADY: softmax warps of both CTAs
+    init(B_OFULL, 1, 1);
+    init(B_OEMPTY, 1, 2 * kEpiWarps);
+    init(B_FIN, 2, kSmWarps);
+    init(B_SSYNC, 2, kSmWarps / 2);     // the warps of 32 rows
+    init(B_CFULL, kRing, 1);
+    init(B_CEMPTY, kRing, 2 * kLoadWarps + 2 + kSmWarps);
+    init(B_DRAIN, 2, 1);
     sas::fence_mbar_init();
     ms.ctl.abort = 0;
     ms.ctl.limit_ns = SAS_WAIT_LIMIT_NS;
     ms.start_b = p.B;
     ms.start_prefix = 0;
   }
-  if (warp == kMmaWarp) {
+  if (warp == kQkWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sas::smem_u32(&ms.tmem)), "r"(TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -404,6 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   volatile sas::CtaCtl* ctl = &ms.ctl;
   const uint32_t q_base = sas::smem_u32(smem + OFF_Q), k_base = sas::smem_u32(smem + OFF_K),
                  v_base = sas::smem_u32(smem + OFF_V), p_base = sas::smem_u32(smem + OFF_P);
+  // (the waits' ids, added to SAS_ERR_TIMEOUT_BASE in the status word, are 20 and up)
 #define WAIT(bar, par, id) wait<false>(&bars[bar], (par)&1, ctl, p.status, id)
 #define WAIT_PAIR(bar, par, id) wait<true>(&bars[bar], (par)&1, ctl, p.status, id)
 
@@ -420,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         const Unit& un = ms.units[us];
         const int tok = lane >> 2, pos = un.pos[tok];
         uint32_t m = 0;
-        if (pos >= 0) m = flags & TF_CMP ? 0xffffffffu : window_bits(row0 + 32 * (lane & 3), pos, p.win, un.ctx, un.bits[tok]);
+        if (pos >= 0) m = flags & TF_CMP ? 0xffffffffu : window_bits(row0 + 32 * (lane & 3), pos, p.win, un.ctx, ms.bits[tok]);
         ms.vis[slot][tok][lane & 3] = m;
         __syncwarp();
       }
@@ -451,7 +466,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       if (b != cached) {
         __syncwarp();
         if (!r.bad)
-          for (int i = lane; i < r.n; i += 32) ms.parents[i] = __ldg(p.parents + r.base + i);
+          for (int i = lane; i < r.n; i += 32) {
+            const int q = __ldg(p.parents + r.base + i);
+            ms.parents[i] = (int16_t)(q < -1 ? -2 : min(q, kMaxTree));
+          }
         else if (lane == 0 && u == 0 && k0 == 0)
           bad(p, SAS_ERR_BAD_TREE);
         cached = b;
@@ -472,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       int pos = -1;
       if (lane < kMaxUnitTok) {
         const int slot = lane - mine;
-        uint32_t* bits = slot >= 0 && slot < kMaxTok ? un.bits[slot] : nullptr;
+        uint32_t* bits = slot >= 0 && slot < kMaxTok ? ms.bits[slot] : nullptr;
         const int words = max((min(r.n, kMaxTree) + 31) / 32, 1);
         // window_bits reads up to five words past the last one with a bit
         if (bits)
@@ -540,110 +558,81 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     }
     if (lane == 0 && !lead_cut && rank < R) p.cuts[blockIdx.x].cut = 0;
     if (ok) publish(TF_END, 0, 0, 0);
-  } else if (warp >= kLoadWarp0) {
+  } else if (warp >= kKWarp0) {
     // ================================================= loaders
-    // K of a tile, then V of the tile before: the order in which the buffers
-    // come free (K after the scores, V after the product).
-    const int lw = warp - kLoadWarp0;
+    // Warps of K: 16 of this CTA's 64 K rows of a tile each, and 16 rows of Q.
+    // Warps of V: 32 of the tile's 128 rows each, this CTA's 256 columns; they
+    // also tell which rows are there.
+    const bool is_v = warp >= kVWarp0;
+    const int lw = (warp - kKWarp0) & 3;
+    const int my_row = is_v ? lw * 32 + lane : side * 64 + lw * 16 + (lane & 15);
     uint32_t c = 0, n = 0, q = 0;
-    // Lanes 0-7: tile rows [64 side + 8 lw, + 8), which are also this warp's K
-    // rows; lanes 8-15: the same of the other CTA's half.
-    const int my_row = (lane < 8 ? side : side ^ 1) * 64 + lw * 8 + (lane & 7);
-    Tile t{};
-    auto resolve = [&]() -> int {  // pool row of tile row my_row (-1: none)
-      if (lane >= 16 || my_row >= t.nrows) return -1;
-      const Unit& u = ms.units[t.uslot];
-      const int f = (t.flags & TF_CMP) ? 1 : 0;
-      int pos = t.row0 + my_row;
-      if (t.flags & TF_TOPK) {
-        pos = __ldg(p.idx + (int64_t)u.tok * p.K + pos);
-        if (pos < 0 || pos >= u.thr) return -1;
-      }
-      const int col = pos / p.bs[f];
-      if (col >= p.bt_stride[f]) {
-        bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
-        return -1;
-      }
-      const int blk = __ldg(p.bt[f] + (int64_t)u.b * p.bt_stride[f] + col);
-      if (blk < 0) return -1;
-      if (blk >= p.nblk[f]) {
-        bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
-        return -1;
-      }
-      return blk * p.bs[f] + (pos - col * p.bs[f]);
-    };
-    // V rows of a tile that are copied (others stay as they are): whole K steps of the product
-    auto top = [](const Tile& x) { return max(16, (x.nrows + 15) & ~15); };
-    int v_row = -1, v_top = 0;
-    bool v_due = false;  // V of tile n - 1 is not copied yet
-    const uint8_t* v_pool = nullptr;
-    // V of tile m: 512 bytes (this CTA's 256 columns) of rows my_row of lanes 0-15
-    auto load_v = [&](uint32_t m) -> bool {
-      if (!__all_sync(0xffffffffu, WAIT(B_VEMPTY, m ^ 1u, 23))) return false;
-      const uint8_t* src = v_pool + side * 512 + lane * 16;
-      const uint32_t dst = v_base + (lane >> 3) * VSLAB;
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const int ri = __shfl_sync(0xffffffffu, v_row, i);
-        const int r = (i < 8 ? side : side ^ 1) * 64 + lw * 8 + (i & 7);
-        if (r < v_top)
-          cp16(dst + r * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
-      }
-      cp_arrive(&bars[B_VFULL]);
-      return true;
-    };
     while (true) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
-      t = ms.ring[c % kRing];
-      const bool rows = !(t.flags & (TF_END | TF_ZERO));
-      int row = -1;
-      const uint8_t* pool = nullptr;
-      if (rows) {
-        row = resolve();
-        if (t.flags & TF_FIRST) {
+      const Tile t = ms.ring[c % kRing];
+      if (t.flags & TF_END) break;
+      if (!(t.flags & TF_ZERO)) {
+        const Unit& u = ms.units[t.uslot];
+        const int f = (t.flags & TF_CMP) ? 1 : 0;
+        int row = -1;  // pool row of tile row my_row, -1: none
+        if (my_row < t.nrows) {
+          int pos = t.row0 + my_row;
+          if (t.flags & TF_TOPK) pos = __ldg(p.idx + (int64_t)u.tok * p.K + pos);
+          if (!(t.flags & TF_TOPK) || (pos >= 0 && pos < u.thr)) {
+            const int col = pos / p.bs[f];
+            const int blk = col < p.bt_stride[f] ? __ldg(p.bt[f] + (int64_t)u.b * p.bt_stride[f] + col) : 0x7fffffff;
+            if (blk >= p.nblk[f]) bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
+            else if (blk >= 0) row = blk * p.bs[f] + (pos - col * p.bs[f]);
+          }
+        }
+        if (!is_v && (t.flags & TF_FIRST)) {
           if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
-          const Unit& u = ms.units[t.uslot];
           const int nr = u.nrows;
           const uint8_t* src = p.q + (nr ? u.qrow : 0) * (D * 2) + lane * 16;
-#pragma unroll 2
-          for (int i = 0; i < MR / kLoadWarps; ++i) {
-            const int r = lw * (MR / kLoadWarps) + i;
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const int r = lw * 16 + i;
             const uint32_t dst = q_base + r * 128 + (((lane & 7) ^ (r & 7)) << 4) + (lane >> 3) * QSLAB;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              cp16(dst + h * 4 * QSLAB, src + (r < nr ? (int64_t)r * (D * 2) + h * 512 : 0), r < nr ? 16u : 0u);
+            const uint8_t* from = src + (r < nr ? r * (D * 2) : 0);
+            cp16(dst, from, r < nr ? 16u : 0u);
+            cp16(dst + 4 * QSLAB, from + 512, r < nr ? 16u : 0u);
           }
           cp_arrive(&bars[B_QFULL]);
           ++q;
         }
-        if (!__all_sync(0xffffffffu, WAIT(B_KEMPTY, n ^ 1u, 34))) break;
-        // The rows' mask. Its place was tile n - 3's, which is done with: the
-        // scores of n - 1, after which K came free, were issued after its product.
-        const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
-        if (lane == 0) {
-          uint8_t* bytes = reinterpret_cast<uint8_t*>(ms.vmask[n % 3]);
-          bytes[side * 8 + lw] = (uint8_t)vm;
-          bytes[(side ^ 1) * 8 + lw] = (uint8_t)(vm >> 8);
-          sas::mbar_arrive(&bars[B_MASK + n % 3]);
+        if (is_v) {
+          // Tile n - 3's mask was here; it is done with: the product of n - 2 is,
+          // after which V of n - 1 was copied.
+          const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
+          if (lane == 0) {
+            ms.vmask[n % 3][lw] = vm;
+            sas::mbar_arrive(&bars[B_MASK + n % 3]);
+          }
         }
-        pool = p.kv[(t.flags & TF_CMP) ? 1 : 0];
-        const uint8_t* src = pool + lane * 16;
-        const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 8 * 128;
-#pragma unroll 4
-        for (int i = 0; i < 8; ++i) {  // all 64 rows: absent ones are zero, so that their scores are finite
-          const int ri = __shfl_sync(0xffffffffu, row, i);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            cp16(dst + h * 4 * KSLAB + i * 128 + (((lane & 7) ^ (i & 7)) << 4),
-                 src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
+        if (!__all_sync(0xffffffffu, WAIT(is_v ? B_VEMPTY : B_KEMPTY, n ^ 1u, is_v ? 23 : 34))) break;
+        const uint8_t* src = p.kv[f] + lane * 16 + (is_v ? side * 512 : 0);
+        if (is_v) {
+          // rows that the product's K steps take; the others stay as they are
+          const int cnt = min(32, max(16, (t.nrows + 15) & ~15) - lw * 32);
+          const uint32_t dst = v_base + (lane >> 3) * VSLAB + lw * 32 * 128;
+#pragma unroll 8
+          for (int i = 0; i < cnt; ++i) {
+            const int ri = __shfl_sync(0xffffffffu, row, i);
+            cp16(dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
+          }
+          cp_arrive(&bars[B_VFULL]);
+        } else {
+          const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 16 * 128;
+#pragma unroll 8
+          for (int i = 0; i < 16; ++i) {  // all of them: absent rows are zero, so that their scores are finite
+            const int ri = __shfl_sync(0xffffffffu, row, i);
+            const uint32_t d = dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4);
+            const uint8_t* from = src + (int64_t)max(ri, 0) * (D * 2);
+            cp16(d, from, ri >= 0 ? 16u : 0u);
+            cp16(d + 4 * KSLAB, from + 512, ri >= 0 ? 16u : 0u);
+          }
+          cp_arrive(&bars[B_KFULL]);
         }
-        cp_arrive(&bars[B_KFULL]);
-      }
-      if (v_due && !load_v(n - 1)) break;
-      v_due = rows;
-      if (t.flags & TF_END) break;
-      if (rows) {
-        v_row = row, v_top = top(t), v_pool = pool;
         ++n;
       }
       __syncwarp();
@@ -651,59 +640,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       ++c;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kMmaWarp) {
-    // ================================================= MMA issuer
-    // First CTA: scores of tile n, then the product of tile n - 1. Second CTA:
-    // tells the first, in the loaders' order, that its copies have landed.
+  } else if (warp == kQkWarp || warp == kPvWarp) {
+    // ================================================= MMA issuers
     if (elect_one()) {
       constexpr int fmt = DT == SAS_DTYPE_BF16 ? 1 : 0;
-      constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, UR, CH, 0, 0);
-      constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
-      const uint64_t q_desc = sas::umma_desc_sw128(q_base, 16, 1024), k_desc = sas::umma_desc_sw128(k_base, 16, 1024);
-      const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
-      uint32_t c = 0, n = 0, u = 0, vu = 0;
-      Tile last{};  // tile n - 1
-      bool due = false;  // its product is not issued yet
+      const bool pv = warp == kPvWarp;
       auto pass_on = [&](int bar, int to, uint32_t par) -> bool {
         if (!WAIT(bar, par, 26)) return false;
         sas::fence_proxy_async_smem();  // cp.async writes -> tensor core reads
         arrive_first(&bars[to]);
         return true;
       };
-      auto product = [&](uint32_t m) -> bool {
-        if (side) return pass_on(B_VFULL, B_XV, m);
-        if (!WAIT_PAIR(B_PREADY, m, 27) || !WAIT(B_VFULL, m, 35) || !WAIT_PAIR(B_XV, m, 36)) return false;
-        if ((last.flags & TF_FIRST) && !WAIT_PAIR(B_OEMPTY, vu ^ 1u, 28)) return false;
-        sas::fence_proxy_async_smem();
-        sas::tc_fence_after();
-        const int steps = max(1, (last.nrows + 15) / 16);
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-          for (int ks = 0; ks < steps; ++ks)
-            umma2(tmem + TM_O + 128 * h, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
-                  v_desc + ((2 * h * VSLAB + ks * 2048) >> 4), id_o, !((last.flags & TF_FIRST) && ks == 0));
-        commit2(&bars[B_VEMPTY]);
-        if (last.flags & TF_LAST) {
-          commit2(&bars[B_OFULL]);
-          ++vu;
-        }
-        return true;
-      };
+      uint32_t c = 0, n = 0, u = 0;
       while (true) {
         if (!WAIT(B_CFULL + c % kRing, c / kRing, 24)) break;
         const Tile t = ms.ring[c % kRing];
-        const bool rows = !(t.flags & (TF_END | TF_ZERO));
-        if (rows) {
+        if (t.flags & TF_END) break;
+        if (!(t.flags & TF_ZERO)) {
           if (side) {
-            if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
-            if (!pass_on(B_KFULL, B_XK, n)) break;
-          } else {
+            if (pv) {
+              if (!pass_on(B_VFULL, B_XV, n)) break;
+            } else {
+              if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
+              if (!pass_on(B_KFULL, B_XK, n)) break;
+            }
+          } else if (pv) {  // O += P V
+            constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
+            const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
+            if (!WAIT(B_VFULL, n, 35) || !WAIT_PAIR(B_XV, n, 36) || !WAIT_PAIR(B_PREADY, n, 27)) break;
+            if ((t.flags & TF_FIRST) && !WAIT_PAIR(B_OEMPTY, u ^ 1u, 28)) break;
+            sas::fence_proxy_async_smem();
+            sas::tc_fence_after();
+            const int steps = max(1, (t.nrows + 15) / 16);
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+              for (int ks = 0; ks < steps; ++ks)
+                umma2(tmem + TM_O + 128 * h, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
+                      v_desc + ((2 * h * VSLAB + ks * 2048) >> 4), id_o, !((t.flags & TF_FIRST) && ks == 0));
+            commit2(&bars[B_VEMPTY]);
+            if (t.flags & TF_LAST) {
+              commit2(&bars[B_OFULL]);
+              ++u;
+            }
+          } else {  // S = Q K^T
+            constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, UR, CH, 0, 0);
+            const uint64_t q_desc = sas::umma_desc_sw128(q_base, 16, 1024), k_desc = sas::umma_desc_sw128(k_base, 16, 1024);
             if (t.flags & TF_FIRST) {
               if (!WAIT(B_QFULL, u, 25) || !WAIT_PAIR(B_XQ, u, 37)) break;
               ++u;
             }
-            if (!WAIT(B_KFULL, n, 26) || !WAIT_PAIR(B_XK, n, 38)) break;
+            if (!WAIT(B_KFULL, n, 26) || !WAIT_PAIR(B_XK, n, 38) || !WAIT_PAIR(B_SEMPTY + (n & 1), (n >> 1) ^ 1u, 41)) break;
             sas::fence_proxy_async_smem();
             sas::tc_fence_after();
 #pragma unroll 1
@@ -716,14 +703,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             commit2(&bars[B_KEMPTY]);
             if (t.flags & TF_LAST) commit2(&bars[B_QEMPTY]);
           }
-        }
-        // Also where no tile with rows follows: the softmax warps wait for the
-        // product of a unit's end before they release the ring's next entries.
-        if (due && !product(n - 1)) break;
-        due = rows;
-        if (t.flags & TF_END) break;
-        if (rows) {
-          last = t;
           ++n;
         }
         sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
@@ -731,30 +710,108 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       }
       // nothing may still run on TMEM or shared memory when the pair leaves
       if (!side) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sas::smem_u32(&bars[B_DRAIN])) : "memory");
-        sas::mbar_wait_drain(&bars[B_DRAIN], 0, SAS_WAIT_LIMIT_NS);
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sas::smem_u32(&bars[B_DRAIN + pv])) : "memory");
+        sas::mbar_wait_drain(&bars[B_DRAIN + pv], 0, SAS_WAIT_LIMIT_NS);
       }
     }
     __syncwarp();
-  } else {
-    // ================================================= softmax, epilogue
+  } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
+    // ================================================= epilogue
+    // Warp w has TMEM lanes [32 w, + 32): 32 rows, 256 of their columns.
+    const int ew = warp - kEpiWarp0, row = (ew & 1) * 32 + lane, ch = ew >> 1;
+    const uint32_t tl = tmem + ((uint32_t)ew << 21), box = sas::smem_u32(ms.box[ew]);
+    for (uint32_t u = 0;; ++u) {
+      if (!__all_sync(0xffffffffu, WAIT(B_FIN + (u & 1), u >> 1, 30))) break;
+      const Fin& fin = ms.fin[u & 1];
+      const int nrows = fin.nrows, part = fin.part;
+      if (nrows < 0) break;  // the range is done
+      const int64_t qrow = fin.qrow;
+      const float m = fin.m[row], l0 = fin.l[0][row];
+      const float l = (l0 + fin.l[1][row]) + (fin.l[2][row] + fin.l[3][row]);
+      const bool used = !(l0 < 0.f);
+      float* const o = p.part + ((size_t)blockIdx.x * 2 + max(part, 0)) * kPieceFloats;
+      float k = 0.f;
+      if (part >= 0) {
+        if (ch == 0) {
+          o[MR * D + row] = m;
+          o[MR * D + MR + row] = used ? l : -1.f;  // -1: the token is not in use
+        }
+      } else {
+        const float sink = __ldg(p.sinks + (fin.roff + row) % p.H) * kLog2e;
+        const float top = fmaxf(m, sink);
+        const float a = m == -INFINITY ? 0.f : exp2f(m - top);
+        const float den = l * a + (sink == -INFINITY ? 0.f : exp2f(sink - top));
+        k = !used || (m == -INFINITY && l == 0.f) ? 0.f : a / den;
+        if (row < nrows && ch == 0 && p.lse) p.lse[qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
+      }
+      if (!__all_sync(0xffffffffu, WAIT(B_OFULL, u, 33))) break;
+      sas::tc_fence_after();
+      const int nr = min(32, nrows - (ew & 1) * 32);
+      uint8_t* out = p.out + (qrow + (ew & 1) * 32) * (D * 2) + ch * 512 + (lane & 3) * 16;
+      const uint64_t k2 = twice(k);
+#pragma unroll 1
+      for (int x = 0; x < 8; ++x) {
+        uint32_t r[32];
+        __syncwarp();
+        sas::tmem_ld32(tl + TM_O + 32 * x, r);
+        sas::tmem_wait_ld();
+        if (x == 7) {  // O is read
+          sas::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first(&bars[B_OEMPTY]);
+        }
+        if (part >= 0) {  // [D / 4][64 rows] of float4: a warp's stores are contiguous
+          uint4* d4 = reinterpret_cast<uint4*>(o) + (size_t)(ch * 64 + x * 8) * MR + row;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d4[i * MR] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        } else {
+          // through shared memory, so that a store writes whole sectors of 8 rows
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t y = mul2(pair(r[8 * i + 2 * e], r[8 * i + 2 * e + 1]), k2);
+              v[e] = k == 0.f ? 0u : pack2<DT>(lo(y), hi(y));
+            }
+            st_shared16(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4), v[0], v[1], v[2], v[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = 8 * i + (lane >> 2);
+            uint4 q4;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(q4.x), "=r"(q4.y), "=r"(q4.z), "=r"(q4.w)
+                         : "r"(box + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4)));
+            if (rr < nr) *reinterpret_cast<uint4*>(out + (int64_t)rr * (D * 2) + x * 64) = q4;
+          }
+        }
+      }
+    }
+  } else if (warp < kSmWarps) {
+    // ================================================= softmax
     // Warps w and w + 4 share TMEM lanes: thread = row, columns [32 part, + 32)
-    // of a tile's 128, and 128 of the row's output columns.
+    // of a tile's 128.
     const int row = (warp & 1) * 32 + lane, ch = (warp >> 1) & 1, gr = warp >> 2, part = 2 * ch + gr;
     const uint32_t tl = tmem + ((uint32_t)(warp & 3) << 21);
-    float* const red_row = &ms.red[0][row];
-    constexpr int RED = 32 * kSmWarps;
     const bool flip = p.scale_log2 < 0.f;
     const float scale = flip ? -p.scale_log2 : p.scale_log2;
     uint32_t c = 0, n = 0, u = 0, sy = 0;
     float m = -INFINITY, l = 0.f;
     int tok = 0;
     bool used = false, ok = true;
-    float sink = 0.f;
     while (ok) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 29))) break;
       const Tile t = ms.ring[c % kRing];
-      if (t.flags & TF_END) break;
+      if (t.flags & TF_END) {
+        // the epilogue ends too; its place is free as below
+        if (n > 0 && !__all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40))) break;
+        ms.fin[u & 1].nrows = -1;
+        __syncwarp();
+        if (lane == 0) sas::mbar_arrive(&bars[B_FIN + (u & 1)]);
+        break;
+      }
       const Unit& un = ms.units[t.uslot];
       if (t.flags & TF_ZERO) {
         uint4* o = reinterpret_cast<uint4*>(p.out + un.qrow * (D * 2));
@@ -766,7 +823,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           l = 0.f;
           tok = p.scenario == 3 ? 0 : min((un.roff + row) / p.H, kMaxTok - 1);
           used = row < un.nrows && un.pos[tok] >= 0;
-          sink = __ldg(p.sinks + (un.roff + row) % p.H) * kLog2e;
         }
         uint32_t see = used ? ms.vis[c % kRing][tok][part] : 0u;
         // rows of the tile that are there, and those that this row's token sees
@@ -783,6 +839,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           uint32_t r[32];
           sas::tmem_ld32(tl + TM_S + 64 * (n & 1) + 32 * gr, r);
           sas::tmem_wait_ld();
+          sas::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first(&bars[B_SEMPTY + (n & 1)]);
           if (flip)
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] ^= 0x80000000u;
@@ -821,8 +880,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = max3(mx, lo(s[i]), hi(s[i]));
-        float* const red = red_row + (n & 1) * RED;
-        red[part * 64] = mx;
+        float(*const red)[MR] = ms.red[n & 1];
+        red[part][row] = mx;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
         // P with the reference as it stands, while the row's other maxima come;
@@ -851,7 +910,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
             if (!ok) break;
             ++sy;
-            mx = fmaxf(fmaxf(red[0], red[64]), fmaxf(red[128], red[192])) * scale;
+            mx = fmaxf(fmaxf(red[0][row], red[1][row]), fmaxf(red[2][row], red[3][row])) * scale;
             if (mx > m + kMove || (m == -INFINITY && mx > m)) {
               fac = sas::ex2(m - mx);
               m = mx;
@@ -889,79 +948,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (lane == 0) arrive_first(&bars[B_PREADY]);
         ++n;
         if (t.flags & TF_LAST) {
-          float* const rl = red_row + 2 * RED;
-          rl[part * 64] = l;
-          __syncwarp();
-          if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
-          ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
-          if (!ok) break;
-          ++sy;
-          const float lt = (rl[0] + rl[64]) + (rl[128] + rl[192]);
-          ok = __all_sync(0xffffffffu, WAIT(B_OFULL, u, 33));
-          if (!ok) break;
-          ++u;
-          sas::tc_fence_after();
-          const int col0 = ch * 256 + gr * 128;  // this thread's output columns
-          if (t.flags & (TF_PART0 | TF_PART1)) {
-            // [D / 4][64 rows] of float4: a warp's stores are contiguous
-            float* o = p.part + ((size_t)blockIdx.x * 2 + ((t.flags & TF_PART1) ? 1 : 0)) * kPieceFloats;
-            if (part == 0) {
-              o[MR * D + row] = m;
-              o[MR * D + MR + row] = used ? lt : -1.f;  // -1: the token is not in use
-            }
-#pragma unroll 1
-            for (int x = 0; x < 4; ++x) {
-              uint32_t r[32];
-              __syncwarp();
-              sas::tmem_ld32(tl + TM_O + 128 * gr + 32 * x, r);
-              sas::tmem_wait_ld();
-              uint4* d4 = reinterpret_cast<uint4*>(o) + (size_t)((col0 + 32 * x) / 4) * MR + row;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) d4[i * MR] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-            }
-          } else {
-            const float top = fmaxf(m, sink);
-            const float a = m == -INFINITY ? 0.f : exp2f(m - top);
-            const float den = lt * a + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-            const float k = !used || (m == -INFINITY && lt == 0.f) ? 0.f : a / den;
-            const bool zero = k == 0.f;
-            if (row < un.nrows && part == 0 && p.lse) p.lse[un.qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
-            // 32 columns at a time through this warp's 2 KB of P, which is free
-            // now, so that a store instruction writes whole sectors of 8 rows
-            const uint32_t box = p_base + warp * 2048;
-            const int nr = min(32, un.nrows - (warp & 1) * 32);
-            uint8_t* out = p.out + (un.qrow + (warp & 1) * 32) * (D * 2) + col0 * 2 + (lane & 3) * 16;
-            const uint64_t k2 = twice(k);
-#pragma unroll 1
-            for (int x = 0; x < 4; ++x) {
-              uint32_t r[32];
-              __syncwarp();
-              sas::tmem_ld32(tl + TM_O + 128 * gr + 32 * x, r);
-              sas::tmem_wait_ld();
-              uint32_t v[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const uint64_t y = mul2(pair(r[2 * i], r[2 * i + 1]), k2);
-                v[i] = zero ? 0u : pack2<DT>(lo(y), hi(y));
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                st_shared16(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4), v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-              __syncwarp();
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int rr = 8 * i + (lane >> 2);
-                uint4 q4;
-                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(q4.x), "=r"(q4.y), "=r"(q4.z), "=r"(q4.w)
-                             : "r"(box + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4)));
-                if (rr < nr) *reinterpret_cast<uint4*>(out + (int64_t)rr * (D * 2) + x * 64) = q4;
-              }
-            }
+          // The place was unit u - 2's: its O was read, after these, before the
+          // first product of unit u - 1, and that is complete.
+          Fin& fin = ms.fin[u & 1];
+          fin.l[part][row] = used ? l : -1.f;
+          if (part == 0) fin.m[row] = m;
+          if (tid == 0) {
+            fin.qrow = un.qrow, fin.nrows = un.nrows, fin.roff = un.roff;
+            fin.part = t.flags & TF_PART1 ? 1 : t.flags & TF_PART0 ? 0 : -1;
           }
-          sas::tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_first(&bars[B_OEMPTY]);
+          if (lane == 0) sas::mbar_arrive(&bars[B_FIN + (u & 1)]);
+          ++u;
         }
       }
       __syncwarp();
@@ -972,7 +970,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   sas::tc_fence_before();
   __syncthreads();
   cluster_sync();  // the other CTA no longer reads this one's shared memory or arrives on it
-  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+  if (warp == kQkWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
 #undef WAIT
 #undef WAIT_PAIR
 }
