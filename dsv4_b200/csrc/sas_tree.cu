@@ -38,7 +38,16 @@
 //          that this one's K and Q, or V, have landed (second CTA);
 //   14     coordinator: walks the range and the trees, works out which rows each
 //          token sees and publishes tiles (the pair's two take the same steps);
-//   15-18  copy Q and K, 19-22 V (cp.async, one row's 512 bytes at a time).
+//   15-18  copy Q and K, 19-22 V.
+// Copies: Q, and the rows of pages of a multiple of 64, are TMA boxes of 64 rows
+// x 64 columns issued by one thread (window tiles then begin at a multiple of 64,
+// so that 64 rows never leave a page). Top-k rows and other pages take cp.async,
+// one row's 512 bytes per instruction, whose 256 instructions a tile hold up
+// every other warp's shared-memory accesses.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "sas_common.cuh"
 
 namespace {
@@ -72,9 +81,11 @@ constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
 
 // X* count in the first CTA: the second's copies have landed. So do SEMPTY (the
 // scores are read), PREADY and OEMPTY, on which both CTAs' warps arrive.
-enum Bar { B_KFULL = 0, B_VFULL, B_QFULL, B_XK, B_XV, B_XQ, B_KEMPTY, B_VEMPTY, B_QEMPTY, B_MASK, B_SFULL = B_MASK + 3,
-           B_SEMPTY = B_SFULL + 2, B_PREADY = B_SEMPTY + 2, B_OFULL, B_OEMPTY, B_FIN, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2,
-           B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
+// K and V come in two halves of their columns, each with its own barriers, so
+// that the next tile's first half is on its way while the second is multiplied.
+enum Bar { B_KFULL = 0, B_VFULL = 2, B_QFULL = 4, B_XK, B_XV = B_XK + 2, B_XQ = B_XV + 2, B_KEMPTY, B_VEMPTY = B_KEMPTY + 2,
+           B_QEMPTY = B_VEMPTY + 2, B_MASK, B_SFULL = B_MASK + 3, B_SEMPTY = B_SFULL + 2, B_PREADY = B_SEMPTY + 2, B_OFULL, B_OEMPTY,
+           B_FIN, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
 
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
@@ -131,6 +142,7 @@ struct TreeParams {
   const uint8_t* kv[2];  // window pool, compressed pool
   const int32_t* bt[2];
   int bs[2], bt_stride[2];
+  int tma[2];            // pages of the pool are copied in boxes of 64 rows
   int64_t nblk[2];
   const int32_t* idx;
   const float* sinks;
@@ -139,11 +151,12 @@ struct TreeParams {
   Cut* cuts;    // [CTAs]
   int64_t* total;
   int32_t* status;
+  CUtensorMap map_kv[2], map_q;
 };
 
 // What a request brings: its tokens, and the tiles of each of its units.
 struct Req {
-  int base, slots, n, ctx, thr, units, wtiles, tiles;
+  int base, slots, n, ctx, thr, lo, units, wtiles, tiles;  // lo: the window tiles' first row
   bool bad;
   __device__ __forceinline__ int64_t all() const { return (int64_t)units * tiles; }
 };
@@ -162,11 +175,16 @@ __device__ __noinline__ Req request(const TreeParams& p, int b) {
   r.bad = r.n > kMaxTree || r.ctx < 0 || r.ctx > kMaxCtx;
   r.thr = p.scenario == 1 || r.bad ? 0 : r.ctx / p.ratio;
   r.units = p.scenario == 3 ? r.slots : (int)(((int64_t)r.slots * p.H + UR - 1) / UR);
-  r.wtiles = r.bad || r.n == 0 ? 1 : (min(r.ctx, p.win) + r.n + CH - 1) / CH;
+  r.lo = max(r.ctx - p.win, 0);
+  if (p.tma[0]) r.lo &= ~63;
+  r.wtiles = r.bad || r.n == 0 ? 1 : (r.ctx - r.lo + r.n + CH - 1) / CH;
   r.tiles = r.wtiles + (r.bad || r.n == 0 ? 0 : p.scenario == 2 ? (r.thr + CH - 1) / CH : p.scenario == 3 && r.thr > 0 ? (p.K + CH - 1) / CH : 0);
   return r;
 }
-__device__ __forceinline__ int64_t range_start(int64_t total, int R, int r) { return total * r / R; }
+__device__ __forceinline__ int64_t range_start(int64_t total, int R, int r) {
+  if (total < (1 << 20)) return (uint32_t)total * (uint32_t)r / (uint32_t)R;  // R <= 2048 here; 64-bit division is slow
+  return total * r / R;
+}
 // CTAs (per head group) that share the sequence; every range has a tile
 __device__ __forceinline__ int ranges(int64_t total, int R) { return (int)max((int64_t)1, min((int64_t)R, total)); }
 
@@ -175,6 +193,25 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t byt
 }
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sas::smem_u32(bar)) : "memory");
+}
+}  // namespace
+namespace sas {
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+}  // namespace sas
+namespace {
+__device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sas::smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const void* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sas::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 // D[tmem of both CTAs] (+)= A B^T over the pair
 __device__ __forceinline__ void umma2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -308,13 +345,13 @@ __device__ __noinline__ uint32_t window_bits(int p0, int s, int win, int ctx, co
   return m;
 }
 
-// Zeroes the half rows [row0, row0 + 32) of a tile's V, of those in `there`,
-// that hold infinities or NaN.
+// Zeroes the half rows [row0, row0 + 32) of a tile's V that hold infinities or NaN.
 template <int DT>
-__device__ __noinline__ void clear_rows(uint32_t v_base, uint32_t there, int row0) {
+__device__ __noinline__ void clear_rows(uint32_t v_base, int row0) {
   constexpr uint32_t ex = DT == SAS_DTYPE_BF16 ? 0x7f80u : 0x7c00u;  // the exponent's bits
-  for (; there; there &= there - 1) {
-    const uint32_t at = v_base + (row0 + __ffs(there) - 1) * 128;
+#pragma unroll 1
+  for (int r = row0; r < row0 + 32; ++r) {
+    const uint32_t at = v_base + r * 128;
     uint32_t hot = 0;
 #pragma unroll 1
     for (int e = 0; e < 32; ++e) {  // 16-byte pieces
@@ -341,8 +378,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     auto init = [&](int bar, int n, int count) {
       for (int i = 0; i < n; ++i) sas::mbar_init(&bars[bar + i], count);
     };
-    init(B_KFULL, 3, 32 * kLoadWarps);  // and V, Q
-    init(B_XK, 6, 1);                   // XK, XV, XQ, KEMPTY, VEMPTY, QEMPTY
+    init(B_KFULL, 4, 32 * kLoadWarps);  // and VFULL
+    init(B_QFULL, 11, 1);               // QFULL, XK, XV, XQ, KEMPTY, VEMPTY, QEMPTY
     init(B_MASK, 3, kLoadWarps);
     init(B_SFULL, 2, 1);
     init(B_SEMPTY, 3, 2 * kSmWarps);    // and PREADY: softmax warps of both CTAs
@@ -391,21 +428,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   {
     int64_t at = before + incl - mine;
     for (int b = b0; b < b1; ++b) {
-      const int64_t a = request(p, b).all();
+      const int64_t a = per == 1 ? mine : request(p, b).all();
       if (t0 >= at && t0 < at + a) ms.start_b = b, ms.start_prefix = at;
       at += a;
-    }
-  }
-  if (p.layout == SAS_LAYOUT_TND) {  // rows that no request holds are zero
-    const int64_t lo = (int64_t)min(max(__ldg(p.cu), 0), p.T) * p.H, hi = (int64_t)min(max(__ldg(p.cu + p.B), 0), p.T) * p.H;
-    const int64_t all = (int64_t)p.T * p.H;
-    for (int64_t r = blockIdx.x; r < all; r += gridDim.x) {
-      if (r >= lo && r < hi) {  // jump over the held rows, staying on this CTA's share
-        r += (hi - r + gridDim.x - 1) / gridDim.x * gridDim.x - gridDim.x;
-        continue;
-      }
-      if (tid < 64) reinterpret_cast<uint4*>(p.out + r * D * 2)[tid] = make_uint4(0, 0, 0, 0);
-      if (tid == 64 && p.lse) p.lse[r] = 0.f;
     }
   }
   if (blockIdx.x == 0 && tid == 0) *p.total = total;
@@ -453,7 +478,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         ++b;
         continue;
       }
-      const int u = (int)((t - prefix) / r.tiles);
+      const int64_t in = t - prefix;
+      const int u = in < (1ll << 31) ? (int)((uint32_t)in / (uint32_t)r.tiles) : (int)(in / r.tiles);
       const int64_t ustart = prefix + (int64_t)u * r.tiles, uend = ustart + r.tiles;
       int k0 = (int)(t - ustart), k1 = (int)min((int64_t)r.tiles, t1 - ustart);
       if (!p.split) {  // a unit belongs to the range that its first tile is in
@@ -478,12 +504,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const int us = uc % kUnitSlots;
       Unit& un = ms.units[us];
       // the unit's rows among the request's, and this CTA's half of them
-      const int64_t first = p.scenario == 3 ? (int64_t)u * p.H + g * UR : (int64_t)u * UR;
-      const int64_t end = p.scenario == 3 ? min(first + UR, (int64_t)(u + 1) * p.H) : min(first + UR, (int64_t)r.slots * p.H);
-      const int64_t row_in = first + side * MR;
-      const int nrows = (int)max((int64_t)0, min((int64_t)MR, end - row_in));
-      const int i0 = (int)(first / p.H), i1 = (int)((end - 1) / p.H);
-      const int mine = nrows ? (int)(row_in / p.H) - i0 : 0;  // this CTA's first token among the unit's
+      const uint32_t H = p.H, first = p.scenario == 3 ? u * H + g * UR : (uint32_t)u * UR;  // T * H < 2^31
+      const uint32_t end = p.scenario == 3 ? min(first + UR, (u + 1) * H) : min(first + UR, (uint32_t)r.slots * H);
+      const uint32_t row_in = first + side * MR;
+      const int nrows = end > row_in ? (int)min((uint32_t)MR, end - row_in) : 0;
+      const int i0 = (int)(first / H), i1 = (int)((end - 1) / H);
+      const int mine = nrows ? (int)(row_in / H) - i0 : 0;  // this CTA's first token among the unit's
       // the slot's last readers are done: see kUnitSlots; the ring wait below
       // orders this warp's writes after their reads
       if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + c % kRing, (c / kRing) ^ 1u, 20))) break;
@@ -522,7 +548,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         un.thr = r.thr;
         un.qrow = (int64_t)r.base * p.H + row_in;
         un.nrows = nrows;
-        un.roff = (int)(row_in % p.H);
+        un.roff = (int)(row_in % H);
       }
       __syncwarp();
       const bool any = __any_sync(0xffffffffu, pos >= 0);
@@ -539,12 +565,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       } else {
         ++uc;
         const int part = whole ? 0 : (t == t0 ? TF_PART0 : TF_PART1);
-        const int lo = max(r.ctx - p.win, 0);
-        const int wrows = r.ctx - lo + min(i1, r.n - 1) + 1;  // up to the unit's last drafted token
+        const int wrows = r.ctx - r.lo + min(i1, r.n - 1) + 1;  // up to the unit's last drafted token
         for (int k = k0; k < k1 && ok; ++k) {
           int fl = part | (k == k0 ? TF_FIRST : 0) | (k == k1 - 1 ? TF_LAST : 0), row0, n;
           if (k < r.wtiles) {
-            row0 = lo + k * CH;
+            row0 = r.lo + k * CH;
             n = min(CH, wrows - k * CH);
           } else {
             row0 = (k - r.wtiles) * CH;
@@ -560,13 +585,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     if (ok) publish(TF_END, 0, 0, 0);
   } else if (warp >= kKWarp0) {
     // ================================================= loaders
-    // Warps of K: 16 of this CTA's 64 K rows of a tile each, and 16 rows of Q.
-    // Warps of V: 32 of the tile's 128 rows each, this CTA's 256 columns; they
-    // also tell which rows are there.
+    // By cp.async, warps of K: 16 of this CTA's 64 K rows of a tile each; warps of
+    // V: 32 of the tile's 128 rows each, this CTA's 256 columns. By TMA, lane 0 of
+    // the first warp does it all. The warps of K also tell which rows are there.
     const bool is_v = warp >= kVWarp0;
     const int lw = (warp - kKWarp0) & 3;
-    const int my_row = is_v ? lw * 32 + lane : side * 64 + lw * 16 + (lane & 15);
+    // K: lanes 0-15 have the warp's K rows, 16-31 the same of the other CTA's half (for the mask)
+    const int my_row = is_v ? lw * 32 + lane : (lane < 16 ? side : side ^ 1) * 64 + lw * 16 + (lane & 15);
+    const int full = is_v ? B_VFULL : B_KFULL, empty = is_v ? B_VEMPTY : B_KEMPTY;
     uint32_t c = 0, n = 0, q = 0;
+    // pool row of position pos of a request's table, -1: none
+    auto lookup = [&](int f, int b, int pos) -> int {
+      const int col = pos / p.bs[f];
+      const int blk = col < p.bt_stride[f] ? __ldg(p.bt[f] + (int64_t)b * p.bt_stride[f] + col) : 0x7fffffff;
+      if (blk >= p.nblk[f]) bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
+      return blk < 0 || blk >= p.nblk[f] ? -1 : blk * p.bs[f] + (pos - col * p.bs[f]);
+    };
     while (true) {
       if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
       const Tile t = ms.ring[c % kRing];
@@ -574,72 +608,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       if (!(t.flags & TF_ZERO)) {
         const Unit& u = ms.units[t.uslot];
         const int f = (t.flags & TF_CMP) ? 1 : 0;
-        int row = -1;  // pool row of tile row my_row, -1: none
-        if (my_row < t.nrows) {
+        const bool tma = p.tma[f] && !(t.flags & TF_TOPK);
+        int row = -1;  // pool row of tile row my_row, -1: none (TMA: of the first of lane's 64 rows)
+        if (tma) {
+          if (lane < 2 && 64 * lane < t.nrows) row = lookup(f, u.b, t.row0 + 64 * lane);
+        } else if (my_row < t.nrows) {
           int pos = t.row0 + my_row;
           if (t.flags & TF_TOPK) pos = __ldg(p.idx + (int64_t)u.tok * p.K + pos);
-          if (!(t.flags & TF_TOPK) || (pos >= 0 && pos < u.thr)) {
-            const int col = pos / p.bs[f];
-            const int blk = col < p.bt_stride[f] ? __ldg(p.bt[f] + (int64_t)u.b * p.bt_stride[f] + col) : 0x7fffffff;
-            if (blk >= p.nblk[f]) bad(p, SAS_ERR_BAD_BLOCK_ENTRY);
-            else if (blk >= 0) row = blk * p.bs[f] + (pos - col * p.bs[f]);
-          }
+          if (!(t.flags & TF_TOPK) || (pos >= 0 && pos < u.thr)) row = lookup(f, u.b, pos);
         }
-        if (!is_v && (t.flags & TF_FIRST)) {
+        if (!is_v && lw == 0 && (t.flags & TF_FIRST)) {
           if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
-          const int nr = u.nrows;
-          const uint8_t* src = p.q + (nr ? u.qrow : 0) * (D * 2) + lane * 16;
-#pragma unroll 4
-          for (int i = 0; i < 16; ++i) {
-            const int r = lw * 16 + i;
-            const uint32_t dst = q_base + r * 128 + (((lane & 7) ^ (r & 7)) << 4) + (lane >> 3) * QSLAB;
-            const uint8_t* from = src + (r < nr ? r * (D * 2) : 0);
-            cp16(dst, from, r < nr ? 16u : 0u);
-            cp16(dst + 4 * QSLAB, from + 512, r < nr ? 16u : 0u);
+          const int q0 = (int)u.qrow;
+          if (elect_one()) {  // rows past the unit's are other rows, or zero past the last: nobody reads their results
+            sas::mbar_arrive_expect_tx(&bars[B_QFULL], 8 * QSLAB);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) tma_2d(q_base + i * QSLAB, &p.map_q, &bars[B_QFULL], i * 64, q0);
           }
-          cp_arrive(&bars[B_QFULL]);
+          __syncwarp();
           ++q;
         }
-        if (is_v) {
-          // Tile n - 3's mask was here; it is done with: the product of n - 2 is,
-          // after which V of n - 1 was copied.
-          const uint32_t vm = __ballot_sync(0xffffffffu, row >= 0);
-          if (lane == 0) {
-            ms.vmask[n % 3][lw] = vm;
+        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+        // TMA: page and row of the two halves; one without a page is read past the
+        // last block, where TMA gives zeros
+        const int pg = row < 0 ? (int)p.nblk[f] : row / p.bs[f], at = row < 0 ? 0 : row - pg * p.bs[f];
+        const int b0 = __shfl_sync(0xffffffffu, pg, 0), b1 = __shfl_sync(0xffffffffu, pg, 1);
+        const int a0 = __shfl_sync(0xffffffffu, at, 0), a1 = __shfl_sync(0xffffffffu, at, 1);
+        const CUtensorMap* map = &p.map_kv[f];
+        const uint8_t* src = p.kv[f] + lane * 16 + (is_v ? side * 512 : 0);
+        // V rows that the product's K steps take; the others stay as they are
+        const int cnt = is_v ? min(32, max(16, (t.nrows + 15) & ~15) - lw * 32) : 16;
+        bool ok = true;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          ok = __all_sync(0xffffffffu, WAIT(empty + h, n ^ 1u, is_v ? 23 : 34));
+          if (!ok) break;
+          if (tma) {
+            if (lw == 0 && elect_one()) {
+              sas::mbar_expect_tx(&bars[full + h], 4 * KSLAB);
+              if (is_v) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t dst = v_base + (2 * h + i) * VSLAB;
+                  tma_3d(dst, map, &bars[B_VFULL + h], side * 256 + (2 * h + i) * 64, a0, b0);
+                  tma_3d(dst + 8192, map, &bars[B_VFULL + h], side * 256 + (2 * h + i) * 64, a1, b1);
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  tma_3d(k_base + (4 * h + i) * KSLAB, map, &bars[B_KFULL + h], (4 * h + i) * 64, side ? a1 : a0, side ? b1 : b0);
+              }
+            }
+            __syncwarp();
+            sas::mbar_arrive(&bars[full + h]);
+          } else if (is_v) {  // 256 bytes of two rows at a time
+            const uint32_t dst = v_base + (2 * h + ((lane >> 3) & 1)) * VSLAB + lw * 32 * 128;
+#pragma unroll 8
+            for (int i = 0; i < cnt; i += 2) {
+              const int ii = i + (lane >> 4), ri = __shfl_sync(0xffffffffu, row, ii);
+              cp16(dst + ii * 128 + (((lane & 7) ^ (ii & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2) + h * 256 - (lane >> 4) * 256, ri >= 0 ? 16u : 0u);
+            }
+            cp_arrive(&bars[full + h]);
+          } else {
+            const uint32_t dst = k_base + (4 * h + (lane >> 3)) * KSLAB + lw * 16 * 128;
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {  // all of them: absent rows are zero, so that their scores are finite
+              const int ri = __shfl_sync(0xffffffffu, row, i);
+              cp16(dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2) + h * 512, ri >= 0 ? 16u : 0u);
+            }
+            cp_arrive(&bars[full + h]);
+          }
+          if (!is_v && h == 0 && lane == 0) {
+            // Tile n - 3's mask was here. It is done with: K came free after the
+            // scores of n - 1, for which those of n - 3 had been read, after it.
+            if (tma) {
+              ms.vmask[n % 3][lw] = (there >> (lw >> 1)) & 1u ? low_bits(t.nrows - 32 * lw) : 0u;
+            } else {
+              uint16_t* part = reinterpret_cast<uint16_t*>(ms.vmask[n % 3]);
+              part[side * 4 + lw] = (uint16_t)there;
+              part[(side ^ 1) * 4 + lw] = (uint16_t)(there >> 16);
+            }
             sas::mbar_arrive(&bars[B_MASK + n % 3]);
           }
         }
-        if (!__all_sync(0xffffffffu, WAIT(is_v ? B_VEMPTY : B_KEMPTY, n ^ 1u, is_v ? 23 : 34))) break;
-        const uint8_t* src = p.kv[f] + lane * 16 + (is_v ? side * 512 : 0);
-        if (is_v) {
-          // rows that the product's K steps take; the others stay as they are
-          const int cnt = min(32, max(16, (t.nrows + 15) & ~15) - lw * 32);
-          const uint32_t dst = v_base + (lane >> 3) * VSLAB + lw * 32 * 128;
-#pragma unroll 8
-          for (int i = 0; i < cnt; ++i) {
-            const int ri = __shfl_sync(0xffffffffu, row, i);
-            cp16(dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2), ri >= 0 ? 16u : 0u);
-          }
-          cp_arrive(&bars[B_VFULL]);
-        } else {
-          const uint32_t dst = k_base + (lane >> 3) * KSLAB + lw * 16 * 128;
-#pragma unroll 8
-          for (int i = 0; i < 16; ++i) {  // all of them: absent rows are zero, so that their scores are finite
-            const int ri = __shfl_sync(0xffffffffu, row, i);
-            const uint32_t d = dst + i * 128 + (((lane & 7) ^ (i & 7)) << 4);
-            const uint8_t* from = src + (int64_t)max(ri, 0) * (D * 2);
-            cp16(d, from, ri >= 0 ? 16u : 0u);
-            cp16(d + 4 * KSLAB, from + 512, ri >= 0 ? 16u : 0u);
-          }
-          cp_arrive(&bars[B_KFULL]);
-        }
+        if (!ok) break;
         ++n;
       }
       __syncwarp();
       if (lane == 0) sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
       ++c;
     }
+    // no copy may still be landing when the CTA leaves
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lw == 0) {
+      for (int h = 0; n > 0 && h < 2; ++h) sas::mbar_wait_drain(&bars[full + h], (n - 1) & 1, SAS_WAIT_LIMIT_NS);
+      if (!is_v && q > 0) sas::mbar_wait_drain(&bars[B_QFULL], (q - 1) & 1, SAS_WAIT_LIMIT_NS);
+    }
   } else if (warp == kQkWarp || warp == kPvWarp) {
     // ================================================= MMA issuers
     if (elect_one()) {
@@ -659,26 +723,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (!(t.flags & TF_ZERO)) {
           if (side) {
             if (pv) {
-              if (!pass_on(B_VFULL, B_XV, n)) break;
+              if (!pass_on(B_VFULL, B_XV, n) || !pass_on(B_VFULL + 1, B_XV + 1, n)) break;
             } else {
               if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
-              if (!pass_on(B_KFULL, B_XK, n)) break;
+              if (!pass_on(B_KFULL, B_XK, n) || !pass_on(B_KFULL + 1, B_XK + 1, n)) break;
             }
           } else if (pv) {  // O += P V
             constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
             const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
-            if (!WAIT(B_VFULL, n, 35) || !WAIT_PAIR(B_XV, n, 36) || !WAIT_PAIR(B_PREADY, n, 27)) break;
+            if (!WAIT_PAIR(B_PREADY, n, 27)) break;
             if ((t.flags & TF_FIRST) && !WAIT_PAIR(B_OEMPTY, u ^ 1u, 28)) break;
-            sas::fence_proxy_async_smem();
-            sas::tc_fence_after();
             const int steps = max(1, (t.nrows + 15) / 16);
+            bool ok = true;
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+              ok = WAIT(B_VFULL + h, n, 35) && WAIT_PAIR(B_XV + h, n, 36);
+              if (!ok) break;
+              sas::fence_proxy_async_smem();
+              sas::tc_fence_after();
 #pragma unroll 1
               for (int ks = 0; ks < steps; ++ks)
                 umma2(tmem + TM_O + 128 * h, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
                       v_desc + ((2 * h * VSLAB + ks * 2048) >> 4), id_o, !((t.flags & TF_FIRST) && ks == 0));
-            commit2(&bars[B_VEMPTY]);
+              commit2(&bars[B_VEMPTY + h]);
+            }
+            if (!ok) break;
             if (t.flags & TF_LAST) {
               commit2(&bars[B_OFULL]);
               ++u;
@@ -690,17 +759,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
               if (!WAIT(B_QFULL, u, 25) || !WAIT_PAIR(B_XQ, u, 37)) break;
               ++u;
             }
-            if (!WAIT(B_KFULL, n, 26) || !WAIT_PAIR(B_XK, n, 38) || !WAIT_PAIR(B_SEMPTY + (n & 1), (n >> 1) ^ 1u, 41)) break;
-            sas::fence_proxy_async_smem();
-            sas::tc_fence_after();
+            if (!WAIT_PAIR(B_SEMPTY + (n & 1), (n >> 1) ^ 1u, 41)) break;
+            bool ok = true;
 #pragma unroll 1
-            for (int s = 0; s < 8; ++s)
+            for (int h = 0; h < 2; ++h) {
+              ok = WAIT(B_KFULL + h, n, 26) && WAIT_PAIR(B_XK + h, n, 38);
+              if (!ok) break;
+              sas::fence_proxy_async_smem();
+              sas::tc_fence_after();
+#pragma unroll 1
+              for (int s = 4 * h; s < 4 * h + 4; ++s)
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                umma2(tmem + TM_S + 64 * (n & 1), q_desc + ((s * QSLAB + kk * 32) >> 4), k_desc + ((s * KSLAB + kk * 32) >> 4), id_s,
-                      (s | kk) != 0);
+                for (int kk = 0; kk < 4; ++kk)
+                  umma2(tmem + TM_S + 64 * (n & 1), q_desc + ((s * QSLAB + kk * 32) >> 4), k_desc + ((s * KSLAB + kk * 32) >> 4), id_s,
+                        (s | kk) != 0);
+              commit2(&bars[B_KEMPTY + h]);
+            }
+            if (!ok) break;
             commit2(&bars[B_SFULL + (n & 1)]);
-            commit2(&bars[B_KEMPTY]);
             if (t.flags & TF_LAST) commit2(&bars[B_QEMPTY]);
           }
           ++n;
@@ -720,6 +796,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     // Warp w has TMEM lanes [32 w, + 32): 32 rows, 256 of their columns.
     const int ew = warp - kEpiWarp0, row = (ew & 1) * 32 + lane, ch = ew >> 1;
     const uint32_t tl = tmem + ((uint32_t)ew << 21), box = sas::smem_u32(ms.box[ew]);
+    if (p.layout == SAS_LAYOUT_TND) {  // rows that no request holds are zero
+      const int et = tid - 32 * kEpiWarp0;
+      const int64_t lo = (int64_t)min(max(__ldg(p.cu), 0), p.T) * p.H, hi = (int64_t)min(max(__ldg(p.cu + p.B), 0), p.T) * p.H;
+      const int64_t all = (int64_t)p.T * p.H;
+      for (int64_t r = blockIdx.x; r < all; r += gridDim.x) {
+        if (r >= lo && r < hi) {  // jump over the held rows, staying on this CTA's share
+          if (hi == all) break;
+          r += (hi - r + gridDim.x - 1) / gridDim.x * gridDim.x - gridDim.x;
+          continue;
+        }
+        if (et < 64) reinterpret_cast<uint4*>(p.out + r * D * 2)[et] = make_uint4(0, 0, 0, 0);
+        if (et == 64 && p.lse) p.lse[r] = 0.f;
+      }
+    }
     for (uint32_t u = 0;; ++u) {
       if (!__all_sync(0xffffffffu, WAIT(B_FIN + (u & 1), u >> 1, 30))) break;
       const Fin& fin = ms.fin[u & 1];
@@ -806,7 +896,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const Tile t = ms.ring[c % kRing];
       if (t.flags & TF_END) {
         // the epilogue ends too; its place is free as below
-        if (n > 0 && !__all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40))) break;
+        if (n > 0 && !__all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, 40))) break;
         ms.fin[u & 1].nrows = -1;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_FIN + (u & 1)]);
@@ -828,7 +918,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         // rows of the tile that are there, and those that this row's token sees
         ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30));
         if (!ok) break;
-        const bool window = !(t.flags & TF_CMP);
+        // rows of the buffers that hold values that some row does not see: stale ones
+        // too, past the last of a page's
+        const bool check = !(t.flags & TF_CMP) || t.nrows < CH;
         const uint32_t there32 = ms.vmask[n % 3][part];
         see &= there32;
         ok = __all_sync(0xffffffffu, WAIT(B_SFULL + (n & 1), n >> 1, 31));
@@ -845,9 +937,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           if (flip)
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] ^= 0x80000000u;
-          if (window || !__all_sync(0xffffffffu, see == 0xffffffffu)) {
-            if (window) {
-              // In the window a row may be seen by some tokens only, and one with
+          if (check || !__all_sync(0xffffffffu, see == 0xffffffffu)) {
+            if (check) {
+              // A row may be seen by some tokens only, or by none, and one with
               // infinities or NaN would reach the others' sums as 0 * NaN. All
               // rows' scores with it are not finite, in both CTAs, which their
               // sum shows; each CTA then clears what it holds of such a row's V.
@@ -862,8 +954,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
               // The tile's V has to be there, after the one before it was done
               // with (its copy alone could be two phases back). A wait that fails
               // shows at the next one.
-              if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY, n ^ 1u, 40) && WAIT(B_VFULL, n, 39)) {
-                clear_rows<DT>(v_base, there32, 32 * part);
+              if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY + 1, n ^ 1u, 40) &&
+                  WAIT(B_VFULL, n, 39) && WAIT(B_VFULL + 1, n, 39)) {
+                clear_rows<DT>(v_base, 32 * part);
                 // a score of -inf weighs nothing, but its row is not finite
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -923,7 +1016,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (!ok) break;
         l += sum;
         // the product before this tile's is complete, and P may be written
-        ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY, n ^ 1u, 40));
+        ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, 40));
         if (!ok) break;
         sas::tc_fence_after();
         if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
@@ -1056,6 +1149,32 @@ int launch(const TreeParams& p, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, tree_combine_kernel<DT>, p) == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(ptr);
+  });
+  return fn;
+}
+// Boxes of 64 rows x 64 columns of rows of 512: [outer, rows, 512], or [rows, 512] with outer 0.
+bool make_map(CUtensorMap* m, const void* base, int dtype, int64_t outer, int64_t rows) {
+  const EncodeTiled enc = encode_tiled();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)outer};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)rows * D * 2};
+  const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
+  return enc(m, dtype == SAS_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, outer ? 3 : 2,
+             const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
 }  // namespace
@@ -1107,6 +1226,12 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.part = reinterpret_cast<float*>(ws + 256);
   p.cuts = reinterpret_cast<Cut*>(ws + 256 + (size_t)num_sms * 2 * kPieceFloats * sizeof(float));
   p.status = status;
+  if ((int64_t)T * H >= (1ll << 31)) return SAS_ERR_UNSUPPORTED;
+  if (!make_map(&p.map_q, q, dtype, 0, (int64_t)T * H)) return SAS_ERR_CUDA;
+  for (int f = 0; f < (scenario == 2 ? 2 : 1); ++f) {
+    p.tma[f] = p.bs[f] % 64 == 0 && p.nblk[f] > 0;
+    if (p.tma[f] && !make_map(&p.map_kv[f], p.kv[f], dtype, p.nblk[f], p.bs[f])) return SAS_ERR_CUDA;
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == SAS_DTYPE_BF16 ? launch<SAS_DTYPE_BF16>(p, st) : launch<SAS_DTYPE_FP16>(p, st);
 }

@@ -37,13 +37,15 @@ class Cta:
     """One side of the pair; a group of warps with one task is one role."""
 
     def __init__(self):
-        names = dict(kfull=1, vfull=1, qfull=1, xk=1, xv=1, xq=1, kempty=1, vempty=1, qempty=1, pready=2, ofull=1, oempty=2)
+        names = dict(qfull=1, xq=1, qempty=1, pready=2, ofull=1, oempty=2)
+        names.update({f"{k}{h}": 1 for k in ("kfull", "vfull", "xk", "xv", "kempty", "vempty") for h in (0, 1)})  # halves of K, V
         names.update({f"{k}{i}": c for k, n, c in (("mask", 3, 1), ("sfull", 2, 1), ("sempty", 2, 2), ("fin", 2, 1), ("cfull", RING, 1),
                                                    ("cempty", RING, 5)) for i in range(n)})  # K, V, scores, products, softmax
         self.b = {k: Bar(v) for k, v in names.items()}
         self.ring, self.units = [None] * RING, [None] * UNIT_SLOTS
         self.mask, self.s, self.fin = [None] * 3, [None] * 2, [None] * 2
-        self.k = self.v = self.q = self.p = self.o = None
+        self.k, self.v = [None] * 2, [None] * 2
+        self.q = self.p = self.o = None
         self.out = []
 
 
@@ -100,19 +102,22 @@ class Model:
                 yield "qempty", q[0] + 1
                 self.copies.append(lambda: (setattr(me, "q", u), b["qfull"].arrive()))
                 q[0] += 1
-            yield "kempty", n + 1
-            self.copies.append(lambda: (setattr(me, "k", (n, u)), b["kfull"].arrive()))
+            for h in (0, 1):
+                yield f"kempty{h}", n + 1
+                self.copies.append(lambda h=h: (me.k.__setitem__(h, (n, u)), b[f"kfull{h}"].arrive()))
+                if h == 0:
+                    assert me.mask[n % 3] is None, "a mask was overwritten before it was read"
+                    me.mask[n % 3] = n
+                    b[f"mask{n % 3}"].arrive()
         yield from self.walk(side, tile)
 
     def v_loader(self, side):
         me, b = self.cta[side], self.cta[side].b
 
         def tile(n, u, fl):
-            assert me.mask[n % 3] is None, "a mask was overwritten before it was read"
-            me.mask[n % 3] = n
-            b[f"mask{n % 3}"].arrive()
-            yield "vempty", n + 1
-            self.copies.append(lambda: (setattr(me, "v", (n, u)), b["vfull"].arrive()))
+            for h in (0, 1):
+                yield f"vempty{h}", n + 1
+                self.copies.append(lambda h=h: (me.v.__setitem__(h, (n, u)), b[f"vfull{h}"].arrive()))
         yield from self.walk(side, tile)
 
     def pass_on(self, bar, to, par):
@@ -127,24 +132,26 @@ class Model:
                 if fl & FIRST:
                     yield from self.pass_on("qfull", "xq", units[0])
                     units[0] += 1
-                yield from self.pass_on("kfull", "xk", n)
+                for h in (0, 1):
+                    yield from self.pass_on(f"kfull{h}", f"xk{h}", n)
                 return
             if fl & FIRST:
                 yield "qfull", units[0]
                 yield "xq", units[0]
                 units[0] += 1
-            yield "kfull", n
-            yield "xk", n
             yield f"sempty{n & 1}", (n >> 1) + 1
+            for h in (0, 1):
+                yield f"kfull{h}", n
+                yield f"xk{h}", n
 
-            def run():
-                for cta in self.cta:
-                    assert cta.k == (n, u) and cta.q == u
-                    assert cta.s[n & 1] is None, "scores overwritten before they were read"
-                    cta.s[n & 1] = n
-            self.mmas["qk"].append(run)
+                def run(h=h):
+                    for cta in self.cta:
+                        assert cta.k[h] == (n, u) and cta.q == u
+                        assert cta.s[n & 1] == (n if h else None), "scores overwritten before they were read"
+                        cta.s[n & 1] = n
+                self.mmas["qk"].append(run)
+                self.commit("qk", f"kempty{h}")
             self.commit("qk", f"sfull{n & 1}")
-            self.commit("qk", "kempty")
             if fl & LAST:
                 self.commit("qk", "qempty")
         yield from self.walk(side, tile)
@@ -154,21 +161,25 @@ class Model:
 
         def tile(n, u, fl):
             if side:
-                yield from self.pass_on("vfull", "xv", n)
+                for h in (0, 1):
+                    yield from self.pass_on(f"vfull{h}", f"xv{h}", n)
                 return
-            yield "vfull", n
-            yield "xv", n
             yield "pready", n
             if fl & FIRST:
                 yield "oempty", done[0] + 1
 
-            def run():
-                for cta in self.cta:
-                    assert cta.v == (n, u) and cta.p == n
-                    assert (cta.o is None) if fl & FIRST else cta.o == (u, n - 1)
-                    cta.o = (u, n)
-            self.mmas["pv"].append(run)
-            self.commit("pv", "vempty")
+            for h in (0, 1):
+                yield f"vfull{h}", n
+                yield f"xv{h}", n
+
+                def run(h=h):
+                    for cta in self.cta:
+                        assert cta.v[h] == (n, u) and cta.p == n
+                        if h == 0:
+                            assert (cta.o is None) if fl & FIRST else cta.o == (u, n - 1)
+                            cta.o = (u, n)
+                self.mmas["pv"].append(run)
+                self.commit("pv", f"vempty{h}")
             if fl & LAST:
                 self.commit("pv", "ofull")
                 done[0] += 1
@@ -187,10 +198,11 @@ class Model:
             me.s[n & 1] = None
             first.b[f"sempty{n & 1}"].arrive()
             if self.rng.random() < 0.2:  # rows that are not finite: V has to be there
-                yield "vempty", n + 1
-                yield "vfull", n
-                assert me.v == (n, u)
-            yield "vempty", n + 1
+                yield "vempty1", n + 1
+                for h in (0, 1):
+                    yield f"vfull{h}", n
+                assert me.v == [(n, u)] * 2
+            yield "vempty1", n + 1
             me.p = n
             first.b["pready"].arrive()
             st["n"] += 1
@@ -200,7 +212,7 @@ class Model:
 
         def end():
             if st["n"]:
-                yield "vempty", st["n"] + 1
+                yield "vempty1", st["n"] + 1
             self.finish(me, st["u"], END)
         yield from self.walk(side, tile, end)
 
