@@ -135,7 +135,7 @@ struct TreeParams {
   uint8_t* out;
   float* lse;
   int T, H, G, R, scenario,  // G: head groups of 128, R: pairs of CTAs per group
-       K, ratio, win, B, S, layout, split;
+       K, ratio, win, B, S, layout;
   const int32_t* cu;
   const int32_t* seqused;
   const int32_t* parents;
@@ -194,13 +194,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t byt
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sas::smem_u32(bar)) : "memory");
 }
-}  // namespace
-namespace sas {
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+__device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sas::smem_u32(bar)), "r"(bytes) : "memory");
 }
-}  // namespace sas
-namespace {
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, uint64_t* bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
@@ -481,14 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const int64_t in = t - prefix;
       const int u = in < (1ll << 31) ? (int)((uint32_t)in / (uint32_t)r.tiles) : (int)(in / r.tiles);
       const int64_t ustart = prefix + (int64_t)u * r.tiles, uend = ustart + r.tiles;
-      int k0 = (int)(t - ustart), k1 = (int)min((int64_t)r.tiles, t1 - ustart);
-      if (!p.split) {  // a unit belongs to the range that its first tile is in
-        if (k0 > 0) {
-          t = uend;
-          continue;
-        }
-        k1 = r.tiles;
-      }
+      const int k0 = (int)(t - ustart), k1 = (int)min((int64_t)r.tiles, t1 - ustart);
       if (b != cached) {
         __syncwarp();
         if (!r.bad)
@@ -645,7 +634,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           if (!ok) break;
           if (tma) {
             if (lw == 0 && elect_one()) {
-              sas::mbar_expect_tx(&bars[full + h], 4 * KSLAB);
+              expect_tx(&bars[full + h], 4 * KSLAB);
               if (is_v) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -1113,10 +1102,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
           o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2]), o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3]);
         }
     }
-    const float k = used && top != -INFINITY ? 1.f / den : 0.f;
+    const float k = used && (top != -INFINITY || den != den) ? 1.f / den : 0.f;
     uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = used && (k != 0.f || den != den) ? pack2<DT>(o[2 * i] * k, o[2 * i + 1] * k) : 0u;
+    for (int i = 0; i < 8; ++i) v[i] = k != 0.f ? pack2<DT>(o[2 * i] * k, o[2 * i + 1] * k) : 0u;
     uint4* to = reinterpret_cast<uint4*>(tile + row * 128 + c4 * 8);
     to[0] = make_uint4(v[0], v[1], v[2], v[3]);
     to[1] = make_uint4(v[4], v[5], v[6], v[7]);
@@ -1136,7 +1125,6 @@ int launch(const TreeParams& p, cudaStream_t st) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return SAS_ERR_CUDA;
   kern<<<2 * p.R * p.G, kThreads, SMEM_BYTES, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SAS_ERR_CUDA;
-  if (!p.split) return SAS_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * p.R * p.G, D / 64);
   cfg.blockDim = dim3(256);
@@ -1213,7 +1201,6 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.G = scenario == 3 ? (H + UR - 1) / UR : 1;
   if (2 * p.G > num_sms) return SAS_ERR_UNSUPPORTED;
   p.R = num_sms / (2 * p.G);
-  p.split = 1;
   p.cu = cu, p.seqused = seqused, p.parents = parents;
   p.kv[0] = static_cast<const uint8_t*>(ori_kv), p.kv[1] = static_cast<const uint8_t*>(cmp_kv);
   p.bt[0] = ori_bt, p.bt[1] = cmp_bt;

@@ -58,26 +58,30 @@ def tree_attn_sharedkv(
     cmp_ratio``: with ``cmp_kv`` to all of them, with ``cmp_sparse_indices``
     (``[T, 1, K]`` or ``[B, S, 1, K]``) to its list, where ids outside that
     range are skipped. A KV row with infinities or NaN makes the output of the
-    tokens that see it NaN, and of no others. A request of over 1024 tokens,
+    tokens that see it NaN, at least in the columns where the row is not
+    finite; it reaches no other token. A request of over 1024 tokens,
     with more tokens than ``seqused_kv``, or a token whose parent does not
     precede it gives zeros and is recorded in the status word.
     """
     assert layout_kv == "PA_ND", "only layout_kv=PA_ND supported"
     assert layout_q in LAYOUTS, f"unsupported layout_q={layout_q!r}"
-    code = _dtype_code(q.dtype)
+    # shapes are read once each: every read of a tensor's property costs 0.2-0.3 us,
+    # and the smallest calls take as long on the host as on the GPU
+    dtype, shape = q.dtype, q.shape
+    code = _dtype_code(dtype)
     if layout_q == "TND":
         assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
-        if q.dim() != 3:
-            raise ValueError(f"q must be [T, heads, {HEAD_DIM}] (got {tuple(q.shape)})")
+        if len(shape) != 3:
+            raise ValueError(f"q must be [T, heads, {HEAD_DIM}] (got {tuple(shape)})")
+        T, H, D = shape
         B, S = cu_seqlens_q.numel() - 1, 0
     else:
-        if q.dim() != 4:
-            raise ValueError(f"q must be [B, S, heads, {HEAD_DIM}] (got {tuple(q.shape)})")
-        B, S = q.shape[0], q.shape[1]
+        if len(shape) != 4:
+            raise ValueError(f"q must be [B, S, heads, {HEAD_DIM}] (got {tuple(shape)})")
+        B, S, H, D = shape
+        T = B * S
         if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
             raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
-    H, D = q.shape[-2:]
-    T = q.shape[:-2].numel()
     if D != HEAD_DIM or H <= 0 or H % 8:
         raise ValueError(f"only D={HEAD_DIM} and heads a multiple of 8 supported (got {H} heads, D={D})")
     if ori_win_left < 0:
@@ -97,53 +101,65 @@ def tree_attn_sharedkv(
         scenario, K = 3, cmp_sparse_indices.shape[-1]
         if K < 1 or cmp_sparse_indices.numel() != T * K:
             raise ValueError(f"cmp_sparse_indices must be [tokens, 1, K] (got {tuple(cmp_sparse_indices.shape)})")
-    for name, kv, table in (("ori", ori_kv, ori_block_table), ("cmp", cmp_kv, cmp_block_table)):
-        if kv is None:
-            continue
-        if kv.dim() != 4 or kv.shape[2] != 1 or kv.shape[3] != D or kv.dtype != q.dtype or kv.shape[1] < 1:
-            raise ValueError(f"{name}_kv must be [blocks, block size, 1, {D}] of q's dtype")
-        if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1:
-            raise ValueError(f"{name}_block_table must be [{B}, blocks] (got {tuple(table.shape)})")
+    ori_dims = _check_pool("ori", ori_kv, ori_block_table, B, dtype)
+    cmp_dims = (0, 0, 0) if cmp_kv is None else _check_pool("cmp", cmp_kv, cmp_block_table, B, dtype)
     if B < 0 or seqused_kv.numel() != B:
         raise ValueError(f"seqused_kv must have one entry per request (got {seqused_kv.numel()} for {B})")
-    for name, t, shape, dt in (("out", out, q.shape, q.dtype), ("lse_out", lse_out, q.shape[:-1], torch.float32)):
-        if t is not None and (t.shape != shape or t.dtype != dt or t.device != q.device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor of {dt} beside q")
-    if not q.is_cuda:
-        raise RuntimeError("tree_attn_sharedkv needs q on a CUDA device (no CPU path)")
     dev = q.device
-    q = _aligned(q)
+    if out is not None:
+        _check_out("out", out, shape, dtype, dev)
+    if lse_out is not None:
+        _check_out("lse_out", lse_out, shape[:-1], torch.float32, dev)
+    if dev.type != "cuda":
+        raise RuntimeError("tree_attn_sharedkv needs q on a CUDA device (no CPU path)")
+    q = _aligned(q, dev)
     if out is None:
         out = torch.empty_like(q)
     if lse_out is None and return_softmax_lse:
-        lse_out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
+        lse_out = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     if T:
         lib = _lib.lib()
         st = _lib.state(dev)
         cu = _i32(cu_seqlens_q, dev) if cu_seqlens_q is not None else None
         skv, par = _i32(seqused_kv, dev), _i32(tree_parents, dev)
         snk = _f32(sinks, dev)
-        ori, obt = _aligned(ori_kv.to(dev)), _i32(ori_block_table, dev)
+        ori, obt = _aligned(ori_kv, dev), _i32(ori_block_table, dev)
         cmp = cbt = idx = None
         if scenario >= 2:
-            cmp, cbt = _aligned(cmp_kv.to(dev)), _i32(cmp_block_table, dev)
+            cmp, cbt = _aligned(cmp_kv, dev), _i32(cmp_block_table, dev)
         if scenario == 3:
             idx = _i32(cmp_sparse_indices, dev)
         # from the allocator, so that calls on several streams do not share it
-        ws = torch.empty(lib.sas_tree_attn_workspace_bytes(st.num_sms), dtype=torch.uint8, device=dev)
+        nws = lib.sas_tree_attn_workspace_bytes(st.num_sms)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         rc = lib.sas_tree_attn_sharedkv(
             q.data_ptr(), T, H, D, code, LAYOUTS[layout_q], B, S, _lib.ptr(cu), skv.data_ptr(), par.data_ptr(),
-            ori.data_ptr(), ori.shape[0], ori.shape[1], obt.data_ptr(), obt.shape[1], _lib.ptr(cmp),
-            0 if cmp is None else cmp.shape[0], 0 if cmp is None else cmp.shape[1], _lib.ptr(cbt),
-            0 if cbt is None else cbt.shape[1], _lib.ptr(idx), K, snk.data_ptr(), float(softmax_scale), int(ratio),
+            ori.data_ptr(), ori_dims[0], ori_dims[1], obt.data_ptr(), ori_dims[2], _lib.ptr(cmp), cmp_dims[0],
+            cmp_dims[1], _lib.ptr(cbt), cmp_dims[2], _lib.ptr(idx), K, snk.data_ptr(), float(softmax_scale), int(ratio),
             min(int(ori_win_left), 1 << 30), scenario, out.data_ptr(), _lib.ptr(lse_out), st.num_sms,
-            st.status.data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(dev))
+            st.status.data_ptr(), ws.data_ptr(), nws, _lib.raw_stream(dev))
         if rc in (1, 2):
             raise ValueError(f"tree_attn_sharedkv: {_lib.ERRORS[rc]}")
         _lib.check(rc, "sas_tree_attn_sharedkv")
     return (out, lse_out) if return_softmax_lse else out
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+def _check_pool(name, kv, table, B, dtype) -> Tuple[int, int, int]:
+    """Blocks, rows of a block, and entries of a request in the block table."""
+    ks, ts = kv.shape, table.shape
+    if len(ks) != 4 or ks[2] != 1 or ks[3] != HEAD_DIM or kv.dtype != dtype or ks[1] < 1:
+        raise ValueError(f"{name}_kv must be [blocks, block size, 1, {HEAD_DIM}] of q's dtype")
+    if len(ts) != 2 or ts[0] != B or ts[1] < 1:
+        raise ValueError(f"{name}_block_table must be [{B}, blocks] (got {tuple(ts)})")
+    return ks[0], ks[1], ts[1]
+
+
+def _check_out(name, t, shape, dtype, dev) -> None:
+    if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor of {dtype} beside q")
+
+
+def _aligned(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if t.device != dev or not t.is_contiguous():
+        t = t.to(dev).contiguous()
     return t if t.data_ptr() & 15 == 0 else t.clone()

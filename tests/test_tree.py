@@ -286,6 +286,30 @@ def test_rows_that_are_not_finite(gpu, bad, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bs", [64, 48, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_past_the_committed_ones_are_not_finite(gpu, bad, bs):
+    """What a page of the compressed cache holds past its request's last row reaches nobody."""
+    c = Case([3, 1, 2], [1000, 514, 5], H=16, scenario=2, bs=bs)
+    for b, ctx in enumerate(c.ctx):
+        for p in range(ctx // c.ratio, (ctx // c.ratio + bs - 1) // bs * bs):
+            c.cmp[c.cbt[b, p // bs], p % bs] = bad
+    c.check(*c.call())
+
+
+@pytest.mark.gpu
+def test_weightless_rows_that_are_not_finite(gpu):
+    """Scores of -inf alone in a part of a cut unit: the joined result is still NaN for the tokens that see the rows."""
+    c = Case([1], [40000], H=8, scenario=1, win=1 << 20)
+    c.q[..., 7] = -1.0
+    for p in range(40001):
+        c.ori[c.obt[0, p // c.bs], p % c.bs, 0, 7] = float("inf")
+    c.sinks[:] = float("-inf")
+    out, lse = c.call()
+    assert torch.isnan(out[..., 7].float()).all() and torch.isnan(lse).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scenario", [1, 2, 3])
 def test_chain_is_the_frameworks_decode(gpu, scenario):
     """A tree that is a chain, with no compressed row ending among its tokens, is sparse_attn_sharedkv's case."""
