@@ -22,6 +22,7 @@ status word (``check_device_status``).
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -85,19 +86,29 @@ def _rows(t: torch.Tensor, name: str, out: bool = False):
 
 
 def _new(like: torch.Tensor) -> torch.Tensor:
-    if like.is_contiguous():
+    if like.is_contiguous():  # 0.7 us less than with a memory format given
         return torch.empty_like(like)
-    return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
-def _rope_args(dev, D, T, positions, cos, sin, norm, inverse, interleaved, slots=False):
+def _out_rows(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    """The output tensor, a new one without ``out``, and its rows as the kernel takes them."""
+    if out is None:
+        out = _new(like)
+        H, D = like.shape[-2:]
+        return out, (out.data_ptr(), H * D, D)
+    return out, _rows(out, name, out=True)[1]
+
+
+def _rope_args(D, T, positions, cos, sin, norm, inverse, interleaved, slots=False):
     """(positions, cos, sin, P, R, flags), checked; the tensors are returned to be kept alive."""
     flags = (FLAG_NORM if norm else 0) | (FLAG_INVERSE if inverse else 0) | (FLAG_INTERLEAVED if interleaved else 0)
     if cos is None and sin is None:
         return None, None, None, 0, 0, flags
-    if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2:
+    shape = None if cos is None else cos.shape
+    if shape is None or sin is None or shape != sin.shape or len(shape) != 2:
         raise ValueError("cos and sin must both be [positions, rotated dims / 2]")
-    P, R = cos.shape[0], 2 * cos.shape[1]
+    P, R = shape[0], 2 * shape[1]
     step = 8 if interleaved else 16
     if P < 1 or R < 1 or R > D or R % step:
         raise ValueError(f"the rotated dims must be a multiple of {step} and at most D={D} (got {R})")
@@ -107,9 +118,10 @@ def _rope_args(dev, D, T, positions, cos, sin, norm, inverse, interleaved, slots
     else:
         if positions.numel() != T:
             raise ValueError(f"positions must have one entry per token (got {positions.numel()} for {T})")
-        if positions.dtype == torch.int64:
+        dtype = positions.dtype
+        if dtype is torch.int64:
             flags |= FLAG_POS64
-        elif positions.dtype != torch.int32:
+        elif dtype is not torch.int32:
             raise ValueError(f"positions must be int32 or int64 (got {positions.dtype})")
     return positions, cos, sin, P, R, flags
 
@@ -124,16 +136,23 @@ def _check_dim(D: int, *weights) -> None:
     if D % 8 or not 0 < D <= MAX_DIM:
         raise ValueError(f"the head dim must be a multiple of 8 and at most {MAX_DIM} (got {D})")
     for w in weights:
-        if w is not None and tuple(w.shape) != (D,):
+        if w is not None and w.shape != (D,):
             raise ValueError(f"a weight must be [{D}] (got {tuple(w.shape)})")
 
 
 def _check_pair(q, k):
-    if q.dim() < 2 or q.shape[-2] < 1:
-        raise ValueError(f"q must be [..., heads, D] (got {tuple(q.shape)})")
-    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]
-                          or k.shape[-2] < 1 or k.dtype != q.dtype or k.device != q.device):
-        raise ValueError("k must have q's token dims, head dim, dtype and device")
+    """(tokens, head dim) of q and k, checked. Shapes are read once: every read of
+    a tensor's property costs 0.2-0.3 us, and the smallest calls take longer on the host
+    than on the GPU."""
+    qs = q.shape
+    if len(qs) < 2 or qs[-2] < 1:
+        raise ValueError(f"q must be [..., heads, D] (got {tuple(qs)})")
+    if k is not None:
+        ks = k.shape
+        if len(ks) != len(qs) or ks[:-2] != qs[:-2] or ks[-1] != qs[-1] or ks[-2] < 1 or k.dtype != q.dtype \
+                or k.device != q.device:
+            raise ValueError("k must have q's token dims, head dim, dtype and device")
+    return math.prod(qs[:-2]), qs[-1]
 
 
 def _check_out(out, like, name):
@@ -173,33 +192,28 @@ def head_norm_rope(
     there is no rotation; ``norm=False`` leaves out the norm; ``inverse`` turns
     by the negative angle. ``q_out`` / ``k_out`` may be the inputs themselves.
     """
-    _check_pair(q, k)
-    D = q.shape[-1]
+    T, D = _check_pair(q, k)
     _check_dim(D, q_weight, k_weight)
     code = _dtype_code(q.dtype)
     assert norm or (q_weight is None and k_weight is None), "weights need norm=True"
-    T = q.shape[:-2].numel()
-    positions, cos, sin, P, R, flags = _rope_args(q.device, D, T, positions, cos, sin, norm, inverse, interleaved)
+    positions, cos, sin, P, R, flags = _rope_args(D, T, positions, cos, sin, norm, inverse, interleaved)
     _check_out(q_out, q, "q_out")
     _check_out(k_out, k, "k_out")
-    if not q.is_cuda:
-        raise RuntimeError("head_norm_rope needs CUDA tensors (no CPU path)")
     dev = q.device
-    if q_out is None:
-        q_out = _new(q)
-    if k is not None and k_out is None:
-        k_out = _new(k)
+    if dev.type != "cuda":
+        raise RuntimeError("head_norm_rope needs CUDA tensors (no CPU path)")
+    q_out, qo = _out_rows(q_out, q, "q_out")
+    ka = ko = _NO_ROWS
+    Hk = 0
+    if k is not None:
+        k_out, ko = _out_rows(k_out, k, "k_out")
     if T:
         positions, cos, sin = _to_dev(dev, positions, cos, sin)
         qw, kw = _f32(q_weight, dev), _f32(k_weight if k is not None else None, dev)
         q, qa = _rows(q, "q")
-        _, qo = _rows(q_out, "q_out", out=True)
-        ka = ko = _NO_ROWS
-        Hk = 0
         if k is not None:
             Hk = k.shape[-2]
             k, ka = _rows(k, "k")
-            _, ko = _rows(k_out, "k_out", out=True)
         rc = _lib.lib().sas_head_norm_rope_fwd(
             *qa, *qo, q.shape[-2], *ka, *ko, Hk, T, D, code, _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), P, R,
             _lib.ptr(qw), _lib.ptr(kw), float(eps), flags, _lib.state(dev).status.data_ptr(), _lib.raw_stream(dev))
@@ -226,20 +240,19 @@ def head_norm_rope_backward(
     """Gradients ``(dq, dk, dq_weight, dk_weight)`` of ``head_norm_rope`` from
     those of its results and its inputs; ``dk`` is None without ``k`` and a
     weight's gradient (fp32, summed in a fixed order) without that weight."""
-    _check_pair(q, k)
-    D = q.shape[-1]
+    T, D = _check_pair(q, k)
     _check_dim(D, q_weight, k_weight)
     code = _dtype_code(q.dtype)
     assert norm or (q_weight is None and k_weight is None), "weights need norm=True"
-    T = q.shape[:-2].numel()
-    positions, cos, sin, P, R, flags = _rope_args(q.device, D, T, positions, cos, sin, norm, inverse, interleaved)
-    if dq_out.shape != q.shape or (k is not None and (dk_out is None or dk_out.shape != k.shape)):
-        raise ValueError("dq_out and dk_out must have the shapes of q and k")
-    if dq_out.device != q.device or (k is not None and dk_out.device != q.device):
-        raise ValueError("dq_out and dk_out must be on the device of q and k")
-    if not q.is_cuda:
-        raise RuntimeError("head_norm_rope_backward needs CUDA tensors (no CPU path)")
+    positions, cos, sin, P, R, flags = _rope_args(D, T, positions, cos, sin, norm, inverse, interleaved)
     dev = q.device
+    for x, dx in ((q, dq_out), (k, dk_out)):
+        if x is not None and (dx is None or dx.shape != x.shape):
+            raise ValueError("dq_out and dk_out must have the shapes of q and k")
+        if x is not None and dx.device != dev:
+            raise ValueError("dq_out and dk_out must be on the device of q and k")
+    if dev.type != "cuda":
+        raise RuntimeError("head_norm_rope_backward needs CUDA tensors (no CPU path)")
     dq = _new(q)
     dk = _new(k) if k is not None else None
     qw = _f32(q_weight, dev)
@@ -297,38 +310,42 @@ class _Paged:
 
     def __init__(self, kv, pool, table, seqused, cu, layout):
         assert layout in LAYOUTS, f"unsupported layout_q={layout!r}"
-        if pool.dim() != 4 or pool.shape[2] != 1:
-            raise ValueError(f"the cache must be [blocks, block size, 1, D] (got {tuple(pool.shape)})")
+        ps, ks, ts = pool.shape, kv.shape, table.shape
+        if len(ps) != 4 or ps[2] != 1:
+            raise ValueError(f"the cache must be [blocks, block size, 1, D] (got {tuple(ps)})")
         if pool.dtype != kv.dtype:
             raise ValueError("the cache must have the dtype of kv")
-        D = pool.shape[3]
+        D = ps[3]
         if not pool.is_contiguous() or pool.data_ptr() % 16:
             raise ValueError("the cache must be contiguous and 16-byte aligned")
         want = 3 if layout == "TND" else 4  # [T, 1, D] or [B, S, 1, D]; the head dim may be left out
-        if kv.dim() == want - 1:
+        if len(ks) == want - 1:
             kv = kv.unsqueeze(-2)
-        if kv.dim() != want or kv.shape[-2] != 1 or kv.shape[-1] != D:
-            raise ValueError(f"kv must be [tokens, 1, {D}] in the layout {layout} (got {tuple(kv.shape)})")
-        if table.dim() != 2:
+            ks = kv.shape
+        if len(ks) != want or ks[-2] != 1 or ks[-1] != D:
+            raise ValueError(f"kv must be [tokens, 1, {D}] in the layout {layout} (got {tuple(ks)})")
+        if len(ts) != 2:
             raise ValueError("ori_block_table must be [requests, blocks]")
         if layout == "TND":
             assert cu is not None, "cu_seqlens_q is required for TND"
-            self.B, self.S = cu.numel() - 1, 0
+            self.B, self.S, self.T = cu.numel() - 1, 0, ks[0]
         else:
-            self.B, self.S = kv.shape[0], kv.shape[1]
+            self.B, self.S = ks[:2]
+            self.T = self.B * self.S
             if cu is not None and cu.numel() != self.B + 1:
                 raise ValueError(f"cu_seqlens_q must have {self.B + 1} entries (got {cu.numel()})")
-        if self.B < 0 or table.shape[0] != self.B or seqused.numel() != self.B:
+        if self.B < 0 or ts[0] != self.B or seqused.numel() != self.B:
             raise ValueError(f"ori_block_table and seqused_kv must have one entry per request ({self.B})")
-        self.kv, self.D, self.T, self.layout = kv, D, kv.shape[:-2].numel(), LAYOUTS[layout]
-        self.pool, self.table, self.cu, self.seqused = pool, table, cu, seqused
+        self.kv, self.D, self.layout = kv, D, LAYOUTS[layout]
+        self.blocks, self.block_size, self.entries = ps[0], ps[1], ts[1]
+        self.table, self.cu, self.seqused = table, cu, seqused
 
     def put(self, dev):
         self.table, self.seqused = _i32(self.table, dev), _i32(self.seqused, dev)
         self.cu = _i32(self.cu, dev) if self.cu is not None else None
 
     def args(self):
-        return (self.pool.shape[0], self.pool.shape[1], self.table.data_ptr(), self.table.shape[1], _lib.ptr(self.cu),
+        return (self.blocks, self.block_size, self.table.data_ptr(), self.entries, _lib.ptr(self.cu),
                 self.seqused.data_ptr(), self.B, self.S, self.layout)
 
 
@@ -370,28 +387,27 @@ def append_shared_kv(
     _check_dim(D, weight, q_weight)
     code = _dtype_code(kv.dtype)
     assert norm or (weight is None and q_weight is None), "weights need norm=True"
-    positions, cos, sin, P, R, flags = _rope_args(kv.device, D, T, positions, cos, sin, norm, False, interleaved, slots=True)
+    positions, cos, sin, P, R, flags = _rope_args(D, T, positions, cos, sin, norm, False, interleaved, slots=True)
     if q is not None:
         _check_pair(q, p.kv)
         _check_out(q_out, q, "q_out")
-    if not kv.is_cuda:
-        raise RuntimeError("append_shared_kv needs CUDA tensors (no CPU path)")
     dev = kv.device
+    if dev.type != "cuda":
+        raise RuntimeError("append_shared_kv needs CUDA tensors (no CPU path)")
     if ori_kv.device != dev or (q is not None and q.device != dev):
         raise ValueError("kv, ori_kv and q must be on one device")
-    if q is not None and q_out is None:
-        q_out = _new(q)
+    qa = qo = _NO_ROWS
+    H = 0
+    if q is not None:
+        q_out, qo = _out_rows(q_out, q, "q_out")
     if T:
         p.put(dev)
         positions, cos, sin = _to_dev(dev, positions, cos, sin)
         w, qw = _f32(weight, dev), _f32(q_weight if q is not None else None, dev)
         r, ra = _rows(p.kv, "kv")
-        qa = qo = _NO_ROWS
-        H = 0
         if q is not None:
             H = q.shape[-2]
             q, qa = _rows(q, "q")
-            _, qo = _rows(q_out, "q_out", out=True)
         rc = _lib.lib().sas_append_sharedkv(
             *ra[:2], ori_kv.data_ptr(), *p.args(), *qa, *qo, H, T, D, code, _lib.ptr(positions), _lib.ptr(cos),
             _lib.ptr(sin), P, R, _lib.ptr(w), _lib.ptr(qw), float(eps), flags, _lib.state(dev).status.data_ptr(),
@@ -425,10 +441,10 @@ def append_shared_kv_backward(
     _check_dim(D, weight)
     code = _dtype_code(kv.dtype)
     assert norm or weight is None, "weights need norm=True"
-    positions, cos, sin, P, R, flags = _rope_args(kv.device, D, T, positions, cos, sin, norm, False, interleaved, slots=True)
-    if not kv.is_cuda:
-        raise RuntimeError("append_shared_kv_backward needs CUDA tensors (no CPU path)")
+    positions, cos, sin, P, R, flags = _rope_args(D, T, positions, cos, sin, norm, False, interleaved, slots=True)
     dev = kv.device
+    if dev.type != "cuda":
+        raise RuntimeError("append_shared_kv_backward needs CUDA tensors (no CPU path)")
     if d_ori_kv.device != dev:
         raise ValueError("kv and d_ori_kv must be on one device")
     dkv = _new(kv)
