@@ -24,8 +24,10 @@
 // 45.6 (N = 128) and the full rate of 64 (N = 256), all measured; and K and V,
 // 64 KB each, are then separate buffers, so that the next tile's K is copied
 // and multiplied while this tile's softmax runs. The accumulators use all 128
-// TMEM lanes (lanes 64-127 hold the upper half of the columns): O takes 256
-// columns, two buffers of S 64 each.
+// TMEM lanes (lanes 64-127 hold the upper half of the columns): two buffers of S
+// take 64 columns each, O two of three places of 128, in turn: half q of the
+// sequence of the units' halves has place q % 3, so that a unit's products begin
+// while the unit before it is read.
 // The softmax is one pass with a running maximum that moves, and rescales O,
 // only when a row's maximum rises by more than 2^8: P then stays below 2^8, and
 // P, l and O keep one common scale. P is rounded to the I/O type for the
@@ -69,7 +71,7 @@ constexpr int kSmWarps = 8, kEpiWarp0 = 8, kEpiWarps = 4, kQkWarp = 12, kPvWarp 
 constexpr int kThreads = 32 * 23;
 constexpr int kRing = 5;          // tiles the coordinator may be ahead
 constexpr int kUnitSlots = 7;     // > kRing + 1: no slot is rewritten while a published tile names it
-constexpr uint32_t TM_O = 0, TM_S = 256, TM_COLS = 512;
+constexpr uint32_t TM_O = 0, TM_S = 384, TM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMove = 8.f;      // log2 units the running maximum may lag
 
@@ -85,7 +87,7 @@ constexpr int OFF_MISC = OFF_P + 2 * QSLAB;
 // that the next tile's first half is on its way while the second is multiplied.
 enum Bar { B_KFULL = 0, B_VFULL = 2, B_QFULL = 4, B_XK, B_XV = B_XK + 2, B_XQ = B_XV + 2, B_KEMPTY, B_VEMPTY = B_KEMPTY + 2,
            B_QEMPTY = B_VEMPTY + 2, B_MASK, B_SFULL = B_MASK + 3, B_SEMPTY = B_SFULL + 2, B_PREADY = B_SEMPTY + 2, B_OFULL, B_OEMPTY,
-           B_FIN, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
+           B_FIN = B_OEMPTY + 3, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
 
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
@@ -380,7 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     init(B_SFULL, 2, 1);
     init(B_SEMPTY, 3, 2 * kSmWarps);    // and PREADY: softmax warps of both CTAs
     init(B_OFULL, 1, 1);
-    init(B_OEMPTY, 1, 2 * kEpiWarps);
+    init(B_OEMPTY, 3, 2 * kEpiWarps);
     init(B_FIN, 2, kSmWarps);
     init(B_SSYNC, 2, kSmWarps / 2);     // the warps of 32 rows
     init(B_CFULL, kRing, 1);
@@ -721,18 +723,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
             const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
             if (!WAIT_PAIR(B_PREADY, n, 27)) break;
-            if ((t.flags & TF_FIRST) && !WAIT_PAIR(B_OEMPTY, u ^ 1u, 28)) break;
             const int steps = max(1, (t.nrows + 15) / 16);
             bool ok = true;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
-              ok = WAIT(B_VFULL + h, n, 35) && WAIT_PAIR(B_XV + h, n, 36);
+              const uint32_t oh = 2 * u + h, place = oh % 3;
+              ok = (!(t.flags & TF_FIRST) || WAIT_PAIR(B_OEMPTY + place, (oh / 3) ^ 1u, 28)) && WAIT(B_VFULL + h, n, 35) &&
+                   WAIT_PAIR(B_XV + h, n, 36);
               if (!ok) break;
               sas::fence_proxy_async_smem();
               sas::tc_fence_after();
 #pragma unroll 1
               for (int ks = 0; ks < steps; ++ks)
-                umma2(tmem + TM_O + 128 * h, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
+                umma2(tmem + TM_O + 128 * place, p_desc + (((ks >> 2) * QSLAB + (ks & 3) * 32) >> 4),
                       v_desc + ((2 * h * VSLAB + ks * 2048) >> 4), id_o, !((t.flags & TF_FIRST) && ks == 0));
               commit2(&bars[B_VEMPTY + h]);
             }
@@ -832,12 +835,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       for (int x = 0; x < 8; ++x) {
         uint32_t r[32];
         __syncwarp();
-        sas::tmem_ld32(tl + TM_O + 32 * x, r);
+        const uint32_t oh = 2 * u + (x >> 2), place = oh % 3;
+        sas::tmem_ld32(tl + TM_O + 128 * place + 32 * (x & 3), r);
         sas::tmem_wait_ld();
-        if (x == 7) {  // O is read
+        if ((x & 3) == 3) {  // this half of O is read
           sas::tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_first(&bars[B_OEMPTY]);
+          if (lane == 0) arrive_first(&bars[B_OEMPTY + place]);
         }
         if (part >= 0) {  // [D / 4][64 rows] of float4: a warp's stores are contiguous
           uint4* d4 = reinterpret_cast<uint4*>(o) + (size_t)(ch * 64 + x * 8) * MR + row;
@@ -1010,13 +1014,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         sas::tc_fence_after();
         if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
 #pragma unroll 1
-          for (int x = 128 * gr; x < 128 * gr + 128; x += 32) {
+          for (int x = 0; x < 128; x += 32) {
+            const uint32_t at = tl + TM_O + 128 * ((2 * u + gr) % 3) + x;
             uint32_t r[32];
-            sas::tmem_ld32(tl + TM_O + x, r);
+            sas::tmem_ld32(at, r);
             sas::tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * fac);
-            sas::tmem_st32(tl + TM_O + x, r);
+            sas::tmem_st32(at, r);
           }
           sas::tmem_wait_st();
         }
@@ -1030,8 +1035,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (lane == 0) arrive_first(&bars[B_PREADY]);
         ++n;
         if (t.flags & TF_LAST) {
-          // The place was unit u - 2's: its O was read, after these, before the
-          // first product of unit u - 1, and that is complete.
+          // The place was unit u - 2's: the first half of its O was read, after
+          // these, before the second half of unit u - 1's first product, and that
+          // is complete.
           Fin& fin = ms.fin[u & 1];
           fin.l[part][row] = used ? l : -1.f;
           if (part == 0) fin.m[row] = m;

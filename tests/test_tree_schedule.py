@@ -37,15 +37,16 @@ class Cta:
     """One side of the pair; a group of warps with one task is one role."""
 
     def __init__(self):
-        names = dict(qfull=1, xq=1, qempty=1, pready=2, ofull=1, oempty=2)
+        names = dict(qfull=1, xq=1, qempty=1, pready=2, ofull=1)
         names.update({f"{k}{h}": 1 for k in ("kfull", "vfull", "xk", "xv", "kempty", "vempty") for h in (0, 1)})  # halves of K, V
-        names.update({f"{k}{i}": c for k, n, c in (("mask", 3, 1), ("sfull", 2, 1), ("sempty", 2, 2), ("fin", 2, 1), ("cfull", RING, 1),
+        names.update({f"{k}{i}": c for k, n, c in (("mask", 3, 1), ("sfull", 2, 1), ("sempty", 2, 2), ("oempty", 3, 2), ("fin", 2, 1), ("cfull", RING, 1),
                                                    ("cempty", RING, 5)) for i in range(n)})  # K, V, scores, products, softmax
         self.b = {k: Bar(v) for k, v in names.items()}
         self.ring, self.units = [None] * RING, [None] * UNIT_SLOTS
         self.mask, self.s, self.fin = [None] * 3, [None] * 2, [None] * 2
         self.k, self.v = [None] * 2, [None] * 2
-        self.q = self.p = self.o = None
+        self.q = self.p = None
+        self.o = [None] * 3  # places of halves of O, in turn
         self.out = []
 
 
@@ -165,19 +166,18 @@ class Model:
                     yield from self.pass_on(f"vfull{h}", f"xv{h}", n)
                 return
             yield "pready", n
-            if fl & FIRST:
-                yield "oempty", done[0] + 1
-
             for h in (0, 1):
+                use, place = divmod(2 * done[0] + h, 3)
+                if fl & FIRST:
+                    yield f"oempty{place}", use + 1
                 yield f"vfull{h}", n
                 yield f"xv{h}", n
 
-                def run(h=h):
+                def run(h=h, place=place):
                     for cta in self.cta:
                         assert cta.v[h] == (n, u) and cta.p == n
-                        if h == 0:
-                            assert (cta.o is None) if fl & FIRST else cta.o == (u, n - 1)
-                            cta.o = (u, n)
+                        assert cta.o[place] == (None if fl & FIRST else (u, n - 1, h)), "O overwritten before it was read"
+                        cta.o[place] = (u, n, h)
                 self.mmas["pv"].append(run)
                 self.commit("pv", f"vempty{h}")
             if fl & LAST:
@@ -229,10 +229,13 @@ class Model:
             if what == END:
                 return
             yield "ofull", u
-            assert me.o == what
-            me.o = None
+            for h in (0, 1):
+                place = (2 * u + h) % 3
+                assert me.o[place] == (*what, h)
+                me.o[place] = None
+                self.cta[0].b[f"oempty{place}"].arrive()
+                yield None, 0  # others may run in between
             me.out.append(what[0])
-            self.cta[0].b["oempty"].arrive()
             u += 1
 
     def run(self):
@@ -242,7 +245,7 @@ class Model:
         live = {i for i, w in waits.items() if w}
         bias = self.rng.choice([None, *range(len(roles))])  # one role is slow, or none
         while live:
-            ready = [i for i in live if self.cta[roles[i][0]].b[waits[i][0]].done(waits[i][1])]
+            ready = [i for i in live if waits[i][0] is None or self.cta[roles[i][0]].b[waits[i][0]].done(waits[i][1])]
             events = ready + [q for q in self.mmas if self.mmas[q]] + (["copy"] if self.copies else [])
             assert events, f"blocked: {[(roles[i][0], kinds[i % len(kinds)].__name__, waits[i]) for i in live]}"
             e = self.rng.choice([x for x in events if x != bias] or events)
