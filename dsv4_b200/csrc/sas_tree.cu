@@ -156,9 +156,11 @@ struct TreeParams {
   CUtensorMap map_kv[2], map_q;
 };
 
-// What a request brings: its tokens, and the tiles of each of its units.
+// What a request brings: its tokens, and the tiles of each of its units. Units of
+// padding alone, after the last token in use, are none of the sequence's (with them
+// ranges that hold few used units wait for those that hold many).
 struct Req {
-  int base, slots, n, ctx, thr, lo, units, wtiles, tiles;  // lo: the window tiles' first row
+  int base, slots, n, used, ctx, thr, lo, units, wtiles, tiles;  // used: tokens up to the last in use, lo: the window tiles' first row
   bool bad;
   __device__ __forceinline__ int64_t all() const { return (int64_t)units * tiles; }
 };
@@ -176,11 +178,23 @@ __device__ __noinline__ Req request(const TreeParams& p, int b) {
   r.ctx = __ldg(p.seqused + b) - r.n;
   r.bad = r.n > kMaxTree || r.ctx < 0 || r.ctx > kMaxCtx;
   r.thr = p.scenario == 1 || r.bad ? 0 : r.ctx / p.ratio;
-  r.units = p.scenario == 3 ? r.slots : (int)(((int64_t)r.slots * p.H + UR - 1) / UR);
+  r.used = r.n;
+  if (p.layout == SAS_LAYOUT_BSND && !r.bad)  // the last 64 slots are looked through, 8 loads at a time
+    for (int k = 0; k < 8 && r.used > 0; ++k) {
+      const int from = max(r.used - 8, 0);
+      int last = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (from + i < r.used && __ldg(p.parents + r.base + from + i) >= -1) last = from + i + 1;
+      r.used = last ? last : from;
+      if (last) break;
+    }
+  const int held = r.bad ? r.slots : r.used;
+  r.units = p.scenario == 3 ? held : (int)(((int64_t)held * p.H + UR - 1) / UR);
   r.lo = max(r.ctx - p.win, 0);
   if (p.tma[0]) r.lo &= ~63;
-  r.wtiles = r.bad || r.n == 0 ? 1 : (r.ctx - r.lo + r.n + CH - 1) / CH;
-  r.tiles = r.wtiles + (r.bad || r.n == 0 ? 0 : p.scenario == 2 ? (r.thr + CH - 1) / CH : p.scenario == 3 && r.thr > 0 ? (p.K + CH - 1) / CH : 0);
+  r.wtiles = r.bad || r.used == 0 ? 1 : (r.ctx - r.lo + r.used + CH - 1) / CH;
+  r.tiles = r.wtiles + (r.bad || r.used == 0 ? 0 : p.scenario == 2 ? (r.thr + CH - 1) / CH : p.scenario == 3 && r.thr > 0 ? (p.K + CH - 1) / CH : 0);
   return r;
 }
 __device__ __forceinline__ int64_t range_start(int64_t total, int R, int r) {
@@ -448,6 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   if (warp == kCoordWarp) {
     // ================================================= coordinator
     int b = ms.start_b, cached = -1;
+    Req r = request(p, min(b, p.B - 1));
     int64_t prefix = ms.start_prefix, t = t0;
     uint32_t c = 0, uc = 0;
     bool ok = true, lead_cut = false;
@@ -470,10 +485,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       return true;
     };
     while (ok && t < t1 && b < p.B) {
-      const Req r = request(p, b);
       if (t >= prefix + r.all()) {
         prefix += r.all();
-        ++b;
+        if (++b < p.B) r = request(p, b);
         continue;
       }
       const int64_t in = t - prefix;
@@ -556,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       } else {
         ++uc;
         const int part = whole ? 0 : (t == t0 ? TF_PART0 : TF_PART1);
-        const int wrows = r.ctx - r.lo + min(i1, r.n - 1) + 1;  // up to the unit's last drafted token
+        const int wrows = r.ctx - r.lo + min(i1, r.used - 1) + 1;  // up to the unit's last drafted token
         for (int k = k0; k < k1 && ok; ++k) {
           int fl = part | (k == k0 ? TF_FIRST : 0) | (k == k1 - 1 ? TF_LAST : 0), row0, n;
           if (k < r.wtiles) {
@@ -802,6 +816,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         if (et == 64 && p.lse) p.lse[r] = 0.f;
       }
     }
+    if (p.layout == SAS_LAYOUT_BSND)  // and rows of padding alone
+      for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+        const Req r = request(p, b);
+        const int64_t lo = (int64_t)r.base * p.H + min((int64_t)r.units * (p.scenario == 3 ? p.H : UR), (int64_t)r.slots * p.H);
+        const int et = tid - 32 * kEpiWarp0, n = (int)((int64_t)(r.base + r.slots) * p.H - lo);
+        for (int64_t i = et; i < (int64_t)n * (D / 8); i += 32 * kEpiWarps) reinterpret_cast<uint4*>(p.out + lo * (D * 2))[i] = make_uint4(0, 0, 0, 0);
+        for (int i = et; p.lse && i < n; i += 32 * kEpiWarps) p.lse[lo + i] = 0.f;
+      }
     for (uint32_t u = 0;; ++u) {
       if (!__all_sync(0xffffffffu, WAIT(B_FIN + (u & 1), u >> 1, 30))) break;
       const Fin& fin = ms.fin[u & 1];
