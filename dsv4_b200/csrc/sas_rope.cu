@@ -22,6 +22,13 @@
 // and the cache slot, and keeps kStages - 1 rows in flight with cp.async into
 // its own shared memory, which costs no registers, so that enough warps fit.
 // A call with few rows takes short runs, so that they spread over all SMs.
+//
+// Measured (the memory's rate is that of a plain copy, 6.5 TB/s): forward of
+// 16384 tokens x 65 heads x 512 335 us, backward of 8192 tokens 249 us, both at
+// that rate; append of 512 tokens with their 128 query heads 28 us (4.9 TB/s), of
+// 16384 rows alone 15 us (2.5 TB/s), its backward of 8192 rows 16 us (two
+// launches), 64 tokens forward 4.1 us. The calls of under 50 MB are bound by their
+// start and end: launch, first loads, partial sums of the weight gradient.
 #include "sas_common.cuh"
 
 namespace {
@@ -264,7 +271,7 @@ __host__ __device__ constexpr int bwd_blocks(int nv) { return nv > 2 ? 1 : 2; }
 __host__ __device__ constexpr int stages_of(int nv) { return nv > 2 ? 2 : 4; }  // rows of a warp in flight or in work
 
 // The shares of a warp: every warps-th one, so that the GPU's reads stay close
-// together (353 against 363 us for 16384 x 64 x 512), or `most` neighbours where
+// together (3% faster for 16384 x 64 x 512), or `most` neighbours where
 // shares need the token's slot, whose request and page then stay.
 struct Walk {
   uint32_t first, end, step;

@@ -41,6 +41,18 @@
 //   14     coordinator: walks the range and the trees, works out which rows each
 //          token sees and publishes tiles (the pair's two take the same steps);
 //   15-18  copy Q and K, 19-22 V.
+// What bounds it. The products of a tile take 2500 cycles, a tile 5900 (dense: 16
+// trees of 32 tokens x 128 heads over 65k-262k, 165 us, 762 TFLOP/s, 46% of the
+// library's bf16 rate; tensor pipe 38-40% busy): the softmax warps' serial chain
+// per tile, some 400 instructions and 12 round trips to shared memory and barriers
+// between the scores and P. Then the ends of units (window of 127, 64 trees of 16
+// x 64 heads: two tiles a unit, the second nearly empty, 71 us), and about 20 us
+// that a call of any size takes (a single tile through every role and the joining
+// kernel, 22 us). Neither memory (top-k, 64 x 8 x 128 heads, 512 of them: 126 us,
+// 2.1 TB/s, DRAM 31% busy) nor L2 (30%) is near its rate.
+// Measured and left out: registers moved between warps (setmaxnreg, slower), P
+// before the row's maximum is known and again if it moved (3% slower), output rows
+// stored from registers (slower).
 // Copies: Q, and the rows of pages of a multiple of 64, are TMA boxes of 64 rows
 // x 64 columns issued by one thread (window tiles then begin at a multiple of 64,
 // so that 64 rows never leave a page). Top-k rows and other pages take cp.async,
@@ -69,8 +81,8 @@ constexpr int QSLAB = MR * 128;   // 64 columns of Q, or of P
 constexpr int kSmWarps = 8, kEpiWarp0 = 8, kEpiWarps = 4, kQkWarp = 12, kPvWarp = 13, kCoordWarp = 14, kKWarp0 = 15, kVWarp0 = 19,
               kLoadWarps = 4;
 constexpr int kThreads = 32 * 23;
-constexpr int kRing = 5;          // tiles the coordinator may be ahead
-constexpr int kUnitSlots = 7;     // > kRing + 1: no slot is rewritten while a published tile names it
+constexpr int kRing = 7;          // tiles the coordinator may be ahead (5: up to 1% slower)
+constexpr int kUnitSlots = 9;     // > kRing + 1: no slot is rewritten while a published tile names it
 constexpr uint32_t TM_O = 0, TM_S = 384, TM_COLS = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMove = 8.f;      // log2 units the running maximum may lag
@@ -668,7 +680,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             sas::mbar_arrive(&bars[full + h]);
           } else if (is_v) {  // 256 bytes of two rows at a time
             const uint32_t dst = v_base + (2 * h + ((lane >> 3) & 1)) * VSLAB + lw * 32 * 128;
-#pragma unroll 8
+#pragma unroll 8  // 2 or 16: 6% slower
             for (int i = 0; i < cnt; i += 2) {
               const int ii = i + (lane >> 4), ri = __shfl_sync(0xffffffffu, row, ii);
               cp16(dst + ii * 128 + (((lane & 7) ^ (ii & 7)) << 4), src + (int64_t)max(ri, 0) * (D * 2) + h * 256 - (lane >> 4) * 256, ri >= 0 ? 16u : 0u);
@@ -902,7 +914,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     const uint32_t tl = tmem + ((uint32_t)(warp & 3) << 21);
     const bool flip = p.scale_log2 < 0.f;
     const float scale = flip ? -p.scale_log2 : p.scale_log2;
-    uint32_t c = 0, n = 0, u = 0, sy = 0;
+    uint32_t c = 0, n = 0, u = 0;
     float m = -INFINITY, l = 0.f;
     int tok = 0;
     bool used = false, ok = true;
@@ -992,13 +1004,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         red[part][row] = mx;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
-        // P with the reference as it stands, while the row's other maxima come;
-        // again if one of the warp's rows moves
-        const uint64_t sc2 = twice(scale);
+        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), n, 32));
+        if (!ok) break;
+        mx = fmaxf(fmaxf(red[0][row], red[1][row]), fmaxf(red[2][row], red[3][row])) * scale;
+        float fac = 1.f;
+        if (mx > m + kMove || (m == -INFINITY && mx > m)) {
+          fac = sas::ex2(m - mx);
+          m = mx;
+          l *= fac;
+        }
+        const uint64_t sc2 = twice(scale), rf2 = twice(m == -INFINITY ? 0.f : -m);
         uint32_t w[16];
-        float sum = 0.f;
-        auto exps = [&]() {
-          const uint64_t rf2 = twice(m == -INFINITY ? 0.f : -m);
+        {
           uint64_t la[2] = {0, 0};
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1008,28 +1025,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             w[i] = pack2<DT>(a, b);
           }
           la[0] = add2(la[0], la[1]);
-          sum = lo(la[0]) + hi(la[0]);
-        };
-        bool redo = t.flags & TF_FIRST;
-        float fac = 1.f;
-#pragma unroll 1
-        for (int pass = redo; pass < 2; ++pass) {
-          if (pass == 1) {
-            ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), sy, 32));
-            if (!ok) break;
-            ++sy;
-            mx = fmaxf(fmaxf(red[0][row], red[1][row]), fmaxf(red[2][row], red[3][row])) * scale;
-            if (mx > m + kMove || (m == -INFINITY && mx > m)) {
-              fac = sas::ex2(m - mx);
-              m = mx;
-              l *= fac;
-            }
-            if (!redo && !__any_sync(0xffffffffu, fac != 1.f)) break;
-          }
-          exps();
+          l += lo(la[0]) + hi(la[0]);
         }
-        if (!ok) break;
-        l += sum;
         // the product before this tile's is complete, and P may be written
         ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, 40));
         if (!ok) break;

@@ -202,6 +202,10 @@ CASES = {
     "long runs of unused slots": dict(lens=[24] * 6, ctx=[30, 300, 128, 2, 400, 260], H=64, layout="BSND", scenario=2,
                                       trees=[[-1] + [-2] * 23, [-2] * 20 + [-1, -1, 20, -2], [-2] * 24, [-1, 0] + [-2] * 22,
                                              [-2] * 23 + [-1], [-1] * 24]),
+    "padding past 64 slots": dict(lens=[150] * 3, ctx=[70, 300, 9], H=8, layout="BSND", scenario=2,
+                                  trees=[[-1] + [-2] * 149, [-2] * 140 + [-1, 140, -2, 141] + [-2] * 6, [-2] * 150]),
+    "padded top-k": dict(lens=[20] * 3, ctx=[70, 300, 900], H=136, layout="BSND", scenario=3, K=70,
+                         trees=[[-2] * 20, [-1, 0] + [-2] * 18, [-2] * 9 + [-1] + [-2] * 10]),
     "ragged bsnd": dict(lens=[2, 5, 0], ctx=[30, 300, 128], H=16, layout="BSND", scenario=2, ratio=16),
     "dense": dict(lens=[5, 1], ctx=[1000, 37], H=64, scenario=2),
     "dense odd": dict(lens=[3, 8, 2], ctx=[515, 4099, 3], H=24, scenario=2, ratio=4, bs=48, dt=FP, win=63),

@@ -14,7 +14,7 @@ import random
 
 import pytest
 
-RING, UNIT_SLOTS = 5, 7
+RING, UNIT_SLOTS = 7, 9
 FIRST, LAST, END, ZERO = 1, 2, 4, 8
 
 
