@@ -118,9 +118,9 @@ struct Fin {  // a finished unit, from the softmax warps to the epilogue
   int64_t qrow;
   int nrows, roff, part;     // part: -1, or the CTA's partial
 };
-struct Cut {  // the piece a CTA's range starts with, when it is not its unit's first
-  int64_t ustart, uend, qrow;
-  int nrows, cut;
+struct Cut {  // of a CTA: the cut unit that it joins, if its range is the first to start inside one
+  int64_t qrow;
+  int nrows, cut, first, last;  // pieces: partial `first` of the range before, then partial 0 of the ranges up to `last`
 };
 struct Misc {
   uint64_t bars[B_COUNT + (B_COUNT & 1)];
@@ -163,7 +163,6 @@ struct TreeParams {
   float scale_log2;
   float* part;  // [CTAs][2] pieces
   Cut* cuts;    // [CTAs]
-  int64_t* total;
   int32_t* status;
   CUtensorMap map_kv[2], map_q;
 };
@@ -457,7 +456,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       at += a;
     }
   }
-  if (blockIdx.x == 0 && tid == 0) *p.total = total;
   sas::pdl_launch_dependents();
   sas::tc_fence_before();
   __syncthreads();
@@ -572,7 +570,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const bool whole = k0 == 0 && k1 == r.tiles;
       if (k0 > 0 && any) {
         lead_cut = true;
-        if (lane == 0) p.cuts[blockIdx.x] = Cut{ustart, uend, (int64_t)r.base * p.H + row_in, nrows, 1};
+        const int64_t before = range_start(total, R, rank - 1);
+        int last = rank;  // the range that holds the unit's last tile
+        while (last + 1 < R && range_start(total, R, last + 1) < uend) ++last;
+        // the first piece is partial 0 of its CTA if the unit starts with that range
+        if (lane == 0)
+          p.cuts[blockIdx.x] = Cut{(int64_t)r.base * p.H + row_in, nrows, before <= ustart, before == ustart ? 0 : 1, last};
       }
       if (!any) {
         if (k0 == 0) {
@@ -598,7 +601,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       }
       t = ustart + k1;
     }
-    if (lane == 0 && !lead_cut && rank < R) p.cuts[blockIdx.x].cut = 0;
+    if (lane == 0 && !lead_cut) p.cuts[blockIdx.x].cut = 0;
     if (ok) publish(TF_END, 0, 0, 0);
   } else if (warp >= kKWarp0) {
     // ================================================= loaders
@@ -1082,51 +1085,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
 #undef WAIT_PAIR
 }
 
-// Joins the pieces of a cut unit, in order. The block of CTA c does so when c's
-// range is the first to start inside the unit; blockIdx.y takes 64 columns.
+// Joins the pieces of a cut unit, in order: the block of CTA c does so when c's
+// range is the first to start inside the unit; blockIdx.y takes 64 columns. A
+// thread has 16 columns of a row. All it needs of the two pieces that there are at
+// least is asked for at once: the kernel is a chain of L2 latencies (with loads as
+// their values were needed it took 5 to 12 us).
 template <int DT>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(256, 4) tree_combine_kernel(const __grid_constant__ TreeParams p) {
   sas::pdl_wait();
   const int ctas = 2 * p.G;  // of a range
   const int g = blockIdx.x % ctas, rank = blockIdx.x / ctas;
-  const int64_t total = *p.total;
-  const int R = ranges(total, p.R);
-  if (rank == 0 || rank >= R) return;
   const Cut c = p.cuts[blockIdx.x];
   if (!c.cut) return;
-  const int64_t before = range_start(total, R, rank - 1);
-  if (before > c.ustart) return;  // an earlier range starts inside the unit
-  int last = rank;                // the range that holds the unit's last tile
-  while (last + 1 < R && range_start(total, R, last + 1) < c.uend) ++last;
-  // the first piece is partial 0 of its CTA if the unit starts with the range
-  const int first_slot = before == c.ustart ? 0 : 1;
-  auto piece = [&](int r) { return p.part + ((size_t)(r * ctas + g) * 2 + (r == rank - 1 ? first_slot : 0)) * kPieceFloats; };
-  // 64 of the 512 columns: thread = row, 16 of them
+  auto piece = [&](int r) { return p.part + ((size_t)(r * ctas + g) * 2 + (r == rank - 1 ? c.first : 0)) * kPieceFloats; };
   __shared__ __align__(16) uint8_t tile[MR * 128];
   const int row = threadIdx.x & 63, c4 = (threadIdx.x >> 6) * 4, d4 = blockIdx.y * 16 + c4;
   if (row < c.nrows) {
+    struct Part { float m, l; float4 v[4]; };
+    auto load = [&](int r) {
+      const float* q = piece(r);
+      Part x;
+      x.m = q[MR * D + row], x.l = q[MR * D + MR + row];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = reinterpret_cast<const float4*>(q)[(size_t)(d4 + i) * MR + row];
+      return x;
+    };
+    const Part a = load(rank - 1), b = load(rank);
     const float sink = __ldg(p.sinks + (c.qrow + row) % p.H) * kLog2e;
-    float top = sink;
-    for (int r = rank - 1; r <= last; ++r) top = fmaxf(top, piece(r)[MR * D + row]);
+    float top = fmaxf(sink, fmaxf(a.m, b.m));
+    for (int r = rank + 1; r <= c.last; ++r) top = fmaxf(top, piece(r)[MR * D + row]);
     const float base = top == -INFINITY ? 0.f : top;
     float den = exp2f(sink - base);
     float o[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = 0.f;
-    bool used = true;
-    for (int r = rank - 1; r <= last; ++r) {
-      const float* q = piece(r);
-      const float w = exp2f(q[MR * D + row] - base), l = q[MR * D + MR + row];
-      if (l < 0.f) used = false;
-      den = fmaf(l, w, den);
+    const bool used = !(a.l < 0.f);
+    auto add = [&](const Part& x) {
+      const float w = exp2f(x.m - base);
+      den = fmaf(x.l, w, den);
       if (w != 0.f)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 v = reinterpret_cast<const float4*>(q)[(size_t)(d4 + i) * MR + row];
-          o[4 * i] = fmaf(v.x, w, o[4 * i]), o[4 * i + 1] = fmaf(v.y, w, o[4 * i + 1]);
-          o[4 * i + 2] = fmaf(v.z, w, o[4 * i + 2]), o[4 * i + 3] = fmaf(v.w, w, o[4 * i + 3]);
+          o[4 * i] = fmaf(x.v[i].x, w, o[4 * i]), o[4 * i + 1] = fmaf(x.v[i].y, w, o[4 * i + 1]);
+          o[4 * i + 2] = fmaf(x.v[i].z, w, o[4 * i + 2]), o[4 * i + 3] = fmaf(x.v[i].w, w, o[4 * i + 3]);
         }
-    }
+    };
+    add(a);
+    add(b);
+    for (int r = rank + 1; r <= c.last; ++r) add(load(r));
     const float k = used && (top != -INFINITY || den != den) ? 1.f / den : 0.f;
     uint32_t v[8];
 #pragma unroll
@@ -1142,7 +1148,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
         *reinterpret_cast<const uint4*>(tile + (i >> 3) * 128 + (i & 7) * 16);
 }
 
-size_t workspace_bytes(int sms) { return 256 + (size_t)sms * (sizeof(Cut) + 2 * kPieceFloats * sizeof(float)); }
+size_t workspace_bytes(int sms) { return (size_t)sms * (sizeof(Cut) + 2 * kPieceFloats * sizeof(float)); }
 
 template <int DT>
 int launch(const TreeParams& p, cudaStream_t st) {
@@ -1234,9 +1240,8 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.nblk[0] = ori_nblk, p.nblk[1] = cmp_nblk;
   p.idx = idx, p.sinks = sinks, p.scale_log2 = softmax_scale == 0.f ? 1e-30f : softmax_scale * kLog2e;  // 0 * -inf would not mask
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.total = reinterpret_cast<int64_t*>(ws);
-  p.part = reinterpret_cast<float*>(ws + 256);
-  p.cuts = reinterpret_cast<Cut*>(ws + 256 + (size_t)num_sms * 2 * kPieceFloats * sizeof(float));
+  p.part = reinterpret_cast<float*>(ws);
+  p.cuts = reinterpret_cast<Cut*>(ws + (size_t)num_sms * 2 * kPieceFloats * sizeof(float));
   p.status = status;
   if ((int64_t)T * H >= (1ll << 31)) return SAS_ERR_UNSUPPORTED;
   if (!make_map(&p.map_q, q, dtype, 0, (int64_t)T * H)) return SAS_ERR_CUDA;
