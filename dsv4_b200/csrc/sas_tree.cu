@@ -48,7 +48,7 @@
 // between the scores and P. Then the ends of units (window of 127, 64 trees of 16
 // x 64 heads: two tiles a unit, the second nearly empty, 71 us), and about 20 us
 // that a call of any size takes (a single tile through every role and the joining
-// kernel, 22 us). Neither memory (top-k, 64 x 8 x 128 heads, 512 of them: 126 us,
+// kernel, 21 us). Neither memory (top-k, 64 x 8 x 128 heads, 512 of them: 126 us,
 // 2.1 TB/s, DRAM 31% busy) nor L2 (30%) is near its rate.
 // Measured and left out: registers moved between warps (setmaxnreg, slower), P
 // before the row's maximum is known and again if it moved (3% slower), output rows
@@ -1088,8 +1088,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
 // Joins the pieces of a cut unit, in order: the block of CTA c does so when c's
 // range is the first to start inside the unit; blockIdx.y takes 64 columns. A
 // thread has 16 columns of a row. All it needs of the two pieces that there are at
-// least is asked for at once: the kernel is a chain of L2 latencies (with loads as
-// their values were needed it took 5 to 12 us).
+// least is asked for at once. For one tile a pair it is a chain of latencies, 3.5 us
+// (5 with loads as their values were needed); 38 MB of pieces take 11 us, with 16 to
+// 128 columns a block and 3 to 8 blocks an SM alike.
 template <int DT>
 __global__ void __launch_bounds__(256, 4) tree_combine_kernel(const __grid_constant__ TreeParams p) {
   sas::pdl_wait();
