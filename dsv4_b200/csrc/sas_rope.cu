@@ -551,6 +551,8 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
       float rstd = 1.f, mean = 0.f;  // mean of g * xhat
       if (norm) {
         rstd = rsqrtf(group_sum<G>(ss.lo() + ss.hi()) * invD + p.eps);
+        // lanes past the last head hold zeros: their xh has to be zero with eps = 0 too
+        if (HW > 1 && i * HW + sub >= hn) rstd = 0.f;
         mean = rstd * group_sum<G>(gx.lo() + gx.hi()) * invD;
       }
       const F2 r2(rstd, rstd), m2(-mean, -mean);

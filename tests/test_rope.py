@@ -485,3 +485,23 @@ def test_append_past_32_bit_offsets(gpu):
     close(torch.cat([pool[-1, 127:], pool[-7, :2]]), want)
     dkv, _ = append_shared_kv_backward(pool, kv, **args)
     assert dkv.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,H,Hk", [(64, 1, 0), (64, 3, 1), (64, 6, 5), (128, 1, 1), (128, 7, 3)])
+def test_weight_gradient_without_eps(gpu, D, H, Hk):
+    """Heads that do not fill a warp's lanes, with eps 0: the lanes without a row add nothing."""
+    from dsv4_b200 import head_norm_rope_backward
+
+    close.dtype = torch.bfloat16
+    q, k, cos, sin, pos, qw, kw, (dq, dk) = _case(9, H, Hk, D, 32, True, True, torch.bfloat16, seed=5)
+    c, s = _rows(cos, sin, pos)
+    dev = _cuda(dq, q, dk, k, pos, cos, sin, qw, kw)
+    got = head_norm_rope_backward(*dev[:4], positions=dev[4], cos=dev[5], sin=dev[6], q_weight=dev[7], k_weight=dev[8], eps=0.0)
+    for gx, gw, x, w, dy in ((got[0], got[2], q, qw, dq), (got[1], got[3], k, kw, dk)):
+        if x is None:
+            continue
+        dx, dw, mag = formula_bwd(dy, x, w, c, s, True, eps=0.0)
+        rstd = 1 / x.double().pow(2).mean(-1, keepdim=True).sqrt()
+        close(gx, dx, dx.abs().amax(-1, keepdim=True) + 4 * rstd * dy.double().abs().amax(-1, keepdim=True))
+        assert ((gw.double().cpu() - dw).abs() <= F32 * mag).all()
