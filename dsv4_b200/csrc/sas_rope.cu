@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
   uint32_t unit = walk.first, share_in = 0, row_in = 0;
   int left = 0, hleft = 0;
   bool have = true;
+  uint32_t skip = 0;  // append, a token being one row: of the last 32 rows asked for, those that were not written
   const uint8_t *x = nullptr, *dy = nullptr;
   const int64_t xs = rs.x_hs * 2 * HW, ds = rs.dy_hs * 2 * HW, ys = rs.y_hs * 2 * HW;
   auto issue = [&]() {
@@ -482,7 +483,10 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
       int slot = -1;
       int64_t row = 0;
       x = rs.x + ((int64_t)t * rs.x_ts + (int64_t)(h0 + sub) * rs.x_hs) * 2 + gl * 16;
-      if (p.pool) row = slots.row(p, t, lane, slot, true);
+      if (p.pool) {
+        row = slots.row(p, t, lane, slot, true);
+        skip = (skip & ~(1u << (row_in & 31))) | ((row < 0 ? 1u : 0u) << (row_in & 31));
+      }
       have = row >= 0;
       dy = (p.pool ? p.pool + (have ? row : 0) * p.D * 2 : rs.dy + (int64_t)t * rs.dy_ts * 2) +
            (int64_t)(h0 + sub) * rs.dy_hs * 2 + gl * 16;
@@ -526,6 +530,16 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
     const uint32_t t = u / per;
     const int h0 = (int)(u - t * per) * rs.run * HW, hn = min(rs.H - h0, rs.run * HW);
     uint8_t* y = rs.y + ((int64_t)t * rs.y_ts + (int64_t)(h0 + sub) * rs.y_hs) * 2 + gl * 16;
+    if (p.pool && ((skip >> (row_out & 31)) & 1u)) {  // zero whatever the raw row holds, and no part of the weight's gradient
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (on[j] && sub == 0) *reinterpret_cast<uint4*>(y + G * 16 * j) = make_uint4(0, 0, 0, 0);
+      issue();
+      cp_wait<S - 1>();  // its copies are done before the stage is filled again
+      __syncwarp();
+      ++row_out;
+      continue;
+    }
     for (int i = 0; i * HW < hn; ++i) {
       issue();
       cp_wait<S - 1>();

@@ -505,3 +505,81 @@ def test_weight_gradient_without_eps(gpu, D, H, Hk):
         rstd = 1 / x.double().pow(2).mean(-1, keepdim=True).sqrt()
         close(gx, dx, dx.abs().amax(-1, keepdim=True) + 4 * rstd * dy.double().abs().amax(-1, keepdim=True))
         assert ((gw.double().cpu() - dw).abs() <= F32 * mag).all()
+
+
+def _unwritten():
+    """(name, layout, cu_seqlens_q, tokens, table, seqused_kv, tokens without a row) of appends of 12 tokens."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    full = [[0, 1], [2, 3], [4, 5]]
+    return [
+        ("padding of BSND", "BSND", i32([0, 4, 5, 8]), (3, 4), i32(full), i32([9, 3, 8]), [5, 6, 7, 11]),
+        ("an empty request of BSND", "BSND", i32([0, 4, 4, 6]), (3, 4), i32(full), i32([4, 0, 8]), [4, 5, 6, 7, 10, 11]),
+        ("after the last request of TND", "TND", i32([0, 4, 5, 9]), (12,), i32(full), i32([9, 3, 8]), [9, 10, 11]),
+        ("without a page", "TND", i32([0, 4, 8, 12]), (12,), i32([[0, 1], [-1, 3], [4, -1]]), i32([9, 10, 9]), [4, 5, 11]),
+        ("before slot 0", "TND", i32([0, 4, 8, 12]), (12,), i32(full), i32([9, 2, 8]), [4, 5]),
+    ]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 192, 512])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 0.0])
+@pytest.mark.parametrize("which", range(5))
+def test_append_backward_of_unwritten_rows(gpu, which, bad, D):
+    """They get zero and leave the weight's gradient alone, whatever they hold; zeros with eps 0 too."""
+    from dsv4_b200 import append_shared_kv_backward
+
+    close.dtype = torch.bfloat16
+    name, layout, cu, lead, table, used, unwritten = _unwritten()[which]
+    eps = 1e-6 if bad else 0.0
+    g = torch.Generator().manual_seed(7)
+    kv = (2 * torch.randn((12, 1, D), generator=g)).bfloat16()
+    kv[unwritten] = bad
+    w = 1 + 0.1 * torch.randn(D, generator=g)
+    dpool = torch.randn((6, 8, 1, D), generator=g).bfloat16()
+    dkv, dw = append_shared_kv_backward(dpool.cuda(), kv.view(*lead, 1, D).cuda(), ori_block_table=table, seqused_kv=used,
+                                        cu_seqlens_q=cu, layout_q=layout, weight=w.cuda(), eps=eps)
+    dkv = dkv.cpu().view(12, 1, D)
+    assert not dkv[unwritten].any(), name
+    written = [t for t in range(12) if t not in unwritten]
+    cu, used, table, S = cu.tolist(), used.tolist(), table.tolist(), lead[-1]
+    rows = []
+    for t in written:
+        b = t // S if layout == "BSND" else max(b for b in range(3) if cu[b] <= t)
+        p = used[b] - (cu[b + 1] - cu[b]) + t - (b * S if layout == "BSND" else cu[b])
+        rows.append(table[b][p // 8] * 8 + p % 8)
+    dy, x = dpool.view(-1, 1, D)[rows], kv[written]
+    dx, rw, mag = formula_bwd(dy, x, w, None, None, True, eps=eps)
+    rstd = 1 / (x.double().pow(2).mean(-1, keepdim=True) + eps).sqrt()
+    close(dkv[written], dx, dx.abs().amax(-1, keepdim=True) + 4 * rstd * dy.double().abs().amax(-1, keepdim=True))
+    assert ((dw.double().cpu() - rw).abs() <= F32 * mag).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 512])
+def test_append_backward_of_long_padding(gpu, D):
+    """Warps that walk over several tokens, runs of padding that hold NaN among them."""
+    from dsv4_b200 import append_shared_kv_backward
+
+    close.dtype = torch.bfloat16
+    B, S, bs = 40, 400, 16
+    r = np.random.default_rng(3)
+    lens = [0, S, 1, *(int(x) for x in r.integers(0, S + 1, B - 3))]
+    pool, table, used, rows, _ = _paged(lens, [int(x) for x in r.integers(0, 40, B)], bs, D, torch.bfloat16, 3)
+    held = torch.zeros(B, S, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        held[b, :n] = True
+    held = held.view(-1)
+    g = torch.Generator().manual_seed(5)
+    kv = torch.randn((B * S, 1, D), generator=g).bfloat16()
+    kv[~held] = float("nan")
+    w = 1 + 0.1 * torch.randn(D, generator=g)
+    dkv, dw = append_shared_kv_backward(pool.cuda(), kv.view(B, S, 1, D).cuda(), ori_block_table=table.cuda(),
+                                        seqused_kv=used.cuda(), layout_q="BSND", weight=w.cuda(),
+                                        cu_seqlens_q=torch.tensor([0, *np.cumsum(lens)], dtype=torch.int32).cuda())
+    dkv = dkv.cpu().view(-1, 1, D)
+    assert not dkv[~held].any()
+    dy, x = pool.view(-1, 1, D)[rows], kv[held]
+    dx, rw, mag = formula_bwd(dy, x, w, None, None, True)
+    rstd = 1 / (x.double().pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+    close(dkv[held], dx, dx.abs().amax(-1, keepdim=True) + 4 * rstd * dy.double().abs().amax(-1, keepdim=True))
+    assert ((dw.double().cpu() - rw).abs() <= F32 * mag).all()
