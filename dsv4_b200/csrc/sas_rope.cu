@@ -503,8 +503,8 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const bool there = (HW == 1 || sub < hleft) && on[j];
-        if (FULL && HW == 1) cp16(dst + j * 512, x + G * 16 * j);
-        else cp16_if(dst + j * 512, there ? x + G * 16 * j : rs.x, there);
+        if (!(FULL && HW == 1)) cp16_if(dst + j * 512, there ? x + G * 16 * j : rs.x, there && norm);
+        else if (norm) cp16(dst + j * 512, x + G * 16 * j);
         cp16_if(dst + (NV + j) * 512, there ? dy + G * 16 * j : rs.x, there && have);
       }
       x += xs;
@@ -515,6 +515,11 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_blocks(NV)) rope_bwd_kernel(c
     }
     cp_commit();
   };
+  // without the norm the gradient is the rotation's and has no part of x, which is not
+  // read: zeros stand in its place
+  if (!norm)
+    for (int i = 0; i < S * NV; ++i)
+      *reinterpret_cast<uint4*>(mine + (i / NV) * STAGE + (i % NV) * 512 + lane * 16) = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue();
   const bool hasw = rs.w != nullptr;

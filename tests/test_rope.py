@@ -583,3 +583,23 @@ def test_append_backward_of_long_padding(gpu, D):
     rstd = 1 / (x.double().pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
     close(dkv[held], dx, dx.abs().amax(-1, keepdim=True) + 4 * rstd * dy.double().abs().amax(-1, keepdim=True))
     assert ((dw.double().cpu() - rw).abs() <= F32 * mag).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("bad", [None, float("nan"), float("inf")])
+def test_backward_without_norm(gpu, bad, inter, inverse):
+    """The rotation's transpose of the gradient alone: the inputs, finite or not, have no part in it."""
+    from dsv4_b200 import head_norm_rope_backward
+
+    close.dtype = torch.float16
+    q, k, cos, sin, pos, _, _, (dq, dk) = _case(11, 5, 2, 128, 64, False, False, torch.float16, seed=6)
+    c, s = _rows(cos, sin, pos)
+    if bad is not None:
+        q[3], k[5, 1, ::3] = bad, -bad
+    dev = _cuda(dq, q, dk, k, pos, cos, sin)
+    got = head_norm_rope_backward(*dev[:4], positions=dev[4], cos=dev[5], sin=dev[6], norm=False, inverse=inverse, interleaved=inter)
+    for gx, dy in ((got[0], dq), (got[1], dk)):
+        close(gx, definition(dy, None, c, s, inter, norm=False, inverse=not inverse))
+    assert got[2] is None and got[3] is None
