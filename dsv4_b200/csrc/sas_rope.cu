@@ -199,16 +199,15 @@ struct Slots {
 };
 
 // Row of the cos / sin tables of token t. A position outside the tables takes
-// the nearest row and is recorded.
+// the nearest row and is recorded, in an append by the token's K=V row and only
+// if that has a slot: padding, of which nothing is written to the cache, may have any.
 __device__ __forceinline__ int table_row(const RopeParams& p, int t, int slot, int lane) {
   int64_t pos = slot;
   if (p.positions)
     pos = (p.flags & SAS_ROPE_POS64) ? __ldg(static_cast<const long long*>(p.positions) + t)
                                : __ldg(static_cast<const int32_t*>(p.positions) + t);
-  else if (slot < 0)
-    return 0;  // a token without a slot: nothing of it is written to the cache
   if (pos < 0 || pos >= p.P) {
-    if (lane == 0 && p.status) atomicCAS(p.status, 0, SAS_ERR_BAD_POSITION);
+    if (lane == 0 && p.status && !(p.pool && slot < 0)) atomicCAS(p.status, 0, SAS_ERR_BAD_POSITION);
     pos = pos < 0 ? 0 : p.P - 1;
   }
   return (int)pos;

@@ -380,7 +380,9 @@ def append_shared_kv(
     ``[B, S, H, D]``) the same launch does ``head_norm_rope`` of the tokens'
     queries. A token whose block-table entry is negative is not written; an
     entry outside the table or the pool is not written and recorded in the
-    status word.
+    status word. What padding (slots of BSND past ``cu_seqlens_q``'s count,
+    tokens after the last request) holds in ``kv`` and ``positions`` does not
+    matter.
     """
     p = _Paged(kv, ori_kv, ori_block_table, seqused_kv, cu_seqlens_q, layout_q)
     D, T = p.D, p.T

@@ -283,8 +283,8 @@ int sas_head_norm_rope_bwd(const void* dq_out, int64_t dqo_ts, int64_t dqo_hs, c
  * too unless `positions` gives one for every token (drafted trees). A token
  * whose block-table entry is negative, or that lies before slot 0, is not
  * written; one past the table's width or the pool is not written and recorded
- * as SAS_ERR_BAD_BLOCK_ENTRY. kv [T, D] has token stride kv_ts. No two tokens
- * may share a slot. Layouts as in the attention: TND with cu_seqlens_q [B+1],
+ * as SAS_ERR_BAD_BLOCK_ENTRY. A token without a slot (padding) may have any
+ * position. kv [T, D] has token stride kv_ts. No two tokens may share a slot. Layouts as in the attention: TND with cu_seqlens_q [B+1],
  * BSND with S tokens per request (cu_seqlens_q then optional).
  * The backward gathers dy from the cache's gradient (I/O type, shaped like
  * the pool) and writes dense dkv [T, D]; tokens that were not written get 0.

@@ -603,3 +603,43 @@ def test_backward_without_norm(gpu, bad, inter, inverse):
     for gx, dy in ((got[0], dq), (got[1], dk)):
         close(gx, definition(dy, None, c, s, inter, norm=False, inverse=not inverse))
     assert got[2] is None and got[3] is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [0, 6])
+@pytest.mark.parametrize("which", [0, 1, 2, 4])
+def test_positions_of_tokens_without_a_slot(gpu, which, H):
+    """Positions outside the tables are recorded for tokens with a slot alone: padding may hold anything. The nearest row
+    of the tables turns it."""
+    from dsv4_b200 import append_shared_kv, append_shared_kv_backward, device_status, reset_device_status
+
+    D = 64
+    name, layout, cu, lead, table, used, unwritten = _unwritten()[which]
+    g = torch.Generator().manual_seed(8)
+    kv = torch.randn((12, 1, D), generator=g).bfloat16().view(*lead, 1, D).cuda()
+    q = torch.randn((12, H, D), generator=g).bfloat16().view(*lead, H, D).cuda() if H else None
+    pool = torch.randn((6, 8, 1, D), generator=g).bfloat16()
+    cos, sin = tables(16, 32, "cuda")
+    pos = torch.arange(12) + 2
+    first = pos.clone()
+    first[unwritten] = 0
+    args = dict(ori_block_table=table, seqused_kv=used, cu_seqlens_q=cu, layout_q=layout, cos=cos, sin=sin)
+
+    def both(positions):
+        args["positions"] = positions.view(lead).cuda()
+        r = append_shared_kv(kv, pool.cuda(), q=q, **args)
+        return (*(r if H else (r,)), append_shared_kv_backward(pool.cuda(), kv, **args)[0])
+
+    for x in (-1, 16, 1 << 40, -(1 << 40)):
+        fill = torch.where(first == 0, torch.tensor(x), first)
+        got, want = both(fill), both(fill.clamp(0, 15))
+        assert device_status() == 0, name
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    written = next(t for t in range(12) if t not in unwritten)
+    fill = first.clone()
+    fill[written] = 16
+    args["positions"] = fill.view(lead).cuda()
+    for call in (lambda: append_shared_kv(kv, pool.cuda(), q=q, **args), lambda: append_shared_kv_backward(pool.cuda(), kv, **args)):
+        call()
+        assert device_status() == 8
+        reset_device_status()
