@@ -127,6 +127,7 @@ struct Misc {
   sas::CtaCtl ctl;
   uint32_t tmem;
   int start_b;
+  uint32_t sent[2][2];   // loaders of K, of V: tiles whose halves were asked for
   int64_t start_prefix, total;
   int64_t wsum[kThreads / 32];
   uint32_t vmask[3][4];  // rows of tile n that are there, in n % 3
@@ -613,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     // K: lanes 0-15 have the warp's K rows, 16-31 the same of the other CTA's half (for the mask)
     const int my_row = is_v ? lw * 32 + lane : (lane < 16 ? side : side ^ 1) * 64 + lw * 16 + (lane & 15);
     const int full = is_v ? B_VFULL : B_KFULL, empty = is_v ? B_VEMPTY : B_KEMPTY;
-    uint32_t c = 0, n = 0, q = 0;
+    uint32_t c = 0, n = 0, q = 0, n0 = 0;  // n, n0: tiles whose second, first half this warp has arrived for
     // pool row of position pos of a request's table, -1: none
     auto lookup = [&](int f, int b, int pos) -> int {
       const int col = pos / p.bs[f];
@@ -698,6 +699,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             }
             cp_arrive(&bars[full + h]);
           }
+          if (h == 0) ++n0;
           if (!is_v && h == 0 && lane == 0) {
             // Tile n - 3's mask was here. It is done with: K came free after the
             // scores of n - 1, for which those of n - 3 had been read, after it.
@@ -718,12 +720,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       if (lane == 0) sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
       ++c;
     }
-    // no copy may still be landing when the CTA leaves
+    // No copy may still be landing when the CTA leaves. After a wait that gave up, the
+    // warp that issues the boxes may have asked for a half (the first one alone, too) for
+    // which another warp has not arrived: each half's last phase then lacks that arrival
+    // and never ends. It is one phase at most, as the phase before it had to be complete.
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (lw == 0) {
-      for (int h = 0; n > 0 && h < 2; ++h) sas::mbar_wait_drain(&bars[full + h], (n - 1) & 1, SAS_WAIT_LIMIT_NS);
-      if (!is_v && q > 0) sas::mbar_wait_drain(&bars[B_QFULL], (q - 1) & 1, SAS_WAIT_LIMIT_NS);
+    if (lw == 0 && lane == 0) ms.sent[is_v][0] = n0, ms.sent[is_v][1] = n;
+    sas::named_bar_sync(1 + is_v, 32 * kLoadWarps);
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t sent = ms.sent[is_v][h];
+      if ((h ? n : n0) < sent) sas::mbar_arrive(&bars[full + h]);
+      if (lw == 0 && sent > 0) sas::mbar_wait_drain(&bars[full + h], (sent - 1) & 1, SAS_WAIT_LIMIT_NS);
     }
+    if (lw == 0 && !is_v && q > 0) sas::mbar_wait_drain(&bars[B_QFULL], (q - 1) & 1, SAS_WAIT_LIMIT_NS);
   } else if (warp == kQkWarp || warp == kPvWarp) {
     // ================================================= MMA issuers
     if (elect_one()) {

@@ -273,3 +273,142 @@ def test_no_sequence_blocks(seed):
 def test_edges(units):
     for seed in range(25):
         Model(units, seed).run()
+
+
+class TxBar(Bar):
+    """A barrier whose phase also waits for the bytes (here: boxes) that it was told to expect."""
+
+    def __init__(self, count):
+        super().__init__(count)
+        self.tx = 0
+
+    def arrive(self, n=1):
+        self.left -= n
+        assert self.left >= 0, "an arrival too many"
+        self.check()
+
+    def expect(self):
+        self.tx += 1
+
+    def landed(self):
+        self.tx -= 1
+        self.check()
+
+    def check(self):
+        if self.left == 0 and self.tx == 0:
+            self.left, self.phase = self.count, self.phase + 1
+
+
+class Loaders:
+    """The four warps that copy K (or V) in halves, a reader, and a wait that gives up at some moment. Afterwards every
+    wait may give up, or pass if its phase is complete. By boxes, warp 0 alone copies; else each warp its rows, which
+    arrive by themselves once they have landed. ``rule`` is how a warp leaves."""
+
+    def __init__(self, tiles, seed, rule):
+        self.rng, self.tiles, self.rule = random.Random(seed), tiles, rule
+        self.full, self.empty = [TxBar(4), TxBar(4)], [Bar(1), Bar(1)]
+        self.flying, self.abort, self.sent, self.left = [], False, None, 0
+        self.blocked = False
+
+    def wait(self, bar, parity):
+        while True:
+            if bar.done(parity) and (not self.abort or self.rng.random() < 0.5):
+                return True
+            if self.abort and self.rng.random() < 0.5:
+                return bar.done(parity)
+            yield
+
+    def loader(self, w):
+        done = [0, 0]
+        for n, boxes in enumerate(self.tiles):
+            for h in (0, 1):
+                if not (yield from self.wait(self.empty[h], n + 1)):
+                    yield from self.leave(w, done)
+                    return
+                if boxes:
+                    if w == 0:
+                        self.full[h].expect()
+                        self.flying.append((w, self.full[h].landed))
+                    yield
+                    self.full[h].arrive()
+                else:
+                    self.flying.append((w, self.full[h].arrive))
+                done[h] += 1
+                yield
+        yield from self.leave(w, done)
+
+    def leave(self, w, done):
+        while any(x == w and land.__name__ == "arrive" for x, land in self.flying):  # cp.async.wait_all
+            yield
+        if self.rule == "whole tiles":
+            if w == 0 and done[1]:
+                for h in (0, 1):
+                    yield from self.drain(self.full[h], done[1] - 1)
+        else:
+            if w == 0:
+                self.sent = list(done)
+            self.left += 1
+            while self.left < 4:
+                yield
+            for h in (0, 1):
+                if done[h] < self.sent[h]:
+                    assert done[h] == self.sent[h] - 1
+                    self.full[h].arrive()
+                if w == 0 and self.sent[h]:
+                    yield from self.drain(self.full[h], self.sent[h] - 1)
+        if w == 0:
+            assert not self.flying, "a copy is still landing"
+
+    def drain(self, bar, parity):
+        while not bar.done(parity):
+            self.blocked = not self.flying and self.left == 4
+            assert not self.blocked or self.idle < 200, "the drain waits for a phase that cannot end"
+            yield
+
+    def reader(self):
+        for n in range(len(self.tiles)):
+            for h in (0, 1):
+                if not (yield from self.wait(self.full[h], n)):
+                    return
+                yield
+                self.empty[h].arrive()
+
+    def run(self):
+        roles = [self.loader(w) for w in range(4)] + [self.reader()]
+        at, step, self.idle = self.rng.randrange(1, 60), 0, 0
+        while roles or self.flying:
+            step += 1
+            self.abort = self.abort or step >= at
+            self.idle = 0 if self.flying else self.idle + 1
+            if self.flying and (not roles or self.rng.random() < 0.1):
+                self.flying.pop(self.rng.randrange(len(self.flying)))[1]()
+            else:
+                g = self.rng.choice(roles)
+                try:
+                    next(g)
+                except StopIteration:
+                    roles.remove(g)
+            assert step < 100000, "blocked"
+
+
+def _loaders(seed, rule):
+    r = random.Random(seed)
+    boxes = r.choice([True, True, None])
+    Loaders([r.random() < 0.5 if boxes is None else boxes for _ in range(r.randrange(1, 12))], seed, rule).run()
+
+
+@pytest.mark.parametrize("block", range(8))
+def test_no_copy_lands_after_a_wait_gave_up(block):
+    for seed in range(250 * block, 250 * block + 250):
+        _loaders(seed, "halves sent")
+
+
+def test_counting_whole_tiles_leaves_copies_in_flight():
+    """The model tells: a warp that waits for its last whole tile leaves while a first half is landing."""
+    found = 0
+    for seed in range(400):
+        try:
+            _loaders(seed, "whole tiles")
+        except AssertionError as e:
+            found += "still landing" in str(e)
+    assert found > 0
