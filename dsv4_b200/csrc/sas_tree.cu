@@ -814,11 +814,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         sas::mbar_arrive(&bars[B_CEMPTY + c % kRing]);
         ++c;
       }
-      // nothing may still run on TMEM or shared memory when the pair leaves
-      if (!side) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sas::smem_u32(&bars[B_DRAIN + pv])) : "memory");
-        sas::mbar_wait_drain(&bars[B_DRAIN + pv], 0, SAS_WAIT_LIMIT_NS);
-      }
+      // nothing may still run on TMEM or shared memory when the pair leaves, nor a commit
+      // still be on its way to the second CTA's barriers, which so waits for the last one
+      if (!side) commit2(&bars[B_DRAIN + pv]);
+      sas::mbar_wait_drain(&bars[B_DRAIN + pv], 0, SAS_WAIT_LIMIT_NS);
     }
     __syncwarp();
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {

@@ -412,3 +412,46 @@ def test_counting_whole_tiles_leaves_copies_in_flight():
         except AssertionError as e:
             found += "still landing" in str(e)
     assert found > 0
+
+
+class LateCommits(Model):
+    """Commits that reach the second CTA's barriers later than the first's, each issuer's in order. ``both``: the second
+    CTA's issuers wait for the first's last one, as the kernel's do."""
+
+    def __init__(self, units, seed, both):
+        super().__init__(units, seed)
+        self.both, self.late = both, {"qk": [], "pv": []}
+        for cta in self.cta:
+            cta.b.update(drainqk=Bar(1), drainpv=Bar(1))
+
+    def commit(self, q, *bars):
+        def done():
+            for x in bars:
+                self.cta[0].b[x].arrive()
+                self.late[q].append(self.cta[1].b[x].arrive)
+                self.copies.append(lambda: self.late[q].pop(0)())
+        self.mmas[q].append(done)
+
+    def issuer(self, q, side, role):
+        yield from role(side)
+        if side == 0:
+            self.commit(q, f"drain{q}")
+        if side == 0 or self.both:
+            yield f"drain{q}", 0
+
+    def scores(self, side):
+        return self.issuer("qk", side, super().scores)
+
+    def products(self, side):
+        return self.issuer("pv", side, super().products)
+
+
+@pytest.mark.parametrize("both", [True, False])
+def test_no_commit_arrives_after_the_pair_left(both):
+    found = 0
+    for seed in range(300):
+        r = random.Random(seed)
+        m = LateCommits([r.choice([0, 1, 1, 2, 3]) for _ in range(r.randrange(1, 6))], seed, both)
+        m.run()
+        found += bool(m.late["qk"] or m.late["pv"])
+    assert found == 0 if both else found > 0
