@@ -315,6 +315,10 @@ __host__ __device__ __forceinline__ int64_t floordiv64(int64_t a, int64_t b) {
 // <= 0 restores the default), defined with the scheduler.
 void set_sched_scan_cap(long long cap);
 
+// The limit of every bounded wait (SAS_OPT_WAIT_LIMIT_NS), defined with the
+// options.
+unsigned long long wait_limit_ns();
+
 inline bool select_device_of(const void* ptr) {
   cudaPointerAttributes a;
   if (cudaPointerGetAttributes(&a, ptr) != cudaSuccess) {

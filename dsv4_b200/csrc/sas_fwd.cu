@@ -2001,6 +2001,8 @@ WsLayout ws_layout(int T, int H, int num_sms) {
 
 }  // namespace
 
+unsigned long long sas::wait_limit_ns() { return g_wait_ns; }
+
 extern "C" int sas_version(void) { return 1; }
 
 extern "C" int sas_fwd_set_option(int32_t option, double value, void* ptr) {

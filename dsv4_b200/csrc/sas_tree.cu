@@ -101,6 +101,16 @@ enum Bar { B_KFULL = 0, B_VFULL = 2, B_QFULL = 4, B_XK, B_XV = B_XK + 2, B_XQ = 
            B_QEMPTY = B_VEMPTY + 2, B_MASK, B_SFULL = B_MASK + 3, B_SEMPTY = B_SFULL + 2, B_PREADY = B_SEMPTY + 2, B_OFULL, B_OEMPTY,
            B_FIN = B_OEMPTY + 3, B_SSYNC = B_FIN + 2, B_CFULL = B_SSYNC + 2, B_CEMPTY = B_CFULL + kRing, B_DRAIN = B_CEMPTY + kRing, B_COUNT = B_DRAIN + 2 };
 
+// Waits, as the status word names them: SAS_ERR_TIMEOUT_BASE + id, those of the forward
+// below 20. One for each place that waits; both halves and both buffers of a thing share it.
+enum WaitId : int {
+  W_UNIT_SLOT = 20, W_PUBLISH, W_LOAD_TILE, W_Q_FREE, W_K_FREE, W_V_FREE,         // coordinator, loaders
+  W_MMA_TILE, W_PASS_Q, W_PASS_K, W_PASS_V,                                       // issuers, second CTA
+  W_PV_P, W_PV_O, W_PV_V, W_PV_XV, W_QK_Q, W_QK_XQ, W_QK_S, W_QK_K, W_QK_XK,      // issuers, first CTA
+  W_EPI_UNIT, W_EPI_O,                                                            // epilogue
+  W_SM_TILE, W_SM_END, W_SM_MASK, W_SM_S, W_SM_V_FREE, W_SM_V, W_SM_MAX, W_SM_P   // softmax
+};
+
 enum TileFlag : int {
   TF_FIRST = 1, TF_LAST = 2, TF_END = 4, TF_ZERO = 8,  // ZERO: no token of the unit is in use, its output is zero
   TF_CMP = 16, TF_TOPK = 32, TF_PART0 = 64, TF_PART1 = 128  // PARTn: the piece goes to the CTA's partial n
@@ -165,6 +175,7 @@ struct TreeParams {
   float* part;  // [CTAs][2] pieces
   Cut* cuts;    // [CTAs]
   int32_t* status;
+  unsigned long long wait_ns;  // limit of every wait
   CUtensorMap map_kv[2], map_q;
 };
 
@@ -279,12 +290,25 @@ __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-template <bool PAIR>
+// A limit that a blocking try could oversleep is met by polls, as there, in a variant
+// of the kernel (POLL): a choice at each wait costs 2 to 5% of every call.
+__device__ __forceinline__ bool poll_pair(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(sas::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+template <bool PAIR, bool POLL>
 __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
   const uint64_t t0 = sas::globaltimer(), lim = ctl->limit_ns;
   for (uint32_t n = 1;; ++n) {
-    if (try_wait<PAIR>(bar, parity)) return true;
-    if ((n & 63u) == 0) {
+    if (!POLL ? try_wait<PAIR>(bar, parity) : PAIR ? poll_pair(bar, parity) : sas::mbar_test_wait(bar, parity)) return true;
+    if (POLL || (n & 63u) == 0) {
       if (ctl->abort) return false;
       if (sas::globaltimer() - t0 > lim) {
         ctl->abort = 1;
@@ -294,9 +318,9 @@ __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile sa
     }
   }
 }
-template <bool PAIR>
+template <bool PAIR, bool POLL>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile sas::CtaCtl* ctl, int* status, int where) {
-  return try_wait<PAIR>(bar, parity) || wait_on<PAIR>(bar, parity, ctl, status, where);
+  return (!POLL && try_wait<PAIR>(bar, parity)) || wait_on<PAIR, POLL>(bar, parity, ctl, status, where);
 }
 // One lane of the warp. The compiler takes the branch on it as a single
 // thread's and keeps MMA operands in uniform registers: 32 products are issued
@@ -389,7 +413,7 @@ __device__ __noinline__ void clear_rows(uint32_t v_base, int row0) {
   }
 }
 
-template <int DT>
+template <int DT, bool POLL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_attn_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -416,7 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     init(B_DRAIN, 2, 1);
     sas::fence_mbar_init();
     ms.ctl.abort = 0;
-    ms.ctl.limit_ns = SAS_WAIT_LIMIT_NS;
+    ms.ctl.limit_ns = p.wait_ns;
     ms.start_b = p.B;
     ms.start_prefix = 0;
   }
@@ -466,9 +490,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
   volatile sas::CtaCtl* ctl = &ms.ctl;
   const uint32_t q_base = sas::smem_u32(smem + OFF_Q), k_base = sas::smem_u32(smem + OFF_K),
                  v_base = sas::smem_u32(smem + OFF_V), p_base = sas::smem_u32(smem + OFF_P);
-  // (the waits' ids, added to SAS_ERR_TIMEOUT_BASE in the status word, are 20 and up)
-#define WAIT(bar, par, id) wait<false>(&bars[bar], (par)&1, ctl, p.status, id)
-#define WAIT_PAIR(bar, par, id) wait<true>(&bars[bar], (par)&1, ctl, p.status, id)
+#define WAIT(bar, par, id) wait<false, POLL>(&bars[bar], (par)&1, ctl, p.status, id)
+#define WAIT_PAIR(bar, par, id) wait<true, POLL>(&bars[bar], (par)&1, ctl, p.status, id)
 
   if (warp == kCoordWarp) {
     // ================================================= coordinator
@@ -479,7 +502,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     bool ok = true, lead_cut = false;
     auto publish = [&](int flags, int row0, int nrows, int us) -> bool {
       const int slot = c % kRing;
-      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + slot, (c / kRing) ^ 1u, 20))) return false;
+      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + slot, (c / kRing) ^ 1u, W_PUBLISH))) return false;
       if (!(flags & (TF_END | TF_ZERO))) {  // lane: token, 32 rows
         const Unit& un = ms.units[us];
         const int tok = lane >> 2, pos = un.pos[tok];
@@ -528,7 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       const int mine = nrows ? (int)(row_in / H) - i0 : 0;  // this CTA's first token among the unit's
       // the slot's last readers are done: see kUnitSlots; the ring wait below
       // orders this warp's writes after their reads
-      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + c % kRing, (c / kRing) ^ 1u, 20))) break;
+      if (!__all_sync(0xffffffffu, WAIT(B_CEMPTY + c % kRing, (c / kRing) ^ 1u, W_UNIT_SLOT))) break;
       int pos = -1;
       if (lane < kMaxUnitTok) {
         const int slot = lane - mine;
@@ -623,7 +646,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
       return blk < 0 || blk >= p.nblk[f] ? -1 : blk * p.bs[f] + (pos - col * p.bs[f]);
     };
     while (true) {
-      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 21))) break;
+      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, W_LOAD_TILE))) break;
       const Tile t = ms.ring[c % kRing];
       if (t.flags & TF_END) break;
       if (!(t.flags & TF_ZERO)) {
@@ -639,7 +662,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           if (!(t.flags & TF_TOPK) || (pos >= 0 && pos < u.thr)) row = lookup(f, u.b, pos);
         }
         if (!is_v && lw == 0 && (t.flags & TF_FIRST)) {
-          if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, 22))) break;
+          if (!__all_sync(0xffffffffu, WAIT(B_QEMPTY, q ^ 1u, W_Q_FREE))) break;
           const int q0 = (int)u.qrow;
           if (elect_one()) {  // rows past the unit's are other rows, or zero past the last: nobody reads their results
             sas::mbar_arrive_expect_tx(&bars[B_QFULL], 8 * QSLAB);
@@ -662,7 +685,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         bool ok = true;
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          ok = __all_sync(0xffffffffu, WAIT(empty + h, n ^ 1u, is_v ? 23 : 34));
+          ok = __all_sync(0xffffffffu, WAIT(empty + h, n ^ 1u, is_v ? W_V_FREE : W_K_FREE));
           if (!ok) break;
           if (tma) {
             if (lw == 0 && elect_one()) {
@@ -738,36 +761,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     if (elect_one()) {
       constexpr int fmt = DT == SAS_DTYPE_BF16 ? 1 : 0;
       const bool pv = warp == kPvWarp;
-      auto pass_on = [&](int bar, int to, uint32_t par) -> bool {
-        if (!WAIT(bar, par, 26)) return false;
+      auto pass_on = [&](int bar, int to, uint32_t par, int id) -> bool {
+        if (!WAIT(bar, par, id)) return false;
         sas::fence_proxy_async_smem();  // cp.async writes -> tensor core reads
         arrive_first(&bars[to]);
         return true;
       };
       uint32_t c = 0, n = 0, u = 0;
       while (true) {
-        if (!WAIT(B_CFULL + c % kRing, c / kRing, 24)) break;
+        if (!WAIT(B_CFULL + c % kRing, c / kRing, W_MMA_TILE)) break;
         const Tile t = ms.ring[c % kRing];
         if (t.flags & TF_END) break;
         if (!(t.flags & TF_ZERO)) {
           if (side) {
             if (pv) {
-              if (!pass_on(B_VFULL, B_XV, n) || !pass_on(B_VFULL + 1, B_XV + 1, n)) break;
+              if (!pass_on(B_VFULL, B_XV, n, W_PASS_V) || !pass_on(B_VFULL + 1, B_XV + 1, n, W_PASS_V)) break;
             } else {
-              if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++)) break;
-              if (!pass_on(B_KFULL, B_XK, n) || !pass_on(B_KFULL + 1, B_XK + 1, n)) break;
+              if ((t.flags & TF_FIRST) && !pass_on(B_QFULL, B_XQ, u++, W_PASS_Q)) break;
+              if (!pass_on(B_KFULL, B_XK, n, W_PASS_K) || !pass_on(B_KFULL + 1, B_XK + 1, n, W_PASS_K)) break;
             }
           } else if (pv) {  // O += P V
             constexpr uint32_t id_o = sas::umma_idesc_f16(fmt, UR, 256, 0, 1);
             const uint64_t p_desc = sas::umma_desc_sw128(p_base, 16, 1024), v_desc = sas::umma_desc_sw128(v_base, VSLAB, 1024);
-            if (!WAIT_PAIR(B_PREADY, n, 27)) break;
+            if (!WAIT_PAIR(B_PREADY, n, W_PV_P)) break;
             const int steps = max(1, (t.nrows + 15) / 16);
             bool ok = true;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               const uint32_t oh = 2 * u + h, place = oh % 3;
-              ok = (!(t.flags & TF_FIRST) || WAIT_PAIR(B_OEMPTY + place, (oh / 3) ^ 1u, 28)) && WAIT(B_VFULL + h, n, 35) &&
-                   WAIT_PAIR(B_XV + h, n, 36);
+              ok = (!(t.flags & TF_FIRST) || WAIT_PAIR(B_OEMPTY + place, (oh / 3) ^ 1u, W_PV_O)) && WAIT(B_VFULL + h, n, W_PV_V) &&
+                   WAIT_PAIR(B_XV + h, n, W_PV_XV);
               if (!ok) break;
               sas::fence_proxy_async_smem();
               sas::tc_fence_after();
@@ -786,14 +809,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
             constexpr uint32_t id_s = sas::umma_idesc_f16(fmt, UR, CH, 0, 0);
             const uint64_t q_desc = sas::umma_desc_sw128(q_base, 16, 1024), k_desc = sas::umma_desc_sw128(k_base, 16, 1024);
             if (t.flags & TF_FIRST) {
-              if (!WAIT(B_QFULL, u, 25) || !WAIT_PAIR(B_XQ, u, 37)) break;
+              if (!WAIT(B_QFULL, u, W_QK_Q) || !WAIT_PAIR(B_XQ, u, W_QK_XQ)) break;
               ++u;
             }
-            if (!WAIT_PAIR(B_SEMPTY + (n & 1), (n >> 1) ^ 1u, 41)) break;
+            if (!WAIT_PAIR(B_SEMPTY + (n & 1), (n >> 1) ^ 1u, W_QK_S)) break;
             bool ok = true;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
-              ok = WAIT(B_KFULL + h, n, 26) && WAIT_PAIR(B_XK + h, n, 38);
+              ok = WAIT(B_KFULL + h, n, W_QK_K) && WAIT_PAIR(B_XK + h, n, W_QK_XK);
               if (!ok) break;
               sas::fence_proxy_async_smem();
               sas::tc_fence_after();
@@ -848,7 +871,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         for (int i = et; p.lse && i < n; i += 32 * kEpiWarps) p.lse[lo + i] = 0.f;
       }
     for (uint32_t u = 0;; ++u) {
-      if (!__all_sync(0xffffffffu, WAIT(B_FIN + (u & 1), u >> 1, 30))) break;
+      if (!__all_sync(0xffffffffu, WAIT(B_FIN + (u & 1), u >> 1, W_EPI_UNIT))) break;
       const Fin& fin = ms.fin[u & 1];
       const int nrows = fin.nrows, part = fin.part;
       if (nrows < 0) break;  // the range is done
@@ -871,7 +894,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         k = !used || (m == -INFINITY && l == 0.f) ? 0.f : a / den;
         if (row < nrows && ch == 0 && p.lse) p.lse[qrow + row] = used ? (top + log2f(den)) * kLn2 : 0.f;
       }
-      if (!__all_sync(0xffffffffu, WAIT(B_OFULL, u, 33))) break;
+      if (!__all_sync(0xffffffffu, WAIT(B_OFULL, u, W_EPI_O))) break;
       sas::tc_fence_after();
       const int nr = min(32, nrows - (ew & 1) * 32);
       uint8_t* out = p.out + (qrow + (ew & 1) * 32) * (D * 2) + ch * 512 + (lane & 3) * 16;
@@ -930,11 +953,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
     int tok = 0;
     bool used = false, ok = true;
     while (ok) {
-      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, 29))) break;
+      if (!__all_sync(0xffffffffu, WAIT(B_CFULL + c % kRing, c / kRing, W_SM_TILE))) break;
       const Tile t = ms.ring[c % kRing];
       if (t.flags & TF_END) {
         // the epilogue ends too; its place is free as below
-        if (n > 0 && !__all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, 40))) break;
+        if (n > 0 && !__all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, W_SM_END))) break;
         ms.fin[u & 1].nrows = -1;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_FIN + (u & 1)]);
@@ -954,14 +977,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         }
         uint32_t see = used ? ms.vis[c % kRing][tok][part] : 0u;
         // rows of the tile that are there, and those that this row's token sees
-        ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, 30));
+        ok = __all_sync(0xffffffffu, WAIT(B_MASK + n % 3, n / 3, W_SM_MASK));
         if (!ok) break;
         // rows of the buffers that hold values that some row does not see: stale ones
         // too, past the last of a page's
         const bool check = !(t.flags & TF_CMP) || t.nrows < CH;
         const uint32_t there32 = ms.vmask[n % 3][part];
         see &= there32;
-        ok = __all_sync(0xffffffffu, WAIT(B_SFULL + (n & 1), n >> 1, 31));
+        ok = __all_sync(0xffffffffu, WAIT(B_SFULL + (n & 1), n >> 1, W_SM_S));
         if (!ok) break;
         sas::tc_fence_after();
         uint64_t s[16];
@@ -992,8 +1015,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
               // The tile's V has to be there, after the one before it was done
               // with (its copy alone could be two phases back). A wait that fails
               // shows at the next one.
-              if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY + 1, n ^ 1u, 40) &&
-                  WAIT(B_VFULL, n, 39) && WAIT(B_VFULL + 1, n, 39)) {
+              if (!(fabsf(zs) < INFINITY) && WAIT(B_VEMPTY + 1, n ^ 1u, W_SM_V_FREE) &&
+                  WAIT(B_VFULL, n, W_SM_V) && WAIT(B_VFULL + 1, n, W_SM_V)) {
                 clear_rows<DT>(v_base, 32 * part);
                 // a score of -inf weighs nothing, but its row is not finite
 #pragma unroll
@@ -1015,7 +1038,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
         red[part][row] = mx;
         __syncwarp();
         if (lane == 0) sas::mbar_arrive(&bars[B_SSYNC + (warp & 1)]);
-        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), n, 32));
+        ok = __all_sync(0xffffffffu, WAIT(B_SSYNC + (warp & 1), n, W_SM_MAX));
         if (!ok) break;
         mx = fmaxf(fmaxf(red[0][row], red[1][row]), fmaxf(red[2][row], red[3][row])) * scale;
         float fac = 1.f;
@@ -1039,7 +1062,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) tree_at
           l += lo(la[0]) + hi(la[0]);
         }
         // the product before this tile's is complete, and P may be written
-        ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, 40));
+        ok = __all_sync(0xffffffffu, WAIT(B_VEMPTY + 1, n ^ 1u, W_SM_P));
         if (!ok) break;
         sas::tc_fence_after();
         if (!(t.flags & TF_FIRST) && __any_sync(0xffffffffu, fac != 1.f)) {
@@ -1161,7 +1184,7 @@ size_t workspace_bytes(int sms) { return (size_t)sms * (sizeof(Cut) + 2 * kPiece
 
 template <int DT>
 int launch(const TreeParams& p, cudaStream_t st) {
-  auto kern = tree_attn_kernel<DT>;
+  auto kern = p.wait_ns < sas::kPollLimitNs ? tree_attn_kernel<DT, true> : tree_attn_kernel<DT, false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return SAS_ERR_CUDA;
   kern<<<2 * p.R * p.G, kThreads, SMEM_BYTES, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return SAS_ERR_CUDA;
@@ -1252,6 +1275,7 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
   p.part = reinterpret_cast<float*>(ws);
   p.cuts = reinterpret_cast<Cut*>(ws + (size_t)num_sms * 2 * kPieceFloats * sizeof(float));
   p.status = status;
+  p.wait_ns = sas::wait_limit_ns();
   if ((int64_t)T * H >= (1ll << 31)) return SAS_ERR_UNSUPPORTED;
   if (!make_map(&p.map_q, q, dtype, 0, (int64_t)T * H)) return SAS_ERR_CUDA;
   for (int f = 0; f < (scenario == 2 ? 2 : 1); ++f) {

@@ -352,7 +352,7 @@ int sas_tree_attn_sharedkv(const void* q, int32_t T, int32_t H, int32_t head_dim
  *     its own running max, so such tokens meet the accuracy bounds and not the
  *     reference's rounding points. value < 0 restores the default.
  *   SAS_OPT_WAIT_LIMIT_NS (value): limit, in ns, of every bounded wait of
- *     the attention kernel for the next launches (0 restores the default of
+ *     the attention kernels (forward and drafted trees) for the next launches (0 restores the default of
  *     2 s). A wait that runs out records SAS_ERR_TIMEOUT_BASE + its id in the
  *     status word; the CTA drains the copies and MMAs it has in flight, frees
  *     its TMEM and returns, so the context stays usable. Small values exist to

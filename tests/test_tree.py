@@ -435,3 +435,27 @@ def test_no_tokens(gpu):
                            tree_parents=c.parents[:0].cuda(), sinks=c.sinks.cuda(), softmax_scale=c.scale,
                            cu_seqlens_q=torch.zeros(2, dtype=torch.int32).cuda())
     assert o.shape == (0, 16, D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["dense", "top-k odd", "padded", "whole context", "top-k 3 head groups", "many requests", "one long request"])
+@pytest.mark.parametrize("limit", [1000, 20000])
+def test_waits_that_run_out(gpu, name, limit):
+    """A limit that real waits miss: the call returns with the id of one in the status word and the next call is right.
+    Pages in boxes and rows by themselves, one tile and many, cut units and whole ones."""
+    from dsv4_b200 import _lib, device_status, reset_device_status
+
+    set_limit = lambda ns: _lib.check(_lib.lib().sas_fwd_set_option(_lib.OPT_WAIT_LIMIT_NS, float(ns), None), "option")  # noqa: E731
+    c = Case(**CASES[name])
+    for _ in range(3):
+        try:
+            set_limit(limit)
+            c.call()
+            torch.cuda.synchronize()
+        finally:
+            set_limit(0)
+        status = device_status()
+        assert status == 0 and limit > 1000 or _lib.STATUS_TIMEOUT_BASE + 20 <= status < _lib.STATUS_TIMEOUT_BASE + 49, status
+        reset_device_status()
+        c.check(*c.call())
+        assert device_status() == 0
