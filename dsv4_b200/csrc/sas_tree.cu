@@ -189,16 +189,19 @@ struct Req {
 };
 __device__ __noinline__ Req request(const TreeParams& p, int b) {
   Req r;
+  int n;  // tokens by cu_seqlens_q, from which the append and the decode count the slots, if q has fewer too
   if (p.layout == SAS_LAYOUT_TND) {
     const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
     r.base = min(max(c0, 0), p.T);
     r.n = r.slots = max(min(c1, p.T) - r.base, 0);
+    n = max(c1 - c0, 0);
   } else {
     r.base = b * p.S;
     r.slots = p.S;
-    r.n = p.cu ? min(max(__ldg(p.cu + b + 1) - __ldg(p.cu + b), 0), p.S) : p.S;
+    n = p.cu ? max(__ldg(p.cu + b + 1) - __ldg(p.cu + b), 0) : p.S;
+    r.n = min(n, p.S);
   }
-  r.ctx = __ldg(p.seqused + b) - r.n;
+  r.ctx = __ldg(p.seqused + b) - n;
   r.bad = r.n > kMaxTree || r.ctx < 0 || r.ctx > kMaxCtx;
   r.thr = p.scenario == 1 || r.bad ? 0 : r.ctx / p.ratio;
   r.used = r.n;

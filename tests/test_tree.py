@@ -459,3 +459,21 @@ def test_waits_that_run_out(gpu, name, limit):
         reset_device_status()
         c.check(*c.call())
         assert device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
+def test_more_tokens_named_than_there_are(gpu, layout):
+    """cu_seqlens_q that counts more tokens than q has: the slots are still those of the append and of the framework's
+    decode, seqused_kv - n on."""
+    from dsv4_b200 import append_shared_kv
+
+    c = Case([3], [40], H=8, layout=layout, trees=[[-1, 0, 1]])
+    cu, used = torch.tensor([0, 5], dtype=torch.int32).cuda(), torch.tensor([45], dtype=torch.int32).cuda()
+    c.check(*c.call(cu_seqlens_q=cu, seqused_kv=used))
+    rows = c.ori.view(-1, D)[[int(c.obt[0, p // c.bs]) * c.bs + p % c.bs for p in (40, 41, 42)]]
+    pool = torch.zeros_like(c.ori).cuda()
+    kv = rows.view(1, 3, 1, D) if layout == "BSND" else rows.view(3, 1, D)
+    append_shared_kv(kv.cuda(), pool, ori_block_table=c.obt.cuda(), seqused_kv=used, cu_seqlens_q=cu, layout_q=layout, norm=False)
+    assert torch.equal(pool.view(-1, D).cpu().nonzero()[:, 0].unique(),
+                       torch.tensor(sorted(int(c.obt[0, p // c.bs]) * c.bs + p % c.bs for p in (40, 41, 42))))
