@@ -14,7 +14,10 @@
 The reference has no counterpart: its op takes a rotated ``q`` and filled
 caches (``sparse_attn_sharedkv_tilelang/api.py:129-163``). Each call is one
 launch on the current stream (a backward with weight gradients two), without
-host synchronisation and without a CPU fallback. Shapes are ``ValueError``,
+host synchronisation and without a CPU fallback. Results carry no autograd
+graph, whatever requires gradients: ``head_norm_rope_train`` and the
+``*_backward`` calls are for training. What is written in place counts as an
+in-place change. Shapes are ``ValueError``,
 modes ``AssertionError``, as in ``sparse_attn_sharedkv``; what only the device
 can see (a bad block-table entry, a position outside the tables) goes to the
 status word (``check_device_status``).
@@ -202,6 +205,7 @@ def head_norm_rope(
     dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("head_norm_rope needs CUDA tensors (no CPU path)")
+    given = [t for t in (q_out, k_out) if t is not None]
     q_out, qo = _out_rows(q_out, q, "q_out")
     ka = ko = _NO_ROWS
     Hk = 0
@@ -218,6 +222,7 @@ def head_norm_rope(
             *qa, *qo, q.shape[-2], *ka, *ko, Hk, T, D, code, _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), P, R,
             _lib.ptr(qw), _lib.ptr(kw), float(eps), flags, _lib.state(dev).status.data_ptr(), _lib.raw_stream(dev))
         _raise(rc, "head_norm_rope", "sas_head_norm_rope_fwd")
+        _lib.written(given)
     return q_out if k is None else (q_out, k_out)
 
 
@@ -398,6 +403,7 @@ def append_shared_kv(
         raise RuntimeError("append_shared_kv needs CUDA tensors (no CPU path)")
     if ori_kv.device != dev or (q is not None and q.device != dev):
         raise ValueError("kv, ori_kv and q must be on one device")
+    given = [ori_kv] if q is None or q_out is None else [ori_kv, q_out]
     qa = qo = _NO_ROWS
     H = 0
     if q is not None:
@@ -415,6 +421,7 @@ def append_shared_kv(
             _lib.ptr(sin), P, R, _lib.ptr(w), _lib.ptr(qw), float(eps), flags, _lib.state(dev).status.data_ptr(),
             _lib.raw_stream(dev))
         _raise(rc, "append_shared_kv", "sas_append_sharedkv")
+        _lib.written(given)
     return ori_kv if q is None else (ori_kv, q_out)
 
 

@@ -6,7 +6,7 @@ a chain of new tokens: the same caches, tables, lengths, sinks and scenarios
 its ancestors instead of everything before it. The reference decodes chains
 only (``sparse_attn_sharedkv_tilelang/api.py:129-397``). No schedule is needed:
 the kernel cuts the work itself. The current stream, no host synchronisation,
-no CPU fallback; errors as in ``sparse_attn_sharedkv``.
+no CPU fallback, no autograd graph; errors as in ``sparse_attn_sharedkv``.
 """
 
 from __future__ import annotations
@@ -112,6 +112,7 @@ def tree_attn_sharedkv(
         _check_out("lse_out", lse_out, shape[:-1], torch.float32, dev)
     if dev.type != "cuda":
         raise RuntimeError("tree_attn_sharedkv needs q on a CUDA device (no CPU path)")
+    given = [t for t in (out, lse_out) if t is not None]
     q = _aligned(q, dev)
     if out is None:
         out = torch.empty_like(q)
@@ -141,6 +142,7 @@ def tree_attn_sharedkv(
         if rc in (1, 2):
             raise ValueError(f"tree_attn_sharedkv: {_lib.ERRORS[rc]}")
         _lib.check(rc, "sas_tree_attn_sharedkv")
+        _lib.written(given)
     return (out, lse_out) if return_softmax_lse else out
 
 

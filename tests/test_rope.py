@@ -643,3 +643,29 @@ def test_positions_of_tokens_without_a_slot(gpu, which, H):
         call()
         assert device_status() == 8
         reset_device_status()
+
+
+@pytest.mark.gpu
+def test_writes_are_seen_by_autograd(gpu):
+    """What a call writes in place of a tensor that a backward saved is an error of that backward, as of torch's own."""
+    from dsv4_b200 import append_shared_kv, head_norm_rope, sparse_attn_sharedkv_train
+
+    D, dt = 512, torch.bfloat16
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = torch.randn(2, 16, 1, D, device="cuda").to(dt)
+    q = torch.randn(3, 8, D, device="cuda").to(dt).requires_grad_()
+    table, used = i32(0, 1).view(1, 2), i32(20)
+    args = dict(ori_block_table=table, cu_seqlens_q=i32(0, 3))
+    out = sparse_attn_sharedkv_train(q, ori_kv=pool, sinks=torch.zeros(8, device="cuda"), softmax_scale=D ** -0.5,
+                                     seqused_kv=used, **args)
+    append_shared_kv(torch.randn(3, 1, D, device="cuda").to(dt), pool, seqused_kv=used, **args)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    x, y = (torch.randn(3, 8, D, device="cuda").to(dt) for _ in range(2))
+    before = [t._version for t in (x, y, pool)]
+    head_norm_rope(x, y, q_out=x, k_out=y)
+    append_shared_kv(y[:, :1], pool, seqused_kv=used, q=x, q_out=x, **args)
+    assert all(t._version > v for t, v in zip((x, y, pool), before)) and x._version == before[0] + 2
+    with torch.inference_mode():  # tensors without versions
+        z = torch.randn(3, 8, D, device="cuda").to(dt)
+        head_norm_rope(z, q_out=z)

@@ -477,3 +477,12 @@ def test_more_tokens_named_than_there_are(gpu, layout):
     append_shared_kv(kv.cuda(), pool, ori_block_table=c.obt.cuda(), seqused_kv=used, cu_seqlens_q=cu, layout_q=layout, norm=False)
     assert torch.equal(pool.view(-1, D).cpu().nonzero()[:, 0].unique(),
                        torch.tensor(sorted(int(c.obt[0, p // c.bs]) * c.bs + p % c.bs for p in (40, 41, 42))))
+
+
+@pytest.mark.gpu
+def test_writes_are_seen_by_autograd(gpu):
+    c = Case([2], [30], H=8)
+    out, lse = torch.empty_like(c.q, device="cuda"), torch.empty(c.T, 8, device="cuda")
+    before = out._version, lse._version
+    c.call(out=out, lse_out=lse)
+    assert out._version > before[0] and lse._version > before[1]
