@@ -29,6 +29,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -288,18 +289,24 @@ def head_norm_rope_backward(
 
 
 class HeadNormRope(torch.autograd.Function):
-    """``head_norm_rope`` as an autograd function of (q, k, q_weight, k_weight)."""
+    """``head_norm_rope`` as an autograd function of (q, k, q_weight, k_weight), differentiable once."""
+
+    TABLES = ("positions", "cos", "sin")
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, kwargs):
-        ctx.kwargs = kwargs
-        ctx.save_for_backward(q, k, q_weight, k_weight)
+        # positions, cos and sin are saved too, so that one changed before the backward is an error
+        held = [kwargs.get(name) for name in HeadNormRope.TABLES]
+        ctx.kwargs = {name: x for name, x in kwargs.items() if name not in HeadNormRope.TABLES}
+        ctx.save_for_backward(q, k, q_weight, k_weight, *held)
         return head_norm_rope(q, k, q_weight=q_weight, k_weight=k_weight, **kwargs)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out=None):
-        q, k, qw, kw = ctx.saved_tensors
-        dq, dk, dqw, dkw = head_norm_rope_backward(dq_out, q, dk_out, k, q_weight=qw, k_weight=kw, **ctx.kwargs)
+        q, k, qw, kw, *held = ctx.saved_tensors
+        dq, dk, dqw, dkw = head_norm_rope_backward(dq_out, q, dk_out, k, q_weight=qw, k_weight=kw,
+                                                   **dict(zip(HeadNormRope.TABLES, held)), **ctx.kwargs)
         return dq, dk, None if dqw is None else dqw.to(qw.dtype), None if dkw is None else dkw.to(kw.dtype), None
 
 

@@ -669,3 +669,60 @@ def test_writes_are_seen_by_autograd(gpu):
     with torch.inference_mode():  # tensors without versions
         z = torch.randn(3, 8, D, device="cuda").to(dt)
         head_norm_rope(z, q_out=z)
+
+
+def _on_cpu(monkeypatch):
+    """``head_norm_rope`` and its backward as far as autograd sees them: a result and gradients that know the positions."""
+    from dsv4_b200 import rope
+
+    calls = []
+
+    def fwd(q, k=None, **kw):
+        calls.append(("forward", kw))
+        return q * 1 if k is None else (q * 1, k * 1)
+
+    def bwd(dq_out, q, dk_out=None, k=None, **kw):
+        calls.append(("backward", kw))
+        s = 1 if kw.get("positions") is None else int(kw["positions"].sum())
+        w = [None if kw.get(n) is None else torch.ones_like(kw[n]) for n in ("q_weight", "k_weight")]
+        return dq_out * s, None if k is None else dk_out * s, *w
+
+    monkeypatch.setattr(rope, "head_norm_rope", fwd)
+    monkeypatch.setattr(rope, "head_norm_rope_backward", bwd)
+    return calls
+
+
+def test_train_keeps_its_positions(monkeypatch):
+    """A buffer of positions or angles that is refilled before the backward is an error, not the wrong gradient."""
+    from dsv4_b200 import head_norm_rope_train
+
+    calls = _on_cpu(monkeypatch)
+    cos, sin = tables(8, 32)
+    pos = torch.tensor([1, 2], dtype=torch.int32)
+    args = dict(positions=pos, cos=cos, sin=sin, eps=1e-5, interleaved=False)
+    q, k = (t.float().requires_grad_() for t in _qk())
+    w = torch.ones(64, requires_grad=True)
+    yq, yk = head_norm_rope_train(q, k, q_weight=w, **args)
+    torch.autograd.backward([yq, yk], [torch.ones_like(yq), torch.ones_like(yk)])
+    assert (q.grad == 3).all() and (k.grad == 3).all() and (w.grad == 1).all()
+    (_, f), (_, b) = calls
+    for n, x in args.items():
+        assert f[n] is x if not torch.is_tensor(x) else f[n].data_ptr() == x.data_ptr() == b[n].data_ptr()
+        assert torch.is_tensor(x) or b[n] == x
+    assert set(f) == set(b)
+    for held in (pos, cos, sin):
+        y = head_norm_rope_train(q, **args)
+        held += 1
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+    head_norm_rope_train(q).sum().backward()  # without positions
+
+
+def test_train_is_once_differentiable(monkeypatch):
+    from dsv4_b200 import head_norm_rope_train
+
+    _on_cpu(monkeypatch)
+    q = torch.ones(2, 4, 64, requires_grad=True)
+    g, = torch.autograd.grad(head_norm_rope_train(q).pow(2).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
