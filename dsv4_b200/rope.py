@@ -313,7 +313,8 @@ class HeadNormRope(torch.autograd.Function):
 def head_norm_rope_train(q, k=None, *, q_weight=None, k_weight=None, **kwargs):
     """``head_norm_rope`` with autograd: gradients flow to ``q``, ``k`` and the weights."""
     for name in ("q_out", "k_out"):
-        assert kwargs.get(name) is None, f"{name} cannot be given with autograd"
+        given = kwargs.pop(name, None)
+        assert given is None, f"{name} cannot be given with autograd"
     return HeadNormRope.apply(q, k, q_weight, k_weight, kwargs)
 
 

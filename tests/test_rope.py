@@ -726,3 +726,13 @@ def test_train_is_once_differentiable(monkeypatch):
     g, = torch.autograd.grad(head_norm_rope_train(q).pow(2).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_train_takes_absent_outputs(monkeypatch):
+    from dsv4_b200 import head_norm_rope_train
+
+    q = torch.ones(2, 4, 64, requires_grad=True)
+    calls = _on_cpu(monkeypatch)
+    head_norm_rope_train(q, q_out=None, k_out=None).sum().backward()
+    assert all("q_out" not in kw and "k_out" not in kw for _, kw in calls)  # the backward has no such arguments
+    assert (q.grad == 1).all()
