@@ -60,6 +60,19 @@ def _f32(t: Optional[torch.Tensor], dev: torch.device) -> Optional[torch.Tensor]
     return t if t.data_ptr() & 15 == 0 else t.clone()
 
 
+def _overlap(ts: int, T: int, hs: int, H: int, D: int) -> bool:
+    """Whether two of the rows at t * ts + h * hs, D values each, share one."""
+    if T == 1 or H == 1:
+        return T * H > 1 and (ts if T > 1 else hs) < D
+    (a, na), (b, nb) = sorted(((ts, T), (hs, H)))
+    if a < D:
+        return True
+    if b >= a * (na - 1) + D:
+        return False
+    # rows of the wider stride among those of the other: the two nearest ones
+    return any(abs(j * b - i * a) < D for j in range(1, nb) for i in (j * b // a, j * b // a + 1) if i < na)
+
+
 _NO_ROWS = (0, 0, 0)
 
 
@@ -81,6 +94,8 @@ def _rows(t: torch.Tensor, name: str, out: bool = False):
             raise ValueError(f"{name}: the token dims must have one stride") from None
         r = t.reshape(T, H, D)
     ts, hs = (r.stride(0) if T > 1 else H * D), (r.stride(1) if H > 1 else D)
+    if out and _overlap(ts, T, hs, H, D):
+        raise ValueError(f"the rows of {name} overlap")
     if r.stride(2) != 1 or r.data_ptr() & 15 or (ts | hs) & 7:
         if out:
             raise ValueError(f"{name} must have a contiguous last dim and 16-byte aligned rows")

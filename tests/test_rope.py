@@ -736,3 +736,35 @@ def test_train_takes_absent_outputs(monkeypatch):
     head_norm_rope_train(q, q_out=None, k_out=None).sum().backward()
     assert all("q_out" not in kw and "k_out" not in kw for _, kw in calls)  # the backward has no such arguments
     assert (q.grad == 1).all()
+
+
+def test_overlap_of_rows():
+    from dsv4_b200.rope import _overlap
+
+    g = np.random.default_rng(0)
+    for _ in range(3000):
+        T, H, D = (int(g.integers(1, n)) for n in (6, 6, 5))
+        ts, hs = (int(x) for x in g.integers(0, 20, 2))
+        at = np.arange(T)[:, None] * ts + np.arange(H) * hs
+        values = (at.reshape(-1, 1) + np.arange(D)).reshape(-1)
+        assert _overlap(ts, T, hs, H, D) == (len(np.unique(values)) < len(values)), (ts, T, hs, H, D)
+
+
+@pytest.mark.gpu
+def test_outputs_whose_rows_overlap_are_refused(gpu):
+    from dsv4_b200 import append_shared_kv, head_norm_rope
+
+    q = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    base = torch.zeros(3, 4, 64, device="cuda").bfloat16()
+    for out in (base[:1].expand(3, 4, 64), base[:, :1].expand(3, 4, 64), base.view(-1).as_strided((3, 4, 64), (256, 32, 1)),
+                base.view(-1).as_strided((3, 4, 64), (56, 192, 1)),
+                base.view(-1).as_strided((3, 4, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            head_norm_rope(q, q_out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        append_shared_kv(q[:, :1], base[:, :, None], ori_block_table=torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                         seqused_kv=torch.full((1,), 3, dtype=torch.int32, device="cuda"),
+                         cu_seqlens_q=torch.tensor([0, 3], dtype=torch.int32, device="cuda"), q=q, q_out=base[:1].expand(3, 4, 64))
+    assert not base.any()
+    by_head = torch.zeros(4, 3, 72, device="cuda").bfloat16().transpose(0, 1)[..., :64]  # a head's tokens side by side
+    assert torch.equal(head_norm_rope(q, q_out=by_head), head_norm_rope(q))
