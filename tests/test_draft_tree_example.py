@@ -106,3 +106,12 @@ def test_training_step(example):
 def test_main(example, capsys):
     example.main()
     assert "accepted path" in capsys.readouterr().out
+
+
+def test_training_gradients_have_no_part_along_their_rows(example):
+    """A norm takes the part along the row out of its gradient, some 1 / sqrt(512) of it, which the bound on the whole
+    gradient lets pass: sum(dx x) is zero but for the rounding of dx."""
+    (q, kv, _, _), _, (dq, dkv, *_) = example.train(example.Layer([70, 33], heads=8, page=16, topk=16, seed=3), n=6)
+    for x, dx in ((q, dq), (kv, dkv)):
+        part = dx.double() * x.double()
+        assert dx.any() and (part.sum(-1).abs() <= U * part.abs().sum(-1)).all()

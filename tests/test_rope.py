@@ -768,3 +768,60 @@ def test_outputs_whose_rows_overlap_are_refused(gpu):
     assert not base.any()
     by_head = torch.zeros(4, 3, 72, device="cuda").bfloat16().transpose(0, 1)[..., :64]  # a head's tokens side by side
     assert torch.equal(head_norm_rope(q, q_out=by_head), head_norm_rope(q))
+
+
+@pytest.mark.gpu
+def test_train_without_keys_matches_backward(gpu):
+    from dsv4_b200 import head_norm_rope_backward, head_norm_rope_train
+
+    q, _, cos, sin, pos, _, _, (dq, _) = _case(12, 4, 0, 64, 32, False, False, torch.bfloat16)
+    q, cos, sin, pos, dq = _cuda(q, cos, sin, pos, dq)
+    ref = head_norm_rope_backward(dq, q, positions=pos, cos=cos, sin=sin)[0]
+    x = q.clone().requires_grad_()
+    head_norm_rope_train(x, positions=pos, cos=cos, sin=sin).backward(dq)
+    assert ref.any() and torch.equal(x.grad, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 512])
+def test_gradient_has_no_part_along_the_row(gpu, D):
+    """The norm does not depend on a row's length, so sum(dx x) is zero (but for eps) where there is no weight: every
+    product is off by the rounding of dx, and the term that the norm's projection takes out is far larger."""
+    from dsv4_b200 import head_norm_rope_backward
+
+    q, _, cos, sin, pos, _, _, (dq, _) = _case(40, 6, 0, D, 32, False, False, torch.bfloat16, seed=9)
+    dev = _cuda(dq, q, pos, cos, sin)
+    dx = head_norm_rope_backward(dev[0], dev[1], positions=dev[2], cos=dev[3], sin=dev[4])[0].double().cpu()
+    x = q.double()
+    dot, mag = (dx * x).sum(-1).abs(), (dx * x).abs().sum(-1)
+    assert (dot <= U[torch.bfloat16] * mag).all()
+    d = definition(dq, None, *_rows(cos, sin, pos), True, norm=False, inverse=True)  # without the projection
+    assert ((d * x).sum(-1).abs() > 4 * U[torch.bfloat16] * (d * x).abs().sum(-1)).double().mean() > 0.5
+
+
+@pytest.mark.gpu
+def test_append_of_padded_bsnd_and_int64_positions(gpu):
+    from dsv4_b200 import append_shared_kv
+
+    close.dtype = torch.bfloat16
+    B, S, D, H = 3, 5, 128, 3
+    lens, ctx = [5, 2, 0], [11, 40, 9]
+    pool, table, used, rows, slots = _paged(lens, ctx, 16, D, torch.bfloat16, 4)
+    g = torch.Generator().manual_seed(4)
+    kv = torch.randn((B, S, 1, D), generator=g).bfloat16()
+    q = torch.randn((B, S, H, D), generator=g).bfloat16()
+    held = torch.tensor([b * S + i for b, n in enumerate(lens) for i in range(n)])
+    cos, sin = tables(64, 64)
+    given = torch.randint(0, 64, (B, S), generator=g)
+    for pos in (None, given):
+        at = slots.long() if pos is None else given.view(-1)[held]
+        dev = pool.cuda()
+        _, yq = append_shared_kv(kv.cuda(), dev, ori_block_table=table.cuda(), seqused_kv=used.cuda(), layout_q="BSND",
+                                 cu_seqlens_q=torch.tensor([0, 5, 7, 7], dtype=torch.int32).cuda(), q=q.cuda(),
+                                 positions=None if pos is None else pos.cuda(), cos=cos.cuda(), sin=sin.cuda())
+        flat = dev.view(-1, 1, D).cpu()
+        close(flat[rows], definition(kv.view(-1, 1, D)[held], None, cos[at], sin[at], True))
+        close(yq.view(-1, H, D)[held.cuda()], definition(q.view(-1, H, D)[held], None, cos[at], sin[at], True))
+        rest = torch.ones(len(flat), dtype=torch.bool)
+        rest[rows] = False
+        assert torch.equal(flat[rest], pool.view(-1, 1, D)[rest])

@@ -486,3 +486,42 @@ def test_writes_are_seen_by_autograd(gpu):
     before = out._version, lse._version
     c.call(out=out, lse_out=lse)
     assert out._version > before[0] and lse._version > before[1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scenario", [2, 3])
+def test_compressed_rows_that_end_in_the_tree(gpu, scenario):
+    """The limit of the compressed rows is ctx // ratio for every token of a tree; a chain of sparse_attn_sharedkv goes to
+    (position + 1) // ratio. The two agree where a chain's list or cache ends with the cached context."""
+    from dsv4_b200 import sparse_attn_sharedkv
+
+    c = Case([6], [802], H=8, scenario=scenario, ratio=4, K=256, trees=[[-1, 0, 1, 2, 3, 4]])
+    full, used = c.cmp.clone(), 808
+    assert 802 // 4 == 200 and (802 + 5 + 1) // 4 == 202
+    if scenario == 3:
+        c.idx[0, 0, :202] = torch.randperm(202, generator=torch.Generator().manual_seed(0)).to(torch.int32)
+        c.idx[1:] = c.idx[0]
+    out, lse = c.call()
+    c.check(out, lse)  # the rows below 200
+    kw = dict(ori_kv=c.ori.cuda(), ori_block_table=c.obt.cuda(), cmp_kv=full.cuda(), cmp_block_table=c.cbt.cuda(), cmp_ratio=4,
+              seqused_kv=torch.tensor([used], dtype=torch.int32).cuda(), sinks=c.sinks.cuda(), softmax_scale=c.scale,
+              cu_seqlens_q=torch.tensor([0, 6], dtype=torch.int32).cuda())
+    if scenario == 3:
+        kw["cmp_sparse_indices"] = torch.where(c.idx < 200, c.idx, -1).sort(-1, descending=True).values.contiguous().cuda()
+    o, l = sparse_attn_sharedkv(c.q.cuda(), return_softmax_lse=True, **kw)
+    if scenario == 3:  # lists of cached rows: the same rows in both
+        c.check(o, l)
+    else:  # the whole cache: the first token sees the same, the last two rows more
+        c.check(o, l, skip=range(1, 6))
+        assert (l[5].cpu() > lse[5].cpu()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [512, 1024])
+def test_long_lists_of_many_requests(gpu, K):
+    r = np.random.default_rng(K)
+    lens = [int(x) for x in r.integers(0, 3, 130)]
+    ctx = [int(x) for x in r.integers(0, 6000, 130)]
+    lens[0], ctx[0] = 3, 6000
+    c = Case(lens, ctx, H=8, scenario=3, K=K)
+    c.check(*c.call())

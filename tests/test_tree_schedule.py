@@ -455,3 +455,13 @@ def test_no_commit_arrives_after_the_pair_left(both):
         m.run()
         found += bool(m.late["qk"] or m.late["pv"])
     assert found == 0 if both else found > 0
+
+
+def test_the_model_has_the_kernels_constants():
+    import os
+    import re
+
+    with open(os.path.join(os.path.dirname(__file__), "..", "dsv4_b200", "csrc", "sas_tree.cu")) as f:
+        source = f.read()
+    const = lambda name: int(re.search(rf"constexpr int (?:[^;]*,\s+)?{name} = (\d+)", source).group(1))  # noqa: E731
+    assert (const("kRing"), const("kUnitSlots"), const("kLoadWarps")) == (RING, UNIT_SLOTS, 4)
