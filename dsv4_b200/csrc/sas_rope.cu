@@ -24,9 +24,9 @@
 // A call with few rows takes short runs, so that they spread over all SMs.
 //
 // Measured (the memory's rate is that of a plain copy, 6.5 TB/s): forward of
-// 16384 tokens x 65 heads x 512 335 us, backward of 8192 tokens 249 us, both at
-// that rate; append of 512 tokens with their 128 query heads 28 us (4.9 TB/s), of
-// 16384 rows alone 15 us (2.5 TB/s), its backward of 8192 rows 16 us (two
+// 16384 tokens x 65 heads x 512 335 us, backward of 8192 tokens 248 us, both at
+// that rate; append of 512 tokens with their 128 query heads 27 us (5.0 TB/s), of
+// 16384 rows alone 14 us (2.7 TB/s), its backward of 8192 rows 16 us (two
 // launches), 64 tokens forward 4.1 us. The calls of under 50 MB are bound by their
 // start and end: launch, first loads, partial sums of the weight gradient.
 #include "sas_common.cuh"

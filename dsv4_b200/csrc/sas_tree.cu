@@ -30,8 +30,10 @@
 // while the unit before it is read.
 // The softmax is one pass with a running maximum that moves, and rescales O,
 // only when a row's maximum rises by more than 2^8: P then stays below 2^8, and
-// P, l and O keep one common scale. P is rounded to the I/O type for the
-// product, l sums it unrounded (as the framework's forward does).
+// P, l and O keep one common scale. P is rounded to the I/O type for the product,
+// whose operands have one type; l sums it unrounded (both as the framework's
+// forward does). It is the one rounding before the result's, and takes the result
+// from 1.7e-3 to 2.1e-3 off the 64-bit one in bf16, 2.1e-4 to 2.6e-4 in fp16 (norms).
 //
 // Roles (23 warps), each of which walks the ring of published tiles by itself:
 //   0-7    softmax: thread = row, 32 of the tile's columns;
@@ -41,15 +43,19 @@
 //   14     coordinator: walks the range and the trees, works out which rows each
 //          token sees and publishes tiles (the pair's two take the same steps);
 //   15-18  copy Q and K, 19-22 V.
-// What bounds it. The products of a tile take 2500 cycles, a tile 5900 (dense: 16
-// trees of 32 tokens x 128 heads over 65k-262k, 165 us, 762 TFLOP/s, 46% of the
-// library's bf16 rate; tensor pipe 38-40% busy): the softmax warps' serial chain
-// per tile, some 400 instructions and 12 round trips to shared memory and barriers
-// between the scores and P. Then the ends of units (window of 127, 64 trees of 16
-// x 64 heads: two tiles a unit, the second nearly empty, 71 us), and about 20 us
-// that a call of any size takes (a single tile through every role and the joining
-// kernel, 21 us). Neither memory (top-k, 64 x 8 x 128 heads, 512 of them: 126 us,
-// 2.1 TB/s, DRAM 31% busy) nor L2 (30%) is near its rate.
+// What bounds it. The products of a tile take 2500 cycles. With about 20 us that a call
+// of any size takes (a single tile through every role and the joining kernel, 21 us)
+// left out, a tile takes 4800 over the whole cache (16 trees of 32 tokens x 128 heads
+// over 65k-262k: 59 tiles a pair, 165 us at 1965 MHz, 762 TFLOP/s, 46% of the
+// library's bf16 rate; tensor pipe 42% busy): the softmax warps' serial chain per
+// tile, some 400 instructions and 12 round trips to shared memory and barriers
+// between the scores and P. With lists it takes 6400 (64 x 8 x 128 heads, 512 of
+// them: 32 tiles a pair, 125 us, 2.1 TB/s, DRAM 31% busy): the same chain, and copies
+// by cp.async in the place of boxes; how much of the difference is theirs was not
+// measured by itself. Window alone (127, 64 trees of 16 x 64 heads: two tiles a unit,
+// the second nearly empty, 70 us): ends of units. Neither memory nor L2 (30%) is near
+// its rate. A chain of drafted tokens costs the coordinator a walk up it for every
+// unit: 8 chains of 1024 x 8 heads take 770 us, where their tiles are worth some 200.
 // Measured and left out: registers moved between warps (setmaxnreg, slower), P
 // before the row's maximum is known and again if it moved (3% slower), output rows
 // stored from registers (slower).

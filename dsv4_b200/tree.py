@@ -57,7 +57,11 @@ def tree_attn_sharedkv(
     and ancestors), to itself, and to compressed rows below ``ctx //
     cmp_ratio``: with ``cmp_kv`` to all of them, with ``cmp_sparse_indices``
     (``[T, 1, K]`` or ``[B, S, 1, K]``) to its list, where ids outside that
-    range are skipped. A KV row with infinities or NaN makes the output of the
+    range are skipped. (A token of ``sparse_attn_sharedkv`` sees those below
+    ``(position + 1) // cmp_ratio``: rows that end among the new tokens too, which
+    a tree's branches would each have their own of. The two are equal for lists of
+    cached rows that end in -1 if they are short, and for tokens with ``(position + 1) // cmp_ratio`` still at
+    ``ctx // cmp_ratio``.) A KV row with infinities or NaN makes the output of the
     tokens that see it NaN, at least in the columns where the row is not
     finite; it reaches no other token. A request of over 1024 tokens,
     with more tokens than ``seqused_kv``, or a token whose parent does not

@@ -9,7 +9,9 @@ ancestors, the window and the compressed cache; ``head_norm_rope`` without the
 norm turns the output back (the cache's rows are turned, and are the values
 too). Once a path of the tree is accepted, its raw rows are appended again, at
 the slots of a chain. What the tree gave for the path is then what
-``sparse_attn_sharedkv`` gives for that chain.
+``sparse_attn_sharedkv`` gives for that chain with the same lists. They hold cached
+rows alone: a compressed row that ends among the drafted tokens is the chain's to
+see, once it is written, and not the tree's.
 
 Training: the same layer on a chain, with the gradients of its raw rows, its
 queries and the norms' weights.
